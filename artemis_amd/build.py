@@ -1,4 +1,5 @@
-"""Build libartemis_synth.so for gfx950 with hipcc (in-tree; cross-compiles without a GPU)."""
+"""Build libartemis_synth.so and libartemis_ops.so for gfx950 with hipcc (in-tree; cross-compiles without a
+GPU)."""
 from __future__ import annotations
 
 import os
@@ -16,6 +17,8 @@ INCLUDE = os.path.join(_ROOT, "include")
 LIB_DIR = os.path.join(_PKG, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libartemis_synth.so")
+OPS_LIB_PATH = os.path.join(LIB_DIR, "libartemis_ops.so")
+OPS_TYPES = ("float", "__bf16", "_Float16")   # ops_attention_type.hip: one object per element type
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -29,13 +32,25 @@ HIPCC_FLAGS = [
     "-Wall",
 ]
 
+# The operators of libartemis_ops.so: no packed fp32 instructions (some of their forms have given wrong results
+# on these machines now and then)
+OPS_FLAGS = HIPCC_FLAGS + ["-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def _stale(path, prefix, header) -> bool:
+    if not os.path.exists(path):
+        return True
+    t = os.path.getmtime(path)
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith(prefix)] + [os.path.join(INCLUDE, header)]
+    return any(os.path.getmtime(d) > t for d in deps)
+
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB_PATH):
-        return True
-    t = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(INCLUDE, "artemis_synth.h")]
-    return any(os.path.getmtime(d) > t for d in deps)
+    return _stale(LIB_PATH, "synth_", "artemis_synth.h")
+
+
+def ops_need_build() -> bool:
+    return _stale(OPS_LIB_PATH, "ops_", "artemis_ops.h")
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
@@ -43,18 +58,34 @@ def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
     translation unit and one object per tile radius in parallel, then one link."""
     if not force and not needs_build():
         return LIB_PATH
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    hipcc = os.environ.get("HIPCC", "hipcc")
     jobs = [(SRC, os.path.join(OBJ_DIR, "synth_kernels.o"), [])]
     jobs += [(TILES_SRC, os.path.join(OBJ_DIR, f"synth_tiles_r{r}.o"), [f"-DSYNTH_TILE_R={r}"])
              for r in TILE_RADII]
     jobs += [(TILES_SRC, os.path.join(OBJ_DIR, f"synth_tiles_r{r}_bf16.o"),
               [f"-DSYNTH_TILE_R={r}", "-DSYNTH_TILE_BF16=1"]) for r in BF16_RADII]
+    return _compile_and_link(jobs, HIPCC_FLAGS, extra_flags, LIB_PATH, verbose)
+
+
+def build_ops(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
+    """The same for artemis_amd/lib/libartemis_ops.so: layer norm, windowed attention (one object per
+    element type), AdamW."""
+    if not force and not ops_need_build():
+        return OPS_LIB_PATH
+    jobs = [(os.path.join(CSRC, f"ops_{n}.hip"), os.path.join(OBJ_DIR, f"ops_{n}.o"), [])
+            for n in ("host", "norm", "adamw", "attention")]
+    jobs += [(os.path.join(CSRC, "ops_attention_type.hip"), os.path.join(OBJ_DIR, f"ops_attention_{t}.o"),
+              [f"-DOPS_TYPE={t}"]) for t in OPS_TYPES]
+    return _compile_and_link(jobs, OPS_FLAGS, extra_flags, OPS_LIB_PATH, verbose)
+
+
+def _compile_and_link(jobs, flags, extra_flags, lib_path, verbose) -> str:
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    hipcc = os.environ.get("HIPCC", "hipcc")
     workers = max(1, min(len(jobs), int(os.environ.get("MAX_JOBS", os.cpu_count() or 1))))
 
     def compile_one(job):
         src, obj, defs = job
-        cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, *defs, "-I" + INCLUDE, "-c", "-o", obj, src]
+        cmd = [hipcc, *flags, *extra_flags, *defs, "-I" + INCLUDE, "-c", "-o", obj, src]
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -64,14 +95,15 @@ def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(workers) as pool:
         list(pool.map(compile_one, jobs))
-    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + [j[1] for j in jobs]
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib_path] + [j[1] for j in jobs]
     if verbose:
         print(" ".join(link))
     r = subprocess.run(link, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stderr)
-    return LIB_PATH
+    return lib_path
 
 
 if __name__ == "__main__":
+    print(build_ops(force=True, verbose=True))
     print(build(force=True, verbose=True))

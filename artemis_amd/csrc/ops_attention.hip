@@ -1,0 +1,303 @@
+// ops_attention.hip -- C ABI of the windowed attention: checks, workspace, and the kernels that do not depend on the
+// element type.
+#include "ops_attention.hpp"
+
+namespace aops {
+namespace {
+
+// by_head[head][entry] = table[entry][head] * log2(e)
+__global__ void bias_rows(const float *__restrict__ table, float *__restrict__ by_head, int entries, int heads)
+{
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < entries * heads) by_head[(size_t)(i % heads) * entries + i / heads] = table[i] * kLog2e;
+}
+
+// dense[head][e] = the sum of the shares of the workgroups that have that head, in a fixed order: 16 elements for a
+// workgroup, 16 threads on each
+__global__ __launch_bounds__(256) void pairs_fold(const float *__restrict__ pairs, float *__restrict__ dense, int heads,
+                                                  int groups, int elements)
+{
+    __shared__ float fold[16][17];
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int head = blockIdx.y, e = blockIdx.x * 16 + tx;
+    // workgroup b has head b / 8 % heads (walk_of): the k-th of a head's is ((k / 8) * heads + head) * 8 + k % 8
+    const int mine = groups / heads;
+    float s = 0.f;
+    for (int k = ty; k < mine; k += 16)
+        s += pairs[(size_t)(((k / 8) * heads + head) * 8 + k % 8) * elements + e];
+    fold[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0) {
+        float t = 0.f;
+        for (int k = 0; k < 16; ++k) t += fold[k][tx];
+        dense[(size_t)head * elements + e] = t;
+    }
+}
+
+// dtable[e][head]: a wave sums the pairs of entry e, queries in its lanes.  `dense` is [head][slots][width]; a window's tokens start
+// at `pitch * i` for i < copies (small windows share 16 slots), and block-diagonal units start every 16 * nb slots.
+__global__ __launch_bounds__(256) void table_small(const WindowArgs a, const float *__restrict__ dense,
+                                                   float *__restrict__ dtable, int nb)
+{
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int e = blockIdx.x * 4 + wave, head = blockIdx.y;
+    if (e >= a.entries) return;
+    const int dw = e % a.rh - (a.ww - 1), dh = e / a.rh % (2 * a.wh - 1) - (a.wh - 1), dd = e / a.rd - (a.wd - 1);
+    const int fit = nb == 1 ? 16 / a.n : 1;
+    const int r = lane % (16 * nb);
+    float s = 0.f;
+    if (r < fit * a.n) {
+        const int t = r % a.n;
+        const int tw = t % a.ww - dw, th = t / a.ww % a.wh - dh, td = t / a.ww / a.wh - dd;
+        if (tw >= 0 && tw < a.ww && th >= 0 && th < a.wh && td >= 0 && td < a.wd) {
+            const int key = r / a.n * a.n + (td * a.wh + th) * a.ww + tw;
+            s = dense[((size_t)head * 64 + lane) * 16 * nb + key];
+        }
+    }
+    s = group_sum<64>(s);
+    if (lane == 0) dtable[(size_t)e * a.heads + head] = s;
+}
+
+// dtable[e][head] for long windows: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
+// lane has one dw, so that neighbouring lanes read neighbouring keys.  Four waves take every fourth row.
+__global__ __launch_bounds__(256) void table_long(const WindowArgs a, const float *__restrict__ dense,
+                                                  float *__restrict__ dtable)
+{
+    __shared__ float fold[4][64];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int head = blockIdx.z;
+    const int dh = (int)blockIdx.y % (2 * a.wh - 1) - (a.wh - 1), dd = (int)blockIdx.y / (2 * a.wh - 1) - (a.wd - 1);
+    const int e = blockIdx.x * 64 + lane, dw = e - (a.ww - 1);
+    float s = 0.f;
+    const int rows = a.wd * a.wh;
+    for (int row = wave; row < rows; row += 4) {
+        const int qd = row / a.wh, qh = row % a.wh, kd = qd - dd, kh = qh - dh;
+        if (kd < 0 || kd >= a.wd || kh < 0 || kh >= a.wh) continue;
+        const float *line = dense + ((size_t)head * a.n + (size_t)row * a.ww) * a.n + (kd * a.wh + kh) * a.ww - dw;
+        const int lo = dw > 0 ? dw : 0, hi = dw < 0 ? a.ww + dw : a.ww;  // queries whose key is in the row
+        if (e < a.rh)
+            for (int qw = lo; qw < hi; ++qw) s += line[(size_t)qw * a.n + qw];
+    }
+    fold[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && e < a.rh)
+        dtable[((size_t)blockIdx.y * a.rh + e) * a.heads + head] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
+}
+
+__global__ void fill_zero(float *p, long long n)
+{
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) p[i] = 0.f;
+}
+
+int small_nb(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
+
+// Workgroups for windows of at most 64 tokens: a multiple of 8 * heads (walk_of), about `target`, at most one for
+// each (tile, head).
+int small_groups(const WindowArgs &a, int target)
+{
+    const int nb = small_nb(a.n);
+    const int per = 4 / nb * (nb == 1 ? 16 / a.n : 1);
+    const long long tiles = (a.windows + per - 1) / per;
+    const long long most = (tiles + 7) / 8;           // times 8 * heads
+    long long want = target / (8LL * a.heads);
+    if (want < 1) want = 1;
+    return (int)((want < most ? want : most) * 8 * a.heads);
+}
+int fwd_groups(const WindowArgs &a) { return small_groups(a, 2048); }
+int bwd_groups(const WindowArgs &a) { return small_groups(a, 1024); }
+
+size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+// 0 ok, > 0 invalid, -1 nothing to do
+int make_args(const char *what, const artemis_ops_window *w, WindowArgs &a)
+{
+    if (!w) return fail(hipErrorInvalidValue, "%s: NULL description", what);
+    if (w->B < 0 || w->D < 0 || w->H < 0 || w->W < 0)
+        return fail(hipErrorInvalidValue, "%s: negative dimension B=%d D=%d H=%d W=%d", what, w->B, w->D, w->H, w->W);
+    if (w->dtype != ARTEMIS_OPS_F32 && w->dtype != ARTEMIS_OPS_BF16 && w->dtype != ARTEMIS_OPS_F16)
+        return fail(hipErrorInvalidValue, "%s: unknown dtype %d", what, w->dtype);
+    if (w->heads < 1 || w->heads > 1024 || w->head_dim < 4 || w->head_dim > 128 || w->head_dim % 4)
+        return fail(hipErrorInvalidValue, "%s: heads=%d head_dim=%d (heads 1..1024, head_dim a multiple of 4 up to 128)",
+                    what, w->heads, w->head_dim);
+    if (w->wd < 1 || w->wh < 1 || w->ww < 1 || w->wd > 4096 || w->wh > 4096 || w->ww > 4096 ||
+        (long long)w->wd * w->wh * w->ww > 4096)
+        return fail(hipErrorInvalidValue, "%s: window (%d, %d, %d) must hold 1..4096 tokens", what, w->wd, w->wh, w->ww);
+    if (w->D % w->wd || w->H % w->wh || w->W % w->ww)
+        return fail(hipErrorInvalidValue, "%s: map (%d, %d, %d) is not a multiple of the window (%d, %d, %d)", what, w->D,
+                    w->H, w->W, w->wd, w->wh, w->ww);
+    if (w->shift_d < 0 || w->shift_d >= w->wd || w->shift_h < 0 || w->shift_h >= w->wh || w->shift_w < 0 ||
+        w->shift_w >= w->ww)
+        return fail(hipErrorInvalidValue, "%s: shift (%d, %d, %d) must lie in [0, window)", what, w->shift_d, w->shift_h,
+                    w->shift_w);
+    if (w->label_maps < 0 || (w->label_maps > 1 && w->label_maps != w->B))
+        return fail(hipErrorInvalidValue, "%s: label_maps=%d must be 0, 1 or B", what, w->label_maps);
+    if (!(w->outside <= 0.f)) return fail(hipErrorInvalidValue, "%s: outside=%g must be <= 0", what, w->outside);
+    if (!(fabsf(w->scale) <= 3.4e38f)) return fail(hipErrorInvalidValue, "%s: scale must be finite", what);
+    const double tokens = (double)w->B * w->D * w->H * w->W;
+    const int n = w->wd * w->wh * w->ww;
+    if (tokens >= 2147483648.0 || tokens / n * w->heads * ((n + 63) / 64) >= 16777216.0 * 64 ||
+        (n > 64 && tokens / n * w->heads * ((n + 63) / 64) >= 16777216.0))
+        return fail(hipErrorInvalidValue, "%s: too many tokens or windows * heads", what);
+    a = WindowArgs{w->B, w->D, w->H, w->W, w->heads, w->head_dim, w->wd, w->wh, w->ww, n, w->shift_d, w->shift_h,
+                   w->shift_w, w->D / w->wd, w->H / w->wh, w->W / w->ww, w->label_maps, (2 * w->wh - 1) * (2 * w->ww - 1),
+                   2 * w->ww - 1, (2 * w->wd - 1) * (2 * w->wh - 1) * (2 * w->ww - 1), 0, w->scale, 0.f};
+    a.windows = (long long)w->B * a.nd * a.nh * a.nw;
+    // a finite `outside` stays finite in the exponent of 2; beyond -1e30 nothing else counts beside it anyway
+    a.outside2 = w->outside == -INFINITY ? -INFINITY : (w->outside < -1e30f ? -1e30f : w->outside) * kLog2e;
+    return a.windows == 0 ? -1 : 0;
+}
+
+struct Layout {
+    size_t bias, pairs, dense, delta, total;
+};
+Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool table)
+{
+    Layout l{};
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += round16(bytes);
+        return here;
+    };
+    const bool is_long = a.n > 64;
+    const int nb = small_nb(a.n);
+    if (is_long && table) l.bias = take((size_t)a.entries * a.heads * 4);
+    if (backward && is_long) l.delta = take((size_t)a.windows * a.heads * a.n * 4);
+    if (backward && need_dtable) {
+        if (is_long) {
+            l.dense = take((size_t)a.heads * a.n * a.n * 4);
+        } else {
+            l.pairs = take((size_t)bwd_groups(a) * 64 * 16 * nb * 4);
+            l.dense = take((size_t)a.heads * 64 * 16 * nb * 4);
+        }
+    }
+    l.total = at;
+    return l;
+}
+
+bool aligned4(const void *p, int dtype) { return ((size_t)p & (dtype == ARTEMIS_OPS_F32 ? 15 : 7)) == 0; }
+
+int rows_of_bias(const WindowArgs &a, const float *table, float *by_head, hipStream_t st)
+{
+    const int n = a.entries * a.heads;
+    hipLaunchKernelGGL(bias_rows, dim3((n + 255) / 256), dim3(256), 0, st, table, by_head, a.entries, a.heads);
+    return 0;
+}
+
+}  // namespace
+}  // namespace aops
+
+using namespace aops;
+
+extern "C" {
+
+size_t artemis_ops_window_attention_lse_count(const artemis_ops_window *w)
+{
+    WindowArgs a;
+    if (make_args("artemis_ops_window_attention", w, a)) return 0;
+    return a.n > 64 ? (size_t)a.windows * a.heads * a.n : 0;
+}
+
+size_t artemis_ops_window_attention_workspace_bytes(const artemis_ops_window *w, int backward, int need_dtable)
+{
+    WindowArgs a;
+    if (make_args("artemis_ops_window_attention", w, a)) return 0;
+    return layout_of(a, backward != 0, need_dtable != 0, true).total;
+}
+
+int artemis_ops_window_attention_forward(const artemis_ops_window *w, const void *qkv, const float *table,
+                                         const int *labels, void *out, float *lse, void *workspace,
+                                         size_t workspace_bytes, void *stream)
+{
+    const char *what = "artemis_ops_window_attention_forward";
+    WindowArgs a;
+    if (const int rc = make_args(what, w, a)) return rc > 0 ? rc : 0;
+    if (!qkv || !out) return fail(hipErrorInvalidValue, "%s: NULL tensor pointer", what);
+    if (!labels != !w->label_maps) return fail(hipErrorInvalidValue, "%s: labels and label_maps do not match", what);
+    if (!aligned4(qkv, w->dtype) || !aligned4(out, w->dtype))
+        return fail(hipErrorInvalidValue, "%s: tensors must be aligned to 4 elements", what);
+    const Layout l = layout_of(a, false, false, table != nullptr);
+    if (l.total && (!workspace || workspace_bytes < l.total || ((size_t)workspace & 15)))
+        return fail(hipErrorInvalidValue, "%s: workspace of %zu bytes aligned to 16 needed", what, l.total);
+    hipStream_t st = (hipStream_t)stream;
+    AttnBuffers b{};
+    b.qkv = qkv;
+    b.table = table;
+    b.labels = labels;
+    b.out = out;
+    b.lse = lse;
+    b.groups = a.n <= 64 ? fwd_groups(a) : 0;
+    if (a.n > 64 && table) {
+        b.bias_by_head = (float *)((char *)workspace + l.bias);
+        rows_of_bias(a, table, (float *)((char *)workspace + l.bias), st);
+    }
+    if (w->dtype == ARTEMIS_OPS_F32)
+        launch_attention_fwd<float>(a, b, st);
+    else if (w->dtype == ARTEMIS_OPS_BF16)
+        launch_attention_fwd<__bf16>(a, b, st);
+    else
+        launch_attention_fwd<_Float16>(a, b, st);
+    return check_launch(what);
+}
+
+int artemis_ops_window_attention_backward(const artemis_ops_window *w, const void *qkv, const float *table,
+                                          const int *labels, const void *out, const float *lse, const void *dout,
+                                          void *dqkv, float *dtable, void *workspace, size_t workspace_bytes,
+                                          void *stream)
+{
+    const char *what = "artemis_ops_window_attention_backward";
+    WindowArgs a;
+    const int made = make_args(what, w, a);
+    if (made > 0) return made;
+    hipStream_t st = (hipStream_t)stream;
+    if (made < 0) {  // no tokens: the table's gradient is a sum over nothing
+        if (dtable) hipLaunchKernelGGL(fill_zero, dim3(64), dim3(256), 0, st, dtable, (long long)a.entries * a.heads);
+        return check_launch(what);
+    }
+    const bool is_long = a.n > 64;
+    if (!qkv || !dout || !dqkv || (is_long && (!out || !lse)))
+        return fail(hipErrorInvalidValue, "%s: NULL tensor pointer", what);
+    if (!labels != !w->label_maps) return fail(hipErrorInvalidValue, "%s: labels and label_maps do not match", what);
+    if (!aligned4(qkv, w->dtype) || !aligned4(out, w->dtype) || !aligned4(dout, w->dtype) || !aligned4(dqkv, w->dtype))
+        return fail(hipErrorInvalidValue, "%s: tensors must be aligned to 4 elements", what);
+    const Layout l = layout_of(a, true, dtable != nullptr, table != nullptr);
+    if (l.total && (!workspace || workspace_bytes < l.total || ((size_t)workspace & 15)))
+        return fail(hipErrorInvalidValue, "%s: workspace of %zu bytes aligned to 16 needed", what, l.total);
+    char *ws = (char *)workspace;
+    AttnBuffers b{};
+    b.qkv = qkv;
+    b.table = table;
+    b.labels = labels;
+    b.out_in = out;
+    b.lse = (float *)lse;
+    b.dout = dout;
+    b.dqkv = dqkv;
+    b.groups = is_long ? 0 : bwd_groups(a);
+    if (is_long) b.delta = (float *)(ws + l.delta);
+    if (dtable) {
+        b.dense = (float *)(ws + l.dense);
+        if (!is_long) b.pairs = (float *)(ws + l.pairs);
+    }
+    if (is_long && table) {
+        b.bias_by_head = (float *)(ws + l.bias);
+        rows_of_bias(a, table, (float *)(ws + l.bias), st);
+    }
+    if (w->dtype == ARTEMIS_OPS_F32)
+        launch_attention_bwd<float>(a, b, st);
+    else if (w->dtype == ARTEMIS_OPS_BF16)
+        launch_attention_bwd<__bf16>(a, b, st);
+    else
+        launch_attention_bwd<_Float16>(a, b, st);
+    if (dtable && is_long) {
+        hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st,
+                           a, b.dense, dtable);
+    } else if (dtable) {
+        const int nb = small_nb(a.n), elements = 64 * 16 * nb;
+        hipLaunchKernelGGL(pairs_fold, dim3(elements / 16, a.heads), dim3(256), 0, st, b.pairs, b.dense, a.heads, b.groups,
+                           elements);
+        hipLaunchKernelGGL(table_small, dim3((a.entries + 3) / 4, a.heads), dim3(256), 0, st, a, b.dense, dtable, nb);
+    }
+    return check_launch(what);
+}
+
+}  // extern "C"

@@ -1,0 +1,446 @@
+// ops_norm.hip -- layer norm over the last dimension, forward and backward.
+//
+//   y  = (x - mean) rstd w + b                        rstd = (var + eps)^-1/2
+//   dx = rstd (a - mean(a) - xh mean(a xh))           a = dy w, xh = (x - mean) rstd
+//   dw = sum over rows of dy xh,  db = sum of dy
+//
+// Both passes are bound by memory: 2 (forward) and 4 (whole training pass: x, dy in, y, dx out) values moved
+// for each element, a few operations on each.  A row is therefore read once and stays in registers: L lanes of
+// a wave hold it, NV vectors of 16 bytes each.  The variance is the mean of squared deviations from the mean
+// in the registers, not E[x^2] - mean^2, which cancels for features far from zero.
+// The weight's gradient is summed over the rows that a workgroup meets in registers, then over its row
+// groups through LDS in a fixed order, then over the workgroups by a second kernel: no atomics, so every run
+// gives the same bits.
+#include "ops_common.hpp"
+
+namespace aops {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Rows of `cols` elements as NV vectors of VEC elements in each of L lanes; lane i holds the vectors i, i + L, ...
+template <class T, int VEC, int L, int NV>
+__global__ __launch_bounds__(kThreads) void norm_fwd(const T *__restrict__ x, const float *__restrict__ w,
+                                                     const float *__restrict__ b, T *__restrict__ y,
+                                                     float *__restrict__ mean_out, float *__restrict__ rstd_out,
+                                                     long long rows, int cols, float eps)
+{
+    const int lane = threadIdx.x % L;
+    const int nvec = cols / VEC;
+    const float inv = 1.0f / (float)cols;
+    // (whole groups of L lanes leave the loop together: the sums below stay within a group)
+    for (long long row = (long long)blockIdx.x * (kThreads / L) + threadIdx.x / L; row < rows;
+         row += (long long)gridDim.x * (kThreads / L)) {
+    const Vec<T, VEC> *xr = (const Vec<T, VEC> *)(x + row * cols);
+    float xv[NV][VEC];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = lane + i * L;
+        Vec<T, VEC> t{};
+        if (j < nvec) t = xr[j];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            xv[i][e] = to_f32(t.v[e]);
+            s += xv[i][e];
+        }
+    }
+    const float mean = group_sum<L>(s) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (lane + i * L < nvec)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                xv[i][e] -= mean;
+                q += xv[i][e] * xv[i][e];
+            }
+    const float rstd = 1.0f / sqrtf(group_sum<L>(q) * inv + eps);
+    if (lane == 0 && mean_out) {
+        mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+    Vec<T, VEC> *yr = (Vec<T, VEC> *)(y + row * cols);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = lane + i * L;
+        if (j >= nvec) continue;
+        Vec<T, VEC> t;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float v = xv[i][e] * rstd;
+            if (w) v *= w[j * VEC + e];
+            if (b) v += b[j * VEC + e];
+            t.v[e] = from_f32<T>(v);
+        }
+        yr[j] = t;
+    }
+    }
+}
+
+// One workgroup for a row of any width: three passes over it, the later two from the caches.
+template <class T>
+__global__ __launch_bounds__(kThreads) void norm_fwd_wide(const T *__restrict__ x, const float *__restrict__ w,
+                                                          const float *__restrict__ b, T *__restrict__ y,
+                                                          float *__restrict__ mean_out,
+                                                          float *__restrict__ rstd_out, long long rows, int cols,
+                                                          float eps)
+{
+    __shared__ float part[2][kThreads / 64];
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T *xr = x + row * cols;
+    T *yr = y + row * cols;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < cols; c += kThreads) s += to_f32(xr[c]);
+    s = group_sum<64>(s);
+    if (threadIdx.x % 64 == 0) part[0][threadIdx.x / 64] = s;  // (the row before read it in front of its 2nd barrier)
+    __syncthreads();
+    const float mean = (part[0][0] + part[0][1] + part[0][2] + part[0][3]) / (float)cols;
+    float q = 0.f;
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+        const float d = to_f32(xr[c]) - mean;
+        q += d * d;
+    }
+    q = group_sum<64>(q);
+    if (threadIdx.x % 64 == 0) part[1][threadIdx.x / 64] = q;
+    __syncthreads();
+    const float rstd = 1.0f / sqrtf((part[1][0] + part[1][1] + part[1][2] + part[1][3]) / (float)cols + eps);
+    if (threadIdx.x == 0 && mean_out) {
+        mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+        float v = (to_f32(xr[c]) - mean) * rstd;
+        if (w) v *= w[c];
+        if (b) v += b[c];
+        yr[c] = from_f32<T>(v);
+    }
+    __syncthreads();  // part[1] has been read
+    }
+}
+
+// partial (gridDim.x, 2, cols): this workgroup's share of dw and db; NULL: not asked for
+template <class T, int VEC, int L, int NV>
+__global__ __launch_bounds__(kThreads) void norm_bwd(const T *__restrict__ x, const T *__restrict__ dy,
+                                                     const float *__restrict__ w,
+                                                     const float *__restrict__ mean_in,
+                                                     const float *__restrict__ rstd_in, T *__restrict__ dx,
+                                                     float *__restrict__ partial, long long rows, int cols)
+{
+    constexpr int G = kThreads / L;  // row groups of a workgroup
+    __shared__ float fold[G * L * NV * VEC];
+    const int lane = threadIdx.x % L, group = threadIdx.x / L;
+    const int nvec = cols / VEC;
+    const float inv = 1.0f / (float)cols;
+    float wv[NV][VEC], dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int c = (lane + i * L) * VEC + e;
+            wv[i][e] = c < cols && w ? w[c] : 1.0f;
+            dw[i][e] = db[i][e] = 0.f;
+        }
+    for (long long row = (long long)blockIdx.x * G + group; row < rows; row += (long long)gridDim.x * G) {
+        const Vec<T, VEC> *xr = (const Vec<T, VEC> *)(x + row * cols);
+        const Vec<T, VEC> *gr = (const Vec<T, VEC> *)(dy + row * cols);
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        float xh[NV][VEC], a[NV][VEC];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = lane + i * L;
+            const bool in = j < nvec;
+            Vec<T, VEC> tx{}, tg{};
+            if (in) {
+                tx = xr[j];
+                tg = gr[j];
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float g = to_f32(tg.v[e]);
+                xh[i][e] = in ? (to_f32(tx.v[e]) - mean) * rstd : 0.f;
+                a[i][e] = g * wv[i][e];
+                s1 += a[i][e];
+                s2 += a[i][e] * xh[i][e];
+                dw[i][e] += g * xh[i][e];
+                db[i][e] += g;
+            }
+        }
+        if (!dx) continue;
+        const float m1 = group_sum<L>(s1) * inv, m2 = group_sum<L>(s2) * inv;
+        Vec<T, VEC> *dr = (Vec<T, VEC> *)(dx + row * cols);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = lane + i * L;
+            if (j >= nvec) continue;
+            Vec<T, VEC> t;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t.v[e] = from_f32<T>(rstd * (a[i][e] - m1 - xh[i][e] * m2));
+            dr[j] = t;
+        }
+    }
+    if (!partial) return;
+    float *out = partial + (size_t)blockIdx.x * 2 * cols;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                fold[group * (L * NV * VEC) + (lane + i * L) * VEC + e] = which ? db[i][e] : dw[i][e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += kThreads) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < G; ++k) s += fold[k * (L * NV * VEC) + c];
+            out[which * cols + c] = s;
+        }
+    }
+}
+
+// Wide rows: a workgroup takes rows blockIdx.x, blockIdx.x + gridDim.x, ...; its columns' sums for dw and db
+// stay in the partial buffer, where every thread adds to its own columns only.
+template <class T>
+__global__ __launch_bounds__(kThreads) void norm_bwd_wide(const T *__restrict__ x, const T *__restrict__ dy,
+                                                          const float *__restrict__ w,
+                                                          const float *__restrict__ mean_in,
+                                                          const float *__restrict__ rstd_in, T *__restrict__ dx,
+                                                          float *__restrict__ partial, long long rows, int cols)
+{
+    __shared__ float part[2][kThreads / 64];
+    float *out = partial ? partial + (size_t)blockIdx.x * 2 * cols : nullptr;
+    bool first = true;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T *xr = x + row * cols, *gr = dy + row * cols;
+        const float mean = mean_in[row], rstd = rstd_in[row];
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x; c < cols; c += kThreads) {
+            const float g = to_f32(gr[c]), xh = (to_f32(xr[c]) - mean) * rstd;
+            const float a = w ? g * w[c] : g;
+            s1 += a;
+            s2 += a * xh;
+            if (out) {
+                out[c] = first ? g * xh : out[c] + g * xh;
+                out[cols + c] = first ? g : out[cols + c] + g;
+            }
+        }
+        first = false;
+        if (!dx) continue;
+        s1 = group_sum<64>(s1);
+        s2 = group_sum<64>(s2);
+        __syncthreads();  // the row before has been read
+        if (threadIdx.x % 64 == 0) {
+            part[0][threadIdx.x / 64] = s1;
+            part[1][threadIdx.x / 64] = s2;
+        }
+        __syncthreads();
+        const float m1 = (part[0][0] + part[0][1] + part[0][2] + part[0][3]) / (float)cols;
+        const float m2 = (part[1][0] + part[1][1] + part[1][2] + part[1][3]) / (float)cols;
+        T *dr = dx + row * cols;
+        for (int c = threadIdx.x; c < cols; c += kThreads) {
+            const float xh = (to_f32(xr[c]) - mean) * rstd;
+            const float a = w ? to_f32(gr[c]) * w[c] : to_f32(gr[c]);
+            dr[c] = from_f32<T>(rstd * (a - m1 - xh * m2));
+        }
+    }
+}
+
+// dw and db from the workgroups' shares: 16 columns for a workgroup, 16 threads on each, joined in order.
+__global__ __launch_bounds__(kThreads) void norm_fold(const float *__restrict__ partial, float *__restrict__ dw,
+                                                      float *__restrict__ db, int parts, int cols)
+{
+    __shared__ float fold[16][17];
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const long long c = (long long)blockIdx.x * 16 + tx;  // of 2 * cols
+    float s = 0.f;
+    if (c < 2LL * cols)
+        for (int p = ty; p < parts; p += 16) s += partial[(size_t)p * 2 * cols + c];
+    fold[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < 2LL * cols) {
+        float t = 0.f;
+        for (int k = 0; k < 16; ++k) t += fold[k][tx];
+        if (c < cols) {
+            if (dw) dw[c] = t;
+        } else if (db) {
+            db[c - cols] = t;
+        }
+    }
+}
+
+// How a row is held: `vec` elements for a vector, `lanes` lanes, `nv` vectors in each; lanes = 0: a workgroup
+// for a row.  Vectors of 16 bytes where rows and pointers allow them, single elements otherwise; as few lanes
+// as hold a row, so that a wave takes several narrow rows.
+struct Shape {
+    int vec, lanes, nv;
+};
+
+int element_size(int dtype) { return dtype == ARTEMIS_OPS_F32 ? 4 : 2; }
+
+Shape shape_for(long long cols, int dtype, bool aligned)
+{
+    const int wide = 16 / element_size(dtype);
+    const int vec = aligned && cols % wide == 0 ? wide : 1;
+    const long long nvec = cols / vec;
+    if (nvec <= 64) {
+        int lanes = 8;
+        while (lanes < nvec) lanes *= 2;
+        return {vec, lanes, 1};
+    }
+    const int most = vec == 1 ? 16 : 8;
+    for (int nv = 2; nv <= most; nv *= 2)
+        if (nvec <= 64LL * nv) return {vec, 64, nv};
+    return {1, 0, 0};
+}
+
+// Workgroups of the backward pass: enough to fill 256 CUs several times over, no more than there are rows
+// for, since each writes a share of dw and db.
+long long bwd_blocks(long long rows, int rows_at_once)
+{
+    const long long need = (rows + rows_at_once - 1) / rows_at_once;
+    return need < 1024 ? need : 1024;
+}
+
+// a workgroup for each group of rows, up to a launch's 2^32 threads
+unsigned fwd_blocks(long long rows, int rows_at_once)
+{
+    const long long need = (rows + rows_at_once - 1) / rows_at_once;
+    return (unsigned)(need < (1 << 22) ? need : (1 << 22));
+}
+
+bool aligned16(const void *p) { return ((size_t)p & 15) == 0; }
+
+template <class T, class F>
+bool with_shape(const Shape &s, F f)
+{
+    constexpr int W = 16 / (int)sizeof(T);
+    using std::integral_constant;
+#define ARTEMIS_CASE(V, L, N)                                                                                   \
+    if (s.vec == V && s.lanes == L && s.nv == N) {                                                              \
+        f(integral_constant<int, V>{}, integral_constant<int, L>{}, integral_constant<int, N>{});              \
+        return true;                                                                                            \
+    }
+#define ARTEMIS_CASES(V)                                                                                        \
+    ARTEMIS_CASE(V, 8, 1)                                                                                       \
+    ARTEMIS_CASE(V, 16, 1) ARTEMIS_CASE(V, 32, 1) ARTEMIS_CASE(V, 64, 1) ARTEMIS_CASE(V, 64, 2)                 \
+    ARTEMIS_CASE(V, 64, 4) ARTEMIS_CASE(V, 64, 8)
+    ARTEMIS_CASES(W)
+    ARTEMIS_CASES(1)
+    ARTEMIS_CASE(1, 64, 16)
+#undef ARTEMIS_CASES
+#undef ARTEMIS_CASE
+    return false;
+}
+
+template <class T>
+int run_fwd(const void *x, const float *w, const float *b, void *y, float *mean, float *rstd, long long rows,
+            int cols, float eps, int dtype, hipStream_t st)
+{
+    const Shape s = shape_for(cols, dtype, aligned16(x) && aligned16(y));
+    if (!with_shape<T>(s, [&](auto V, auto L, auto N) {
+            hipLaunchKernelGGL((norm_fwd<T, V, L, N>), dim3(fwd_blocks(rows, kThreads / L)), dim3(kThreads), 0, st, (const T *)x, w, b,
+                               (T *)y, mean, rstd, rows, cols, eps);
+        }))
+        hipLaunchKernelGGL((norm_fwd_wide<T>), dim3(fwd_blocks(rows, 1)), dim3(kThreads), 0, st, (const T *)x, w, b,
+                           (T *)y, mean, rstd, rows, cols, eps);
+    return check_launch("artemis_ops_layer_norm_forward");
+}
+
+template <class T>
+int run_bwd(const void *x, const void *dy, const float *w, const float *mean, const float *rstd, void *dx,
+            float *dw, float *db, long long rows, int cols, int dtype, float *partial, hipStream_t st)
+{
+    const Shape s = shape_for(cols, dtype, aligned16(x) && aligned16(dy) && aligned16(dx));
+    const int parts = (int)bwd_blocks(rows, s.lanes ? kThreads / s.lanes : 1);
+    if (!with_shape<T>(s, [&](auto V, auto L, auto N) {
+            hipLaunchKernelGGL((norm_bwd<T, V, L, N>), dim3(parts), dim3(kThreads), 0, st, (const T *)x,
+                               (const T *)dy, w, mean, rstd, (T *)dx, partial, rows, cols);
+        }))
+        hipLaunchKernelGGL((norm_bwd_wide<T>), dim3(parts), dim3(kThreads), 0, st, (const T *)x, (const T *)dy, w,
+                           mean, rstd, (T *)dx, partial, rows, cols);
+    if (partial)
+        hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2LL * cols + 15) / 16)), dim3(kThreads), 0, st, partial,
+                           dw, db, parts, cols);
+    return check_launch("artemis_ops_layer_norm_backward");
+}
+
+int check_sizes(const char *what, long long rows, long long cols, int dtype)
+{
+    if (rows < 0 || cols < 0 || rows >= (1LL << 31) || cols >= (1LL << 30))
+        return fail(hipErrorInvalidValue, "%s: %lld rows of %lld columns (0 <= rows < 2^31, 0 <= cols < 2^30)",
+                    what, rows, cols);
+    if (rows > 0 && cols == 0) return fail(hipErrorInvalidValue, "%s: rows without columns", what);
+    if (dtype != ARTEMIS_OPS_F32 && dtype != ARTEMIS_OPS_BF16 && dtype != ARTEMIS_OPS_F16)
+        return fail(hipErrorInvalidValue, "%s: unknown dtype %d", what, dtype);
+    return 0;
+}
+
+}  // namespace
+}  // namespace aops
+
+using namespace aops;
+
+extern "C" {
+
+int artemis_ops_layer_norm_forward(const void *x, const float *weight, const float *bias, void *y, float *mean,
+                                   float *rstd, long long rows, long long cols, float eps, int dtype,
+                                   void *stream)
+{
+    const char *what = "artemis_ops_layer_norm_forward";
+    if (int rc = check_sizes(what, rows, cols, dtype)) return rc;
+    if (rows == 0) return 0;
+    if (!x || !y) return fail(hipErrorInvalidValue, "%s: NULL tensor pointer", what);
+    if (!mean != !rstd) return fail(hipErrorInvalidValue, "%s: mean and rstd are written together", what);
+    if (!(eps >= 0.f)) return fail(hipErrorInvalidValue, "%s: eps must be >= 0", what);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == ARTEMIS_OPS_F32) return run_fwd<float>(x, weight, bias, y, mean, rstd, rows, (int)cols, eps, dtype, st);
+    if (dtype == ARTEMIS_OPS_BF16)
+        return run_fwd<__bf16>(x, weight, bias, y, mean, rstd, rows, (int)cols, eps, dtype, st);
+    return run_fwd<_Float16>(x, weight, bias, y, mean, rstd, rows, (int)cols, eps, dtype, st);
+}
+
+size_t artemis_ops_layer_norm_workspace_bytes(long long rows, long long cols, int dtype)
+{
+    if (rows < 0 || cols <= 0 || dtype < 0 || dtype > ARTEMIS_OPS_F16) return 0;
+    // as many shares as either way of holding a row makes: the pointers' alignment is not known here
+    long long most = 1;
+    for (int aligned = 0; aligned < 2; ++aligned) {
+        const Shape s = shape_for(cols, dtype, aligned != 0);
+        const long long n = bwd_blocks(rows, s.lanes ? kThreads / s.lanes : 1);
+        most = n > most ? n : most;
+    }
+    return (size_t)most * 2 * (size_t)cols * sizeof(float);
+}
+
+int artemis_ops_layer_norm_backward(const void *x, const void *dy, const float *weight, const float *mean,
+                                    const float *rstd, void *dx, float *dweight, float *dbias, long long rows,
+                                    long long cols, int dtype, void *workspace, size_t workspace_bytes,
+                                    void *stream)
+{
+    const char *what = "artemis_ops_layer_norm_backward";
+    if (int rc = check_sizes(what, rows, cols, dtype)) return rc;
+    if (cols == 0 || (!dx && !dweight && !dbias)) return 0;
+    hipStream_t st = (hipStream_t)stream;
+    const bool sums = dweight || dbias;
+    if (rows == 0) {  // sums over nothing
+        if (sums)
+            hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2 * cols + 15) / 16)), dim3(kThreads), 0, st,
+                               (const float *)nullptr, dweight, dbias, 0, (int)cols);
+        return check_launch(what);
+    }
+    if (!x || !dy || !mean || !rstd) return fail(hipErrorInvalidValue, "%s: NULL tensor pointer", what);
+    if (sums && (!workspace || workspace_bytes < artemis_ops_layer_norm_workspace_bytes(rows, cols, dtype)))
+        return fail(hipErrorInvalidValue, "%s: workspace of %zu bytes, %zu needed", what,
+                    workspace ? workspace_bytes : (size_t)0,
+                    artemis_ops_layer_norm_workspace_bytes(rows, cols, dtype));
+    float *partial = sums ? (float *)workspace : nullptr;
+    if (dtype == ARTEMIS_OPS_F32)
+        return run_bwd<float>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, (int)cols, dtype, partial, st);
+    if (dtype == ARTEMIS_OPS_BF16)
+        return run_bwd<__bf16>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, (int)cols, dtype, partial, st);
+    return run_bwd<_Float16>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, (int)cols, dtype, partial, st);
+}
+
+}  // extern "C"

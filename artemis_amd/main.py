@@ -30,6 +30,7 @@ import torch
 from .device import add_device_argument, select_device
 from .model import ArTEMIS
 from .sharding import shard_items
+from .train import add_operator_arguments
 
 
 def get_args(argv=None):
@@ -58,6 +59,7 @@ def get_args(argv=None):
     ap.add_argument("--backend", default=os.environ.get("ARTEMIS_DIST_BACKEND", "nccl"))
     ap.add_argument("--composed", action="store_true",
                     help="the reference's per-frame composition instead of the fused head op")
+    add_operator_arguments(ap)
     add_device_argument(ap)
     return ap.parse_args(argv)
 
@@ -92,7 +94,7 @@ def save_image(tensor, path):
 def interpolate(args, device, rank=0, world=1):
     torch.manual_seed(args.random_seed)
     model = ArTEMIS(args.nbr_frame, args.joinType, args.kernel_size, args.dilation,
-                    fused=not args.composed)
+                    fused=not args.composed, encoder_ops=args.encoder_ops)
     if args.model_path:
         load_weights(model, args.model_path)
     model.to(device).eval()
@@ -120,7 +122,8 @@ def interpolate(args, device, rank=0, world=1):
 def train(args, device):
     from .train import ModelTrainer, synthetic_frames
     tr = ModelTrainer(device, lr=args.lr, betas=(args.beta1, args.beta2), seed=args.random_seed,
-                      fused=not args.composed)
+                      fused=not args.composed, encoder_ops=args.encoder_ops, optimizer=args.optimizer,
+                      weight_decay=args.weight_decay)
     step = 0
     for epoch in range(args.max_epoch):
         for _ in range(args.steps):

@@ -2,7 +2,9 @@
 ChronoSynth head (reference: model/artemis.py:8-90, model/helper_modules.py:5-51).  Harness code
 (SURVEY.md 8f-2): it exists so that BASELINE configs 1, 3 and 4 run at model level, CuPy-free.
 
-Same constructor, same forward and the same ``state_dict`` keys as upstream (``encoder.*``,
+``encoder_ops="hip"`` runs the encoder's layer norms and attention on this package's kernels too.
+
+Same constructor (``fused`` and ``encoder_ops`` are additions), same forward and the same ``state_dict`` keys as upstream (``encoder.*``,
 ``decoder.{0,1,2}.upconv.*``, ``smooth{1,2,3}.{0.conv.0,1.conv1,1.conv2}.*``,
 ``predict{1,2,3}.*``): 29,090,528 parameters for the large configuration.
 
@@ -61,14 +63,16 @@ class ArTEMIS(nn.Module):
     WINDOW = (1, 8, 8)
     HEAD_FEATURES = 64
 
-    def __init__(self, num_inputs=4, joinType="concat", kernel_size=5, dilation=1, fused=True):
+    def __init__(self, num_inputs=4, joinType="concat", kernel_size=5, dilation=1, fused=True,
+                 encoder_ops="torch"):
         super().__init__()
         nf = list(self.NUM_FEATURES)
         self.joinType = joinType
         self.num_inputs = num_inputs
         growth = 2 if joinType == "concat" else 1
         self.lrelu = nn.LeakyReLU(0.2)
-        self.encoder = SepSTSEncoder(nf, num_inputs, [self.WINDOW] * 4, list(self.NUM_HEADS))
+        self.encoder = SepSTSEncoder(nf, num_inputs, [self.WINDOW] * 4, list(self.NUM_HEADS),
+                                     ops=encoder_ops)
         self.decoder = nn.Sequential(UpSplit(nf[0], nf[1]), UpSplit(nf[1] * growth, nf[2]),
                                      UpSplit(nf[2] * growth, nf[3]))
         self.smooth1 = _smooth_net(nf[1] * growth, self.HEAD_FEATURES)

@@ -1,6 +1,8 @@
-"""The Sep-STS encoder of ArTEMIS on stock PyTorch ops (reference: model/sep_sts_encoder.py:5-67,
-model/sep_sts_layer.py:10-401).  Harness code around the synthesis hot path: no
-custom kernels here; it exists so that configs 1, 3 and 4 run at model level from this repository.
+"""The Sep-STS encoder of ArTEMIS (reference: model/sep_sts_encoder.py:5-67, model/sep_sts_layer.py:10-401).
+Harness code around the synthesis hot path, on stock PyTorch ops by default; it exists so that
+configs 1, 3 and 4 run at model level from this repository.  ``ops="hip"`` runs the layer norms and the attention
+through this package's kernels (``artemis_amd.layer_norm``, ``artemis_amd.window_attention``): same parameters, same
+results but for rounding, no copies for the cyclic roll and the window partition.
 
 Own structure, upstream parameter names: every sub-module carries the attribute name the
 reference gives it (``stem``, ``stage1..4.upper.blocks.N.{norm1,depth_attn,point_attn,norm2,mlp}``,
@@ -27,6 +29,19 @@ from functools import lru_cache
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..encoder_ops import layer_norm, window_attention
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm, on this package's kernel when ``ops`` is "hip"."""
+
+    ops = "torch"
+
+    def forward(self, x):
+        if self.ops == "hip":
+            return layer_norm(x.contiguous(), self.weight, self.bias, self.eps)
+        return super().forward(x)
 
 
 class Mlp(nn.Module):
@@ -89,6 +104,13 @@ class WindowAttention3D(nn.Module):
         out = out.reshape(Bn, h, N, C // h).transpose(1, 2).reshape(Bn, N, C)
         return self.project(out)
 
+    def on_map(self, x, shift=(0, 0, 0)):
+        """The same on the whole map x (B, D, H, W, C), whose D, H, W are multiples of ``window_size``: the
+        cyclic shift by -``shift``, the window partition, the attention with the -100 mask between regions, and
+        their inverses, in one kernel that reads the projection's output where it lies."""
+        return self.project(window_attention(self.qkv(x), self.relative_position_bias_table, self.window_size,
+                                             self.num_heads, shift=shift, outside=-100.0))
+
 
 def _windows(x, ws):
     """(B, D, H, W, C) -> (B * windows, Wd*Wh*Ww, C); D, H, W multiples of the window."""
@@ -132,16 +154,19 @@ def _shift_mask(size, ws, shift, device):
 
 
 class SepSTSBlock(nn.Module):
+    #: "torch": stock ops; "hip": this package's kernels (ArTEMIS(encoder_ops=...) sets it)
+    ops = "torch"
+
     def __init__(self, dim, num_heads, depth_window_size, shift_size, point_window_size,
                  mlp_ratio=4.0):
         super().__init__()
         self.depth_window_size = tuple(depth_window_size)
         self.point_window_size = tuple(point_window_size)
         self.shift_size = tuple(shift_size)
-        self.norm1 = nn.LayerNorm(dim)
+        self.norm1 = LayerNorm(dim)
         self.depth_attn = WindowAttention3D(dim, self.depth_window_size, num_heads)
         self.point_attn = WindowAttention3D(dim, self.point_window_size, num_heads)
-        self.norm2 = nn.LayerNorm(dim)
+        self.norm2 = LayerNorm(dim)
         self.mlp = Mlp(dim, int(dim * mlp_ratio))
 
     def attend(self, x):
@@ -152,17 +177,24 @@ class SepSTSBlock(nn.Module):
         if any(pad):
             x = F.pad(x, (0, 0, 0, pad[2], 0, pad[1], 0, pad[0]))
         Dp, Hp, Wp = D + pad[0], H + pad[1], W + pad[2]
-        shifted = any(s > 0 for s in shift)
-        if shifted:
-            x = torch.roll(x, shifts=[-s for s in shift], dims=(1, 2, 3))
-        mask = _shift_mask((Dp, Hp, Wp), ws, shift, x.device) if shifted else None
-        x = _unwindows(self.depth_attn(_windows(x, ws), mask), ws, B, Dp, Hp, Wp)
-        if shifted:
-            x = torch.roll(x, shifts=list(shift), dims=(1, 2, 3))
+        # (a window cut down to a smaller map takes its bias from the first rows and columns of the full window's
+        # index, sep_sts_layer.py:195-198, which is no function of the distance: stock ops)
+        if self.ops == "hip" and ws == self.depth_window_size:
+            x = self.depth_attn.on_map(x, shift)
+        else:
+            shifted = any(s > 0 for s in shift)
+            if shifted:
+                x = torch.roll(x, shifts=[-s for s in shift], dims=(1, 2, 3))
+            mask = _shift_mask((Dp, Hp, Wp), ws, shift, x.device) if shifted else None
+            x = _unwindows(self.depth_attn(_windows(x, ws), mask), ws, B, Dp, Hp, Wp)
+            if shifted:
+                x = torch.roll(x, shifts=list(shift), dims=(1, 2, 3))
         if any(pad):
             x = x[:, :D, :H, :W].contiguous()
         # attention over time at each pixel
         pw = _fit_window((D, H, W), self.point_window_size)
+        if self.ops == "hip" and pw == self.point_window_size:
+            return self.point_attn.on_map(x)
         return _unwindows(self.point_attn(_windows(x, pw)), pw, B, D, H, W)
 
     def forward(self, x):
@@ -215,8 +247,10 @@ class SepSTSEncoder(nn.Module):
     """Five feature levels x0..x4 at 1, 1/2, 1/4, 1/8, 1/16 of the frame size (ceil-halving:
     stride-(1,2,2) convolutions with kernel 3, padding 1), channels nf[-1]/2, nf[-1], ..., nf[0]."""
 
-    def __init__(self, nf, num_frames, window_size, num_heads):
+    def __init__(self, nf, num_frames, window_size, num_heads, ops="torch"):
         super().__init__()
+        if ops not in ("torch", "hip"):
+            raise ValueError(f"ops must be 'torch' or 'hip', got {ops!r}")
         c = list(reversed(nf))                   # (64, 128, 256, 512) for the large model
         self.stem = nn.Sequential(nn.Conv3d(3, c[0] // 2, 3, stride=1, padding=1),
                                   nn.LeakyReLU(0.2), ResBlock(c[0] // 2, 3))
@@ -228,6 +262,9 @@ class SepSTSEncoder(nn.Module):
         for i in range(4):
             setattr(self, f"down{i}", nn.Conv3d(chans[i], chans[i + 1], 3, stride=(1, 2, 2),
                                                 padding=1))
+        for m in self.modules():
+            if isinstance(m, (LayerNorm, SepSTSBlock)):
+                m.ops = ops
 
     def forward(self, x):
         feats = [self.stem(x)]

@@ -1,0 +1,188 @@
+"""AdamW over many tensors at once, moments in 32 or 8 bits (``include/artemis_ops.h``: a launch takes up to 64
+tensors).  ``adamw_step`` and ``adamw_step_8bit`` are the steps as functions on lists of tensors; ``AdamW``
+is the optimizer around them (``train.py --optimizer adamw | adamw8``).
+
+The 8-bit moments: 256 consecutive elements share an int32 base; a uint8 code counts from it in steps of
+an eighth of a binade (v: 255 codes, m: a sign and 127), rounded up or down at random with the right mean, so
+that a second moment that changes by a thousandth a step still moves.  State takes 2 + 8/256 bytes for a
+parameter instead of 8.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .encoder_ops import _DTYPES
+
+GROUP = 256   # elements that share a base
+
+
+def _check_list(name, tensors, params, dtype, counts, device):
+    if len(tensors) != len(params):
+        raise ValueError(f"{len(params)} params but {len(tensors)} {name}")
+    for i, t in enumerate(tensors):
+        if t.dtype != dtype:
+            raise TypeError(f"{name}[{i}] must be {dtype}, got {t.dtype}")
+        if t.numel() != counts[i]:
+            raise ValueError(f"{name}[{i}] has {t.numel()} elements, {counts[i]} are wanted")
+        if t.device != device:
+            raise ValueError(f"{name}[{i}] is on {t.device}, params[0] on {device}")
+        assert (t.is_contiguous() == True)
+
+
+def _describe(params, lists):
+    """The C array of the tensors' addresses; lists: one of tensors (or None) for each pointer field."""
+    array = (_lib.TensorDesc * len(params))()
+    for i, p in enumerate(params):
+        array[i] = _lib.TensorDesc(*(None if ts is None else ts[i].data_ptr() for ts in lists), p.numel())
+    return array
+
+
+def _step(params, grads, m, v, m_base, v_base, step, lr, betas, eps, weight_decay, seed):
+    bits = 32 if m_base is None else 8
+    if len(params) == 0:
+        return
+    device, dtype = params[0].device, params[0].dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"params must be float32, bfloat16 or float16, got {dtype}")
+    counts = [p.numel() for p in params]
+    _check_list("params", params, params, dtype, counts, device)
+    _check_list("grads", grads, params, dtype, counts, device)
+    kind = torch.float32 if bits == 32 else torch.uint8
+    _check_list("exp_avgs", m, params, kind, counts, device)
+    _check_list("exp_avg_sqs", v, params, kind, counts, device)
+    if bits == 8:
+        groups = [(n + GROUP - 1) // GROUP for n in counts]
+        _check_list("exp_avg_bases", m_base, params, torch.int32, groups, device)
+        _check_list("exp_avg_sq_bases", v_base, params, torch.int32, groups, device)
+    for name, tensors in (("params", params), ("exp_avgs", m), ("exp_avg_sqs", v)):
+        if len({t.data_ptr() for t, n in zip(tensors, counts) if n}) != sum(n > 0 for n in counts):
+            raise ValueError(f"{name} holds a tensor twice")  # two workgroups would update it at once
+    if int(step) != step or step < 1:
+        raise ValueError(f"step must be a whole number >= 1, got {step}")
+    if not params[0].is_cuda:
+        raise NotImplementedError()
+    if torch.cuda.is_current_stream_capturing():
+        # the step number goes into the kernels' arguments: a replay would repeat it
+        raise RuntimeError("an AdamW step cannot be captured into a graph: every replay would be the same step")
+    lib = _lib.load_ops()
+    array = _describe(params, (params, grads, m, v, m_base, v_base))
+    with torch.cuda.device(device):
+        _lib.check_ops(lib.artemis_ops_adamw(
+            array, len(params), _DTYPES[dtype], bits, lr, betas[0], betas[1], eps, weight_decay, int(step),
+            int(seed) & 0xFFFFFFFF, torch.cuda.current_stream().cuda_stream), "artemis_ops_adamw")
+    torch.autograd.graph.increment_version(params)  # what autograd saved of them is out of date
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=1e-2):
+    """Step number ``step`` (from 1) of AdamW, in place: lists of contiguous tensors of one type (fp32, bf16 or
+    fp16; gradients of the same) on one device, moments fp32.
+
+        p *= 1 - lr * weight_decay;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+        p -= lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+    """
+    _step(params, grads, exp_avgs, exp_avg_sqs, None, None, step, lr, betas, eps, weight_decay, 0)
+
+
+@torch.no_grad()
+def adamw_step_8bit(params, grads, exp_avg_codes, exp_avg_bases, exp_avg_sq_codes, exp_avg_sq_bases, step, *,
+                    lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
+    """The same with moments in 8 bits: uint8 codes like the parameters, one int32 base for each 256 elements (the
+    last group may be short); zeros stand for 0.  ``seed`` goes into the random rounding, with the step and the
+    element's place in the list of tensors: the same call gives the same bits.  A gradient that is not finite
+    spoils the moments of its group."""
+    _step(params, grads, exp_avg_codes, exp_avg_sq_codes, exp_avg_bases, exp_avg_sq_bases, step, lr, betas, eps,
+          weight_decay, seed)
+
+
+@torch.no_grad()
+def moments_from_8bit(codes, bases, signed):
+    """The fp32 values (a list of tensors like ``codes``) that 8-bit moments stand for; ``signed``: of first
+    moments (exp_avg), not second ones."""
+    if len(codes) == 0:
+        return []
+    device = codes[0].device
+    counts = [c.numel() for c in codes]
+    _check_list("codes", codes, codes, torch.uint8, counts, device)
+    _check_list("bases", bases, codes, torch.int32, [(n + GROUP - 1) // GROUP for n in counts], device)
+    if not codes[0].is_cuda:
+        raise NotImplementedError()
+    lib = _lib.load_ops()
+    with torch.cuda.device(device):
+        out = [torch.empty(c.shape, dtype=torch.float32, device=device) for c in codes]
+        array = _describe(codes, (out, None, codes, None, bases, None))
+        _lib.check_ops(lib.artemis_ops_moments_from_8bit(
+            array, len(codes), int(bool(signed)), torch.cuda.current_stream().cuda_stream),
+            "artemis_ops_moments_from_8bit")
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW whose step is one kernel launch for each 64 tensors.  ``moment_bits`` 32 or 8.  Parameters on HIP
+    devices, contiguous, fp32, bf16 or fp16; dense gradients."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, moment_bits=32, seed=0):
+        if moment_bits not in (32, 8):
+            raise ValueError(f"moment_bits must be 32 or 8, got {moment_bits}")
+        if not lr >= 0 or not eps >= 0 or not weight_decay >= 0:
+            raise ValueError(f"lr={lr}, eps={eps} and weight_decay={weight_decay} must be >= 0")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      moment_bits=moment_bits, seed=seed))
+
+    def _start(self, p, bits):
+        state = self.state[p]
+        state["step"] = 0
+        n = (p.numel() + GROUP - 1) // GROUP
+        for name in ("exp_avg", "exp_avg_sq"):
+            if bits == 32:
+                state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:
+                state[name + "_codes"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+                state[name + "_bases"] = torch.zeros(n, dtype=torch.int32, device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            bits = group["moment_bits"]
+            # one launch takes tensors of one type, device and step number
+            calls = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                state = self.state[p] or self._start(p, bits)
+                state["step"] += 1
+                calls.setdefault((p.dtype, p.device, state["step"]), []).append((p, p.grad.contiguous(), state))
+            for (_, _, number), items in calls.items():
+                ps, gs = [i[0] for i in items], [i[1] for i in items]
+                args = dict(lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
+                            weight_decay=group["weight_decay"])
+                if bits == 32:
+                    adamw_step(ps, gs, [i[2]["exp_avg"] for i in items], [i[2]["exp_avg_sq"] for i in items], number, **args)
+                else:
+                    adamw_step_8bit(ps, gs, *[[i[2][n] for i in items] for n in (
+                        "exp_avg_codes", "exp_avg_bases", "exp_avg_sq_codes", "exp_avg_sq_bases")], number,
+                        seed=group["seed"], **args)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class casts state to the parameter's type; codes, bases and fp32 moments keep their own
+        given = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(given, params):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(value):
+                    self.state[p][name] = value.to(device=p.device, copy=True)

@@ -24,6 +24,7 @@ import torch.nn as nn
 
 from .device import add_device_argument, select_device
 from .model import ArTEMIS, ChronoSynth
+from .optim import AdamW
 from .sharding import shard_bounds
 
 
@@ -63,6 +64,20 @@ def synthetic_frames(batch, size, seed, device):
     return [f.to(device) for f in frames], gt.to(device), t.to(device)
 
 
+OPTIMIZERS = ("adamax", "adamw", "adamw8")
+
+
+def make_optimizer(name, parameters, lr, betas, weight_decay, seed):
+    """"adamax": the reference's (main.py:45).  "adamw" / "adamw8": this package's AdamW with moments in 32 / 8
+    bits (2 bytes of state for a parameter instead of 8), one launch for each 64 tensors."""
+    if name == "adamax":
+        return torch.optim.Adamax(parameters, lr=lr, betas=betas)
+    if name not in OPTIMIZERS:
+        raise ValueError(f"optimizer must be one of {OPTIMIZERS}, got {name!r}")
+    return AdamW(parameters, lr=lr, betas=betas, weight_decay=weight_decay, moment_bits=8 if name == "adamw8" else 32,
+                 seed=seed)
+
+
 class HeadTrainer:
     """One ChronoSynth head under Adamax + MultiStepLR, data-parallel over the process group."""
 
@@ -71,10 +86,10 @@ class HeadTrainer:
     MILESTONES = (40, 60, 75, 85, 95, 100)
 
     def __init__(self, device, num_features=64, lr=2e-4, betas=(0.9, 0.999), milestones=MILESTONES,
-                 seed=103, fused=True):
+                 seed=103, fused=True, encoder_ops="torch", optimizer="adamax", weight_decay=1e-2):
         torch.manual_seed(seed)          # config.py:62; same init on every rank
         self.device = device
-        self.module = self.build(num_features, fused).to(device)
+        self.module = self.build(num_features, fused, encoder_ops).to(device)
         self.world = torch.distributed.get_world_size() if torch.distributed.is_initialized() else 1
         self.rank = torch.distributed.get_rank() if self.world > 1 else 0
         self.model = self.module
@@ -85,12 +100,12 @@ class HeadTrainer:
         if self.ddp:
             self.model = nn.parallel.DistributedDataParallel(
                 self.module, device_ids=[device.index], broadcast_buffers=False)
-        self.optimizer = torch.optim.Adamax(self.module.parameters(), lr=lr, betas=betas)
+        self.optimizer = make_optimizer(optimizer, self.module.parameters(), lr, betas, weight_decay, seed)
         self.scheduler = torch.optim.lr_scheduler.MultiStepLR(self.optimizer, list(milestones), gamma=0.5)
         self.loss = nn.L1Loss(reduction="mean")
 
     @staticmethod
-    def build(num_features, fused):
+    def build(num_features, fused, encoder_ops="torch"):   # a head alone has no encoder
         return ChronoSynth(4, num_features, 5, 1, apply_softmax=True, fused=fused)
 
     def shard(self, batch):
@@ -124,8 +139,9 @@ class ModelTrainer(HeadTrainer):
     DDP all-reduces the 29.09 M parameters' gradients."""
 
     @staticmethod
-    def build(num_features, fused):
-        return ArTEMIS(num_inputs=4, joinType="concat", kernel_size=5, dilation=1, fused=fused)
+    def build(num_features, fused, encoder_ops="torch"):
+        return ArTEMIS(num_inputs=4, joinType="concat", kernel_size=5, dilation=1, fused=fused,
+                       encoder_ops=encoder_ops)
 
     def shard(self, batch):
         frames, gt, t = batch
@@ -145,6 +161,14 @@ class ModelTrainer(HeadTrainer):
         return loss.detach()
 
 
+def add_operator_arguments(ap):
+    ap.add_argument("--encoder_ops", choices=["torch", "hip"], default="torch",
+                    help="the encoder's layer norms and attention: stock ops, or this package's kernels")
+    ap.add_argument("--optimizer", choices=OPTIMIZERS, default="adamax",
+                    help="the reference's Adamax, or this package's AdamW with moments in 32 or 8 bits")
+    ap.add_argument("--weight_decay", type=float, default=1e-2, help="of adamw and adamw8")
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     add_device_argument(ap)
@@ -156,6 +180,7 @@ def main(argv=None):
     ap.add_argument("--features", type=int, default=64)
     ap.add_argument("--backend", default=os.environ.get("ARTEMIS_DIST_BACKEND", "nccl"))
     ap.add_argument("--composed", action="store_true", help="reference composition instead of the fused head")
+    add_operator_arguments(ap)
     ap.add_argument("--dump", default="", help="rank 0 writes the final parameters here (tests)")
     ap.add_argument("--cudnn_benchmark", type=int, default=1,
                     help="main.py:23-24 sets torch.backends.cudnn.benchmark (MIOpen find mode on ROCm); "
@@ -181,7 +206,8 @@ def main(argv=None):
         torch.distributed.init_process_group(args.backend, **kw)
     full = args.model == "artemis"
     tr = (ModelTrainer if full else HeadTrainer)(device, num_features=args.features,
-                                                 fused=not args.composed)
+                                                 fused=not args.composed, encoder_ops=args.encoder_ops,
+                                                 optimizer=args.optimizer, weight_decay=args.weight_decay)
     import time
     for i in range(args.steps * args.epochs):
         t0 = time.perf_counter()
