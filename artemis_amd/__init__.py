@@ -6,10 +6,10 @@ from .synth import (FunctionSynth, FunctionSynthFrame, synth, synth_unpadded, sy
                     synth_options, options, offset_radius, suggest_tile_radius, adaptive_state,
                     FunctionChronoHead,
                     chrono_head)
-from .encoder_ops import FunctionLayerNorm, FunctionWindowAttention, layer_norm, window_attention  # noqa: F401
+from .encoder_ops import layer_norm, window_attention  # noqa: F401
 from .optim import AdamW, adamw_step, adamw_step_8bit, moments_from_8bit  # noqa: F401
 from ._lib import version, SynthLibraryError  # noqa: F401
 
 __all__ = ["FunctionSynth", "FunctionSynthFrame", "synth", "synth_unpadded", "synth_strip", "FunctionChronoHead", "chrono_head", "synth_options", "options", "offset_radius", "suggest_tile_radius", "adaptive_state", "version",
-           "SynthLibraryError", "layer_norm", "window_attention", "FunctionLayerNorm", "FunctionWindowAttention", "AdamW",
+           "SynthLibraryError", "layer_norm", "window_attention", "AdamW",
            "adamw_step", "adamw_step_8bit", "moments_from_8bit"]

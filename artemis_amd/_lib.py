@@ -13,6 +13,7 @@ from . import build as _build
 
 _lib = None
 _ops = None
+_ops_host = None
 
 ABI_VERSION = 1
 RADIUS_DEFAULT = -1
@@ -93,10 +94,6 @@ def lib_path() -> str:
     return os.environ.get("ARTEMIS_SYNTH_LIB", _build.LIB_PATH)
 
 
-def ops_lib_path() -> str:
-    return os.environ.get("ARTEMIS_OPS_LIB", _build.OPS_LIB_PATH)
-
-
 def _open(path, signatures):
     if not os.path.exists(path):
         raise SynthLibraryError(
@@ -125,19 +122,35 @@ def load_ops():
     """Load libartemis_ops.so once per process; raise loudly when it is absent."""
     global _ops
     if _ops is None:
-        _ops = _open(ops_lib_path(), OPS_SIGNATURES)
+        _ops = _open(_build.OPS_LIB_PATH, OPS_SIGNATURES)
     return _ops
+
+
+def load_ops_host():
+    """The extension module around libartemis_ops.so (csrc/ops_torch.cpp: the operators on torch tensors), loaded once
+    per process; raise loudly when it is absent."""
+    global _ops_host
+    if _ops_host is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries first)
+        load_ops()
+        path = _build.OPS_HOST_PATH
+        if not os.path.exists(path):
+            raise SynthLibraryError(f"{path} not found: build it with `python -m artemis_amd.build`. There is no fallback path.")
+        try:
+            spec = importlib.util.spec_from_file_location("_artemis_ops", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise SynthLibraryError(f"cannot load {path}: {e}") from e
+        _ops_host = module
+    return _ops_host
 
 
 def check(code: int, what: str) -> None:
     if code != 0:
         msg = load().artemis_synth_last_error().decode("utf-8", "replace")
-        raise RuntimeError(f"{what} failed (hipError {code}): {msg}")
-
-
-def check_ops(code: int, what: str) -> None:
-    if code != 0:
-        msg = load_ops().artemis_ops_last_error().decode("utf-8", "replace")
         raise RuntimeError(f"{what} failed (hipError {code}): {msg}")
 
 

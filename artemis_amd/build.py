@@ -18,6 +18,7 @@ LIB_DIR = os.path.join(_PKG, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libartemis_synth.so")
 OPS_LIB_PATH = os.path.join(LIB_DIR, "libartemis_ops.so")
+OPS_HOST_PATH = os.path.join(LIB_DIR, "_artemis_ops.so")   # ops_torch.cpp: the operators on torch tensors
 OPS_TYPES = ("float", "__bf16", "_Float16")   # ops_attention_type.hip: one object per element type
 
 HIPCC_FLAGS = [
@@ -50,7 +51,7 @@ def needs_build() -> bool:
 
 
 def ops_need_build() -> bool:
-    return _stale(OPS_LIB_PATH, "ops_", "artemis_ops.h")
+    return _stale(OPS_LIB_PATH, "ops_", "artemis_ops.h") or _stale(OPS_HOST_PATH, "ops_torch", "artemis_ops.h")
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
@@ -68,9 +69,43 @@ def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
 
 def build_ops(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
     """The same for artemis_amd/lib/libartemis_ops.so: layer norm, windowed attention (one object per
-    element type), AdamW."""
+    element type), AdamW; and the extension module around it."""
     if not force and not ops_need_build():
         return OPS_LIB_PATH
+    from concurrent.futures import ThreadPoolExecutor
+    with ThreadPoolExecutor(1) as pool:      # (the module's 45 s of torch headers beside the kernels)
+        module = pool.submit(_compile_ops_host, OPS_HOST_PATH + ".o", verbose)
+        _build_ops_lib(verbose, extra_flags)
+        module.result()
+    _run(["g++", "-shared", "-o", OPS_HOST_PATH, OPS_HOST_PATH + ".o", "-L" + LIB_DIR, "-lartemis_ops",
+          *[f"-L{p}" for p in _torch_paths()[1]], "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+          "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
+    os.remove(OPS_HOST_PATH + ".o")
+    return OPS_LIB_PATH
+
+
+def _torch_paths():
+    from torch.utils import cpp_extension
+    return cpp_extension.include_paths("cuda"), cpp_extension.library_paths("cuda")
+
+
+def _compile_ops_host(obj, verbose):
+    import sysconfig
+    os.makedirs(LIB_DIR, exist_ok=True)
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I" + INCLUDE,
+          *[f"-I{p}" for p in (*_torch_paths()[0], sysconfig.get_paths()["include"])], "-c", "-o", obj,
+          os.path.join(CSRC, "ops_torch.cpp")], verbose)
+
+
+def _run(cmd, verbose):
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("failed: " + " ".join(cmd) + "\n" + r.stderr)
+
+
+def _build_ops_lib(verbose, extra_flags) -> str:
     jobs = [(os.path.join(CSRC, f"ops_{n}.hip"), os.path.join(OBJ_DIR, f"ops_{n}.o"), [])
             for n in ("host", "norm", "adamw", "attention")]
     jobs += [(os.path.join(CSRC, "ops_attention_type.hip"), os.path.join(OBJ_DIR, f"ops_attention_{t}.o"),
@@ -85,22 +120,12 @@ def _compile_and_link(jobs, flags, extra_flags, lib_path, verbose) -> str:
 
     def compile_one(job):
         src, obj, defs = job
-        cmd = [hipcc, *flags, *extra_flags, *defs, "-I" + INCLUDE, "-c", "-o", obj, src]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("hipcc failed: " + " ".join(cmd) + "\n" + r.stderr)
+        _run([hipcc, *flags, *extra_flags, *defs, "-I" + INCLUDE, "-c", "-o", obj, src], verbose)
 
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(workers) as pool:
         list(pool.map(compile_one, jobs))
-    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib_path] + [j[1] for j in jobs]
-    if verbose:
-        print(" ".join(link))
-    r = subprocess.run(link, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("link failed:\n" + r.stderr)
+    _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib_path] + [j[1] for j in jobs], verbose)
     return lib_path
 
 

@@ -1,0 +1,352 @@
+// ops_torch.cpp -- the operators of libartemis_ops.so as functions on torch tensors: checks, memory, the current
+// stream and autograd.  A call costs a few microseconds here; the same in Python took 60 to 130, longer
+// than the kernels on all but large inputs, and a step over 320 tensors 0.7 ms.
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <limits>
+#include <unordered_set>
+
+#include "artemis_ops.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using MaybeTensor = std::optional<at::Tensor>;
+
+int type_code(const at::Tensor &t, const char *what)
+{
+    switch (t.scalar_type()) {
+    case at::kFloat: return ARTEMIS_OPS_F32;
+    case at::kBFloat16: return ARTEMIS_OPS_BF16;
+    case at::kHalf: return ARTEMIS_OPS_F16;
+    default: TORCH_CHECK_TYPE(false, what, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+    }
+}
+
+// the framework's contract: contiguity is asserted
+void assert_contiguous(const at::Tensor &t, const char *what)
+{
+    if (t.is_contiguous()) return;
+    PyErr_Format(PyExc_AssertionError, "%s must be contiguous", what);
+    throw pybind11::error_already_set();
+}
+
+void on_gpu(const at::Tensor &t)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(t.is_cuda(), "the operators run on HIP devices only, got a tensor on ", t.device());
+}
+
+void ok(int code, const char *what)
+{
+    TORCH_CHECK(code == 0, what, " failed (hipError ", code, "): ", artemis_ops_last_error());
+}
+
+void *stream_of(const at::Tensor &t)
+{
+    return (void *)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+}
+
+const void *in(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void *out(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+const float *in_f(const at::Tensor &t) { return (const float *)in(t); }
+float *out_f(const at::Tensor &t) { return (float *)out(t); }
+
+at::Tensor workspace_of(size_t bytes, const at::Tensor &like)
+{
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// A parameter as the kernels read it: contiguous fp32 on the input's device.  Another floating type is widened through
+// autograd, so that its gradient comes back in that type.
+MaybeTensor parameter(const MaybeTensor &t, at::IntArrayRef shape, const at::Tensor &like, const char *what)
+{
+    if (!t || !t->defined()) return std::nullopt;
+    type_code(*t, what);
+    TORCH_CHECK_VALUE(t->sizes() == shape, what, " must be ", shape, ", got ", t->sizes());
+    TORCH_CHECK_VALUE(t->device() == like.device(), what, " is on ", t->device(), ", the input on ", like.device());
+    assert_contiguous(*t, what);
+    return t->scalar_type() == at::kFloat ? t : t->to(at::kFloat);
+}
+
+// First derivatives only: where a graph of the backward pass is being built (create_graph), its results lead to an error.
+variable_list once(variable_list grads)
+{
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list given;
+    for (auto &g : grads)
+        if (g.defined()) given.push_back(g.detach().requires_grad_(true));
+    auto node = std::make_shared<torch::autograd::DelayedError>(
+        "artemis_amd's encoder operators have no second derivatives", (int64_t)given.size());
+    variable_list kept = (*node)(std::move(given));
+    size_t i = 0;
+    for (auto &g : grads)
+        if (g.defined()) g = kept[i++];
+    return grads;
+}
+
+// -------------------------------------------------------------------------------------------- layer norm
+
+class LayerNorm : public torch::autograd::Function<LayerNorm> {
+public:
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const MaybeTensor &maybe_weight,
+                              const MaybeTensor &maybe_bias, double eps, bool train)
+    {
+        const at::Tensor weight = maybe_weight.value_or(at::Tensor()), bias = maybe_bias.value_or(at::Tensor());
+        const int64_t cols = x.size(-1), rows = cols ? x.numel() / cols : 0;
+        const c10::DeviceGuard guard(x.device());
+        at::Tensor y = at::empty_like(x), stats;
+        if (train) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+        float *mean = out_f(stats);
+        ok(artemis_ops_layer_norm_forward(in(x), in_f(weight), in_f(bias), out(y), mean, mean ? mean + rows : nullptr, rows,
+                                          cols, (float)eps, type_code(x, "x"), stream_of(x)),
+           "artemis_ops_layer_norm_forward");
+        if (train) {
+            ctx->save_for_backward({x, weight, stats});
+            ctx->saved_data["bias"] = bias.defined();
+        }
+        return y;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list dys)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+        if (!dys[0].defined()) return {{}, {}, {}, {}, {}};
+        const int64_t cols = x.size(-1), rows = cols ? x.numel() / cols : 0;
+        const int type = type_code(x, "x");
+        const c10::DeviceGuard guard(x.device());
+        const at::Tensor dy = dys[0].contiguous();
+        const auto f32 = x.options().dtype(at::kFloat);
+        at::Tensor dx, dw, db, workspace;
+        if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
+        // (the tensors among the arguments are counted)
+        if (weight.defined() && ctx->needs_input_grad(1)) dw = at::empty({cols}, f32);
+        if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(1 + weight.defined())) db = at::empty({cols}, f32);
+        size_t bytes = 0;
+        if (dw.defined() || db.defined()) {
+            bytes = artemis_ops_layer_norm_workspace_bytes(rows, cols, type);
+            workspace = workspace_of(bytes, x);
+        }
+        const float *mean = in_f(stats);
+        ok(artemis_ops_layer_norm_backward(in(x), in(dy), in_f(weight), mean, mean + rows, out(dx), out_f(dw), out_f(db),
+                                           rows, cols, type, out(workspace), bytes, stream_of(x)),
+           "artemis_ops_layer_norm_backward");
+        return once({dx, dw, db, {}, {}});
+    }
+};
+
+bool wants_grad(const at::Tensor &x, const MaybeTensor &a, const MaybeTensor &b)
+{
+    return at::GradMode::is_enabled() && (x.requires_grad() || (a && a->requires_grad()) || (b && b->requires_grad()));
+}
+
+at::Tensor layer_norm(const at::Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, double eps)
+{
+    type_code(x, "x");
+    TORCH_CHECK_VALUE(x.dim() >= 1, "x must be (..., C)");
+    TORCH_CHECK_VALUE(eps >= 0, "eps must be >= 0, got ", eps);
+    const MaybeTensor w = parameter(weight, {x.size(-1)}, x, "weight"), b = parameter(bias, {x.size(-1)}, x, "bias");
+    assert_contiguous(x, "x");
+    on_gpu(x);
+    return LayerNorm::apply(x, w, b, eps, wants_grad(x, w, b));
+}
+
+// --------------------------------------------------------------------------------------------- attention
+
+// The kernels load four elements at once; a view that starts elsewhere is copied.
+at::Tensor aligned(const at::Tensor &t)
+{
+    return (size_t)t.const_data_ptr() % (4 * t.element_size()) == 0 ? t : t.clone();
+}
+
+class WindowAttention : public torch::autograd::Function<WindowAttention> {
+public:
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &qkv, const MaybeTensor &maybe_table,
+                              const MaybeTensor &maybe_labels, const artemis_ops_window &w, bool train)
+    {
+        const at::Tensor table = maybe_table.value_or(at::Tensor()), labels = maybe_labels.value_or(at::Tensor());
+        const c10::DeviceGuard guard(qkv.device());
+        at::Tensor o = at::empty({w.B, w.D, w.H, w.W, (int64_t)w.heads * w.head_dim}, qkv.options()), lse;
+        if (train)
+            if (const size_t n = artemis_ops_window_attention_lse_count(&w))
+                lse = at::empty({(int64_t)n}, qkv.options().dtype(at::kFloat));
+        const size_t bytes = artemis_ops_window_attention_workspace_bytes(&w, 0, 0);
+        const at::Tensor workspace = workspace_of(bytes, qkv);
+        ok(artemis_ops_window_attention_forward(&w, in(qkv), in_f(table), (const int *)in(labels), out(o), out_f(lse),
+                                                out(workspace), bytes, stream_of(qkv)),
+           "artemis_ops_window_attention_forward");
+        if (train) {
+            // short windows: the backward pass computes the softmax again and reads neither output nor lse
+            ctx->save_for_backward({qkv, table, labels, lse.defined() ? o : at::Tensor(), lse});
+            ctx->saved_data["w"] = std::string((const char *)&w, sizeof(w));
+        }
+        return o;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list douts)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &qkv = saved[0], &table = saved[1], &labels = saved[2], &o = saved[3], &lse = saved[4];
+        if (!douts[0].defined()) return {{}, {}, {}, {}, {}};
+        artemis_ops_window w;
+        const std::string packed = ctx->saved_data["w"].toStringRef();
+        memcpy(&w, packed.data(), sizeof(w));
+        const c10::DeviceGuard guard(qkv.device());
+        const at::Tensor dout = aligned(douts[0].contiguous());
+        const at::Tensor dqkv = at::empty_like(qkv);
+        at::Tensor dtable;
+        if (table.defined() && ctx->needs_input_grad(1)) dtable = at::empty_like(table);
+        const size_t bytes = artemis_ops_window_attention_workspace_bytes(&w, 1, dtable.defined());
+        const at::Tensor workspace = workspace_of(bytes, qkv);
+        ok(artemis_ops_window_attention_backward(&w, in(qkv), in_f(table), (const int *)in(labels), in(o), in_f(lse), in(dout),
+                                                 out(dqkv), out_f(dtable), out(workspace), bytes, stream_of(qkv)),
+           "artemis_ops_window_attention_backward");
+        return once({ctx->needs_input_grad(0) ? dqkv : at::Tensor(), dtable, {}, {}, {}});
+    }
+};
+
+at::Tensor window_attention(const at::Tensor &qkv, const MaybeTensor &bias_table, const std::vector<int64_t> &window,
+                            int64_t heads, const std::vector<int64_t> &shift, const MaybeTensor &labels, double outside,
+                            std::optional<double> scale)
+{
+    const int type = type_code(qkv, "qkv");
+    TORCH_CHECK_VALUE(qkv.dim() == 5, "qkv must be (B, D, H, W, 3 * C), got ", qkv.sizes());
+    TORCH_CHECK_VALUE(window.size() == 3, "window must be (d, h, w), got ", window);
+    TORCH_CHECK_VALUE(shift.size() == 3, "shift must be (d, h, w), got ", shift);
+    const int64_t B = qkv.size(0), C3 = qkv.size(4);
+    TORCH_CHECK_VALUE(heads >= 1 && heads <= 1024 && C3 % (3 * heads) == 0, "qkv's last dimension ", C3,
+                      " is not 3 * num_heads * head_dim for ", heads, " heads (1 to 1024)");
+    const int64_t hd = C3 / (3 * heads);
+    TORCH_CHECK_VALUE(hd % 4 == 0 && hd >= 4 && hd <= 128, "head_dim ", hd, " must be a multiple of 4 up to 128");
+    int64_t tokens = 1, entries = 1;
+    for (int i = 0; i < 3; ++i) {
+        TORCH_CHECK_VALUE(window[i] >= 1 && window[i] <= 4096, "window ", window, " must hold 1 to 4096 tokens");
+        tokens *= window[i];
+        entries *= 2 * window[i] - 1;
+        TORCH_CHECK_VALUE(tokens <= 4096, "window ", window, " must hold 1 to 4096 tokens");
+        TORCH_CHECK_VALUE(qkv.size(1 + i) % window[i] == 0, "map ", qkv.sizes().slice(1, 3), " is not a multiple of the window ",
+                          window);
+        TORCH_CHECK_VALUE(shift[i] >= 0 && shift[i] < window[i], "shift ", shift, " must lie in [0, window) for the window ",
+                          window);
+        TORCH_CHECK_VALUE(qkv.size(1 + i) <= std::numeric_limits<int>::max(), "the map is too large");
+    }
+    TORCH_CHECK_VALUE(B <= std::numeric_limits<int>::max(), "the batch is too large");
+    TORCH_CHECK_VALUE(outside <= 0, "outside must be <= 0, got ", outside);
+    const double s = scale ? *scale : 1.0 / std::sqrt((double)hd);
+    TORCH_CHECK_VALUE(std::isfinite(s) && std::isfinite((float)s), "scale must be finite, got ", s);
+    const MaybeTensor table = parameter(bias_table, {entries, heads}, qkv, "bias_table");
+    int maps = 0;
+    if (labels) {
+        const at::Tensor &lab = *labels;
+        TORCH_CHECK_TYPE(lab.scalar_type() == at::kInt, "labels must be int32, got ", lab.scalar_type());
+        TORCH_CHECK_VALUE(lab.sizes() == qkv.sizes().slice(1, 3) || lab.sizes() == qkv.sizes().slice(0, 4), "labels must be ",
+                          qkv.sizes().slice(1, 3), " or ", qkv.sizes().slice(0, 4), ", got ", lab.sizes());
+        TORCH_CHECK_VALUE(lab.device() == qkv.device(), "labels are on ", lab.device(), ", qkv on ", qkv.device());
+        assert_contiguous(lab, "labels");
+        maps = lab.dim() == 4 && B > 1 ? (int)B : 1;
+    }
+    assert_contiguous(qkv, "qkv");
+    on_gpu(qkv);
+    const artemis_ops_window w{(int)B, (int)qkv.size(1), (int)qkv.size(2), (int)qkv.size(3), (int)heads, (int)hd,
+                               (int)window[0], (int)window[1], (int)window[2], (int)shift[0], (int)shift[1], (int)shift[2],
+                               maps, type, (float)s, (float)outside};
+    const at::Tensor x = aligned(qkv);
+    return WindowAttention::apply(x, table, labels, w, wants_grad(x, table, std::nullopt));
+}
+
+// ------------------------------------------------------------------------------------------------- AdamW
+
+using Tensors = std::vector<at::Tensor>;
+constexpr int64_t kGroup = 256;  // elements that share a base
+
+void check_list(const char *name, const Tensors &ts, const Tensors &params, at::ScalarType type, bool groups)
+{
+    TORCH_CHECK_VALUE(ts.size() == params.size(), params.size(), " params but ", ts.size(), " ", name);
+    for (size_t i = 0; i < ts.size(); ++i) {
+        const at::Tensor &t = ts[i];
+        TORCH_CHECK_TYPE(t.scalar_type() == type, name, "[", i, "] must be ", type, ", got ", t.scalar_type());
+        const int64_t want = groups ? (params[i].numel() + kGroup - 1) / kGroup : params[i].numel();
+        TORCH_CHECK_VALUE(t.numel() == want, name, "[", i, "] has ", t.numel(), " elements, ", want, " are wanted");
+        TORCH_CHECK_VALUE(t.device() == params[0].device(), name, "[", i, "] is on ", t.device(), ", params[0] on ",
+                          params[0].device());
+        assert_contiguous(t, name);
+    }
+}
+
+// two workgroups would update it at once
+void check_distinct(const char *name, const Tensors &ts)
+{
+    std::unordered_set<const void *> seen;
+    for (const at::Tensor &t : ts)
+        TORCH_CHECK_VALUE(t.numel() == 0 || seen.insert(t.const_data_ptr()).second, name, " holds a tensor twice");
+}
+
+void adamw(const Tensors &params, const Tensors &grads, const Tensors &m, const Tensors &v, const Tensors &m_base,
+           const Tensors &v_base, int bits, int64_t step, double lr, double beta1, double beta2, double eps,
+           double weight_decay, int64_t seed)
+{
+    if (params.empty() && grads.empty()) return;
+    TORCH_CHECK_VALUE(!params.empty(), "no params but ", grads.size(), " grads");
+    const int type = type_code(params[0], "params");
+    const at::ScalarType kind = bits == 32 ? at::kFloat : at::kByte;
+    check_list("params", params, params, params[0].scalar_type(), false);
+    check_list("grads", grads, params, params[0].scalar_type(), false);
+    check_list("exp_avgs", m, params, kind, false);
+    check_list("exp_avg_sqs", v, params, kind, false);
+    if (bits == 8) {
+        check_list("exp_avg_bases", m_base, params, at::kInt, true);
+        check_list("exp_avg_sq_bases", v_base, params, at::kInt, true);
+    }
+    check_distinct("params", params);
+    check_distinct("exp_avgs", m);
+    check_distinct("exp_avg_sqs", v);
+    TORCH_CHECK_VALUE(step >= 1, "step must be a whole number >= 1, got ", step);
+    on_gpu(params[0]);
+    std::vector<artemis_ops_tensor> list(params.size());
+    for (size_t i = 0; i < params.size(); ++i)
+        list[i] = {params[i].data_ptr(), grads[i].const_data_ptr(), m[i].data_ptr(), v[i].data_ptr(),
+                   bits == 8 ? (int *)m_base[i].data_ptr() : nullptr, bits == 8 ? (int *)v_base[i].data_ptr() : nullptr,
+                   params[i].numel()};
+    const c10::DeviceGuard guard(params[0].device());
+    ok(artemis_ops_adamw(list.data(), (int)list.size(), type, bits, lr, beta1, beta2, eps, weight_decay, step, (unsigned)seed,
+                         stream_of(params[0])),
+       "artemis_ops_adamw");
+    // what autograd saved of them is out of date
+    for (const at::Tensor &p : params)
+        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensors moments_from_8bit(const Tensors &codes, const Tensors &bases, bool is_signed)
+{
+    if (codes.empty() && bases.empty()) return {};
+    TORCH_CHECK_VALUE(!codes.empty(), "no codes but ", bases.size(), " bases");
+    check_list("codes", codes, codes, at::kByte, false);
+    check_list("bases", bases, codes, at::kInt, true);
+    on_gpu(codes[0]);
+    const c10::DeviceGuard guard(codes[0].device());
+    Tensors values;
+    std::vector<artemis_ops_tensor> list;
+    for (size_t i = 0; i < codes.size(); ++i) {
+        values.push_back(at::empty(codes[i].sizes(), codes[i].options().dtype(at::kFloat)));
+        list.push_back({values[i].data_ptr(), nullptr, codes[i].data_ptr(), nullptr, (int *)bases[i].data_ptr(), nullptr,
+                        codes[i].numel()});
+    }
+    ok(artemis_ops_moments_from_8bit(list.data(), (int)list.size(), is_signed, stream_of(codes[0])),
+       "artemis_ops_moments_from_8bit");
+    return values;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_artemis_ops, m)
+{
+    m.def("layer_norm", &layer_norm);
+    m.def("window_attention", &window_attention);
+    m.def("adamw", &adamw);
+    m.def("moments_from_8bit", &moments_from_8bit);
+}

@@ -9,116 +9,45 @@ parameter instead of 8.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .encoder_ops import _DTYPES
 
 GROUP = 256   # elements that share a base
 
 
-def _check_list(name, tensors, params, dtype, counts, device):
-    if len(tensors) != len(params):
-        raise ValueError(f"{len(params)} params but {len(tensors)} {name}")
-    for i, t in enumerate(tensors):
-        if t.dtype != dtype:
-            raise TypeError(f"{name}[{i}] must be {dtype}, got {t.dtype}")
-        if t.numel() != counts[i]:
-            raise ValueError(f"{name}[{i}] has {t.numel()} elements, {counts[i]} are wanted")
-        if t.device != device:
-            raise ValueError(f"{name}[{i}] is on {t.device}, params[0] on {device}")
-        assert (t.is_contiguous() == True)
-
-
-def _describe(params, lists):
-    """The C array of the tensors' addresses; lists: one of tensors (or None) for each pointer field."""
-    array = (_lib.TensorDesc * len(params))()
-    for i, p in enumerate(params):
-        array[i] = _lib.TensorDesc(*(None if ts is None else ts[i].data_ptr() for ts in lists), p.numel())
-    return array
-
-
-def _step(params, grads, m, v, m_base, v_base, step, lr, betas, eps, weight_decay, seed):
-    bits = 32 if m_base is None else 8
-    if len(params) == 0:
-        return
-    device, dtype = params[0].device, params[0].dtype
-    if dtype not in _DTYPES:
-        raise TypeError(f"params must be float32, bfloat16 or float16, got {dtype}")
-    counts = [p.numel() for p in params]
-    _check_list("params", params, params, dtype, counts, device)
-    _check_list("grads", grads, params, dtype, counts, device)
-    kind = torch.float32 if bits == 32 else torch.uint8
-    _check_list("exp_avgs", m, params, kind, counts, device)
-    _check_list("exp_avg_sqs", v, params, kind, counts, device)
-    if bits == 8:
-        groups = [(n + GROUP - 1) // GROUP for n in counts]
-        _check_list("exp_avg_bases", m_base, params, torch.int32, groups, device)
-        _check_list("exp_avg_sq_bases", v_base, params, torch.int32, groups, device)
-    for name, tensors in (("params", params), ("exp_avgs", m), ("exp_avg_sqs", v)):
-        if len({t.data_ptr() for t, n in zip(tensors, counts) if n}) != sum(n > 0 for n in counts):
-            raise ValueError(f"{name} holds a tensor twice")  # two workgroups would update it at once
-    if int(step) != step or step < 1:
-        raise ValueError(f"step must be a whole number >= 1, got {step}")
-    if not params[0].is_cuda:
-        raise NotImplementedError()
-    if torch.cuda.is_current_stream_capturing():
+def _step(*args):
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
         # the step number goes into the kernels' arguments: a replay would repeat it
         raise RuntimeError("an AdamW step cannot be captured into a graph: every replay would be the same step")
-    lib = _lib.load_ops()
-    array = _describe(params, (params, grads, m, v, m_base, v_base))
-    with torch.cuda.device(device):
-        _lib.check_ops(lib.artemis_ops_adamw(
-            array, len(params), _DTYPES[dtype], bits, lr, betas[0], betas[1], eps, weight_decay, int(step),
-            int(seed) & 0xFFFFFFFF, torch.cuda.current_stream().cuda_stream), "artemis_ops_adamw")
-    torch.autograd.graph.increment_version(params)  # what autograd saved of them is out of date
+    _lib.load_ops_host().adamw(*args)
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
                weight_decay=1e-2):
     """Step number ``step`` (from 1) of AdamW, in place: lists of contiguous tensors of one type (fp32, bf16 or
-    fp16; gradients of the same) on one device, moments fp32.
+    fp16; gradients of the same) on one device that do not overlap, moments fp32.
 
         p *= 1 - lr * weight_decay;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         p -= lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
     """
-    _step(params, grads, exp_avgs, exp_avg_sqs, None, None, step, lr, betas, eps, weight_decay, 0)
+    _step(params, grads, exp_avgs, exp_avg_sqs, [], [], 32, step, lr, *betas, eps, weight_decay, 0)
 
 
-@torch.no_grad()
 def adamw_step_8bit(params, grads, exp_avg_codes, exp_avg_bases, exp_avg_sq_codes, exp_avg_sq_bases, step, *,
                     lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
     """The same with moments in 8 bits: uint8 codes like the parameters, one int32 base for each 256 elements (the
     last group may be short); zeros stand for 0.  ``seed`` goes into the random rounding, with the step and the
     element's place in the list of tensors: the same call gives the same bits.  A gradient that is not finite
     spoils the moments of its group."""
-    _step(params, grads, exp_avg_codes, exp_avg_sq_codes, exp_avg_bases, exp_avg_sq_bases, step, lr, betas, eps,
+    _step(params, grads, exp_avg_codes, exp_avg_sq_codes, exp_avg_bases, exp_avg_sq_bases, 8, step, lr, *betas, eps,
           weight_decay, seed)
 
 
-@torch.no_grad()
 def moments_from_8bit(codes, bases, signed):
     """The fp32 values (a list of tensors like ``codes``) that 8-bit moments stand for; ``signed``: of first
     moments (exp_avg), not second ones."""
-    if len(codes) == 0:
-        return []
-    device = codes[0].device
-    counts = [c.numel() for c in codes]
-    _check_list("codes", codes, codes, torch.uint8, counts, device)
-    _check_list("bases", bases, codes, torch.int32, [(n + GROUP - 1) // GROUP for n in counts], device)
-    if not codes[0].is_cuda:
-        raise NotImplementedError()
-    lib = _lib.load_ops()
-    with torch.cuda.device(device):
-        out = [torch.empty(c.shape, dtype=torch.float32, device=device) for c in codes]
-        array = _describe(codes, (out, None, codes, None, bases, None))
-        _lib.check_ops(lib.artemis_ops_moments_from_8bit(
-            array, len(codes), int(bool(signed)), torch.cuda.current_stream().cuda_stream),
-            "artemis_ops_moments_from_8bit")
-    return out
+    return _lib.load_ops_host().moments_from_8bit(codes, bases, signed)
 
 
 class AdamW(torch.optim.Optimizer):

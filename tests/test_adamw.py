@@ -296,8 +296,8 @@ def test_refusals():
         artemis_amd.adamw_step(p, g[:1], m, v, 1)
     with pytest.raises(ValueError):
         artemis_amd.adamw_step(p, [g[0], g[1][:299]], m, v, 1)
-    for step in (0, -1, 1.5):
-        with pytest.raises(ValueError):
+    for step, error in ((0, ValueError), (-1, ValueError), (1.5, TypeError)):
+        with pytest.raises(error):
             artemis_amd.adamw_step(p, g, m, v, step)
     with pytest.raises(ValueError, match="twice"):
         artemis_amd.adamw_step([p[0], p[0]], g, m, v, 1)

@@ -173,6 +173,19 @@ def test_forward_and_backward_replay_from_a_graph():
             assert torch.equal(a, c)
 
 
+@pytest.mark.gpu
+def test_there_is_no_second_derivative():
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    w = torch.randn(8, device=DEV, requires_grad=True)
+    dx, dw = torch.autograd.grad(artemis_amd.layer_norm(x, w).square().sum(), (x, w), create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        (dx.sum() + dw.sum()).backward()
+    q = torch.randn(1, 1, 8, 8, 24, device=DEV, requires_grad=True)
+    dq, = torch.autograd.grad(artemis_amd.window_attention(q, None, (1, 8, 8), 2).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        dq.sum().backward()
+
+
 def test_refusals():
     x = torch.randn(4, 8)
     with pytest.raises(NotImplementedError):

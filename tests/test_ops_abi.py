@@ -23,7 +23,7 @@ def error():
 def test_every_declared_symbol_is_exported_and_bound():
     text = re.sub(r"/\*.*?\*/", "", header(), flags=re.S)
     names = sorted(set(re.findall(r"\b(artemis_ops_\w+)\s*\(", text)))
-    lib = ctypes.CDLL(_lib.ops_lib_path())
+    lib = ctypes.CDLL(build.OPS_LIB_PATH)
     assert all(hasattr(lib, n) for n in names)
     assert sorted(_lib.OPS_SIGNATURES) == names
 
@@ -126,7 +126,11 @@ def test_adamw_validation():
 
 
 def test_missing_library_fails_loudly(monkeypatch, tmp_path):
-    monkeypatch.setenv("ARTEMIS_OPS_LIB", str(tmp_path / "nope.so"))
+    monkeypatch.setattr(build, "OPS_HOST_PATH", str(tmp_path / "nope.so"))
+    monkeypatch.setattr(_lib, "_ops_host", None)
+    with pytest.raises(_lib.SynthLibraryError, match="no fallback"):
+        _lib.load_ops_host()
+    monkeypatch.setattr(build, "OPS_LIB_PATH", str(tmp_path / "nope.so"))
     monkeypatch.setattr(_lib, "_ops", None)
     with pytest.raises(_lib.SynthLibraryError, match="no fallback"):
-        _lib.load_ops()
+        _lib.load_ops_host()
