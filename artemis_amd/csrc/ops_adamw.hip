@@ -23,7 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kShare = 4096;  // elements a workgroup takes
 constexpr int kGroup = 256;   // elements that share a base
-constexpr int kTensors = 64;  // 64 * 60 bytes: within the 4 KB of a launch's arguments
+constexpr int kTensors = 62;  // 62 * 64 bytes: within the 4 KB of a launch's arguments
 
 struct Tensor {
     void *p;
@@ -35,9 +35,9 @@ struct Tensor {
 
 struct Batch {
     Tensor t[kTensors];
-    int first[kTensors];  // the first workgroup of each tensor
+    int first[kTensors];       // the first workgroup of each tensor
+    unsigned place[kTensors];  // its place among all tensors, in groups of kGroup
     int n;
-    unsigned place;  // of the first tensor, in groups of kGroup
 };
 
 struct Coef {
@@ -87,23 +87,30 @@ __global__ __launch_bounds__(kThreads) void adamw32(const Batch b, const Coef c)
     const bool aligned = (((size_t)m | (size_t)v) & 15) == 0 && (((size_t)p | (size_t)g) & (4 * sizeof(T) - 1)) == 0;
     if (aligned && n == kShare) {
         constexpr int K = kShare / (4 * kThreads);
+        Vec<T, 4> pv[K], gv[K];  // all loads in front of the first store
+        f32x4 mv[K], vv[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int i = k * kThreads + threadIdx.x;
-            Vec<T, 4> pv = ((Vec<T, 4> *)p)[i];
-            const Vec<T, 4> gv = ((const Vec<T, 4> *)g)[i];
-            f32x4 mv = ((f32x4 *)m)[i], vv = ((f32x4 *)v)[i];
+            pv[k] = ((Vec<T, 4> *)p)[i];
+            gv[k] = ((const Vec<T, 4> *)g)[i];
+            mv[k] = ((f32x4 *)m)[i];
+            vv[k] = ((f32x4 *)v)[i];
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = k * kThreads + threadIdx.x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = to_f32(pv.v[e]), a = mv[e], q = vv[e];
-                update(x, to_f32(gv.v[e]), a, q, c);
-                pv.v[e] = from_f32<T>(x);
-                mv[e] = a;
-                vv[e] = q;
+                float x = to_f32(pv[k].v[e]), a = mv[k][e], q = vv[k][e];
+                update(x, to_f32(gv[k].v[e]), a, q, c);
+                pv[k].v[e] = from_f32<T>(x);
+                mv[k][e] = a;
+                vv[k][e] = q;
             }
-            ((Vec<T, 4> *)p)[i] = pv;
-            ((f32x4 *)m)[i] = mv;
-            ((f32x4 *)v)[i] = vv;
+            ((Vec<T, 4> *)p)[i] = pv[k];
+            ((f32x4 *)m)[i] = mv[k];
+            ((f32x4 *)v)[i] = vv[k];
         }
         return;
     }
@@ -166,87 +173,101 @@ __device__ __forceinline__ unsigned encode_signed(float m, int base, unsigned ra
     return (unsigned)q | (m < 0.f && q ? 128u : 0u);
 }
 
+// The largest of 64 lanes' values: within rows of 16 by shifted copies, then across the rows.
 __device__ __forceinline__ unsigned wave_max(unsigned x)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const unsigned o = __shfl_xor(x, d);
-        x = o > x ? o : x;
-    }
+    auto step = [&](int y) { x = (unsigned)y > x ? (unsigned)y : x; };
+    step(__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));
+    step(__shfl_xor((int)x, 16));
+    step(__shfl_xor((int)x, 32));
     return x;
 }
 
-// A wave takes groups of 256 elements, four neighbours in each lane.
+// What a lane holds of a group: four neighbouring elements, the first n of them.
+template <class T>
+struct Held {
+    Vec<T, 4> p, g;
+    Vec<unsigned char, 4> m, v;
+    int mb, vb;
+};
+
+// A wave takes groups of 256 elements, four neighbours in each lane; all groups' loads are in front of the first store.
 template <class T>
 __global__ __launch_bounds__(kThreads) void adamw8(const Batch b, const Coef c)
 {
+    constexpr int K = kShare / kGroup / (kThreads / 64);
     const int which = find(b);
     const Tensor t = b.t[which];
     const long long at = (long long)(blockIdx.x - b.first[which]) * kShare;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    // the element's place among all tensors, counted in whole groups
-    unsigned place = b.place;
-    for (int k = 0; k < which; ++k) place += (unsigned)((b.t[k].count + kGroup - 1) / kGroup);
+    const unsigned place = b.place[which];
     const bool aligned = ((size_t)t.p % (4 * sizeof(T)) | (size_t)t.g % (4 * sizeof(T)) |
                           ((size_t)t.m & 3) | ((size_t)t.v & 3)) == 0;
+    Held<T> held[K];
 #pragma unroll
-    for (int k = 0; k < kShare / kGroup / 4; ++k) {
-        const long long i0 = at + (wave * (kShare / kGroup / 4) + k) * kGroup;
-        if (i0 >= t.count) break;
-        const long long i = i0 + lane * 4;
-        const long long group = i0 / kGroup;
-        const int n = (int)(t.count - i < 0 ? 0 : t.count - i < 4 ? t.count - i : 4);
-        T *p = (T *)t.p + i;
-        const T *g = (const T *)t.g + i;
-        unsigned char *mc = (unsigned char *)t.m + i, *vc = (unsigned char *)t.v + i;
-        Vec<T, 4> pv{}, gv{};
-        Vec<unsigned char, 4> mv{}, vv{};
-        const bool whole = aligned && n == 4;
-        if (whole) {
-            pv = *(Vec<T, 4> *)p;
-            gv = *(const Vec<T, 4> *)g;
-            mv = *(Vec<unsigned char, 4> *)mc;
-            vv = *(Vec<unsigned char, 4> *)vc;
+    for (int k = 0; k < K; ++k) {
+        const long long i0 = at + (wave * K + k) * kGroup, i = i0 + lane * 4;
+        Held<T> &h = held[k];
+        h = Held<T>{};
+        if (i0 >= t.count) continue;
+        const T *p = (const T *)t.p + i, *g = (const T *)t.g + i;
+        const unsigned char *mc = (const unsigned char *)t.m + i, *vc = (const unsigned char *)t.v + i;
+        h.mb = t.mb[i0 / kGroup];
+        h.vb = t.vb[i0 / kGroup];
+        if (aligned && i + 4 <= t.count) {
+            h.p = *(const Vec<T, 4> *)p;
+            h.g = *(const Vec<T, 4> *)g;
+            h.m = *(const Vec<unsigned char, 4> *)mc;
+            h.v = *(const Vec<unsigned char, 4> *)vc;
         } else {
-            for (int e = 0; e < n; ++e) {
-                pv.v[e] = p[e];
-                gv.v[e] = g[e];
-                mv.v[e] = mc[e];
-                vv.v[e] = vc[e];
+            for (int e = 0; e < 4 && i + e < t.count; ++e) {
+                h.p.v[e] = p[e];
+                h.g.v[e] = g[e];
+                h.m.v[e] = mc[e];
+                h.v.v[e] = vc[e];
             }
         }
-        const int mb = t.mb[group], vb = t.vb[group];
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i0 = at + (wave * K + k) * kGroup, i = i0 + lane * 4, group = i0 / kGroup;
+        if (i0 >= t.count) break;
+        Held<T> &h = held[k];
         float m[4], v[4];
         unsigned top_m = 0, top_v = 0;
+        // (elements behind the tensor's end are zeros all through: they do not raise the largest)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x = to_f32(pv.v[e]);
-            m[e] = decode_signed(mv.v[e], mb);
-            v[e] = decode(vv.v[e], vb);
-            update(x, to_f32(gv.v[e]), m[e], v[e], c);
-            pv.v[e] = from_f32<T>(x);
-            if (e < n) {
-                const unsigned a = __float_as_uint(fabsf(m[e])), q = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-                top_m = a > top_m ? a : top_m;
-                top_v = q > top_v ? q : top_v;
-            }
+            float x = to_f32(h.p.v[e]);
+            m[e] = decode_signed(h.m.v[e], h.mb);
+            v[e] = decode(h.v.v[e], h.vb);
+            update(x, to_f32(h.g.v[e]), m[e], v[e], c);
+            h.p.v[e] = from_f32<T>(x);
+            const unsigned a = __float_as_uint(fabsf(m[e])), q = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+            top_m = a > top_m ? a : top_m;
+            top_v = q > top_v ? q : top_v;
         }
         const int nmb = base_for(wave_max(top_m), 127), nvb = base_for(wave_max(top_v), 255);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const unsigned z = noise((place + (unsigned)group) * (unsigned)kGroup + lane * 4 + e + c.key);
-            mv.v[e] = (unsigned char)encode_signed(m[e], nmb, z & 0xFFFFu);
-            vv.v[e] = (unsigned char)encode(v[e], nvb, z >> 16);
+            h.m.v[e] = (unsigned char)encode_signed(m[e], nmb, z & 0xFFFFu);
+            h.v.v[e] = (unsigned char)encode(v[e], nvb, z >> 16);
         }
-        if (whole) {
-            *(Vec<T, 4> *)p = pv;
-            *(Vec<unsigned char, 4> *)mc = mv;
-            *(Vec<unsigned char, 4> *)vc = vv;
+        T *p = (T *)t.p + i;
+        unsigned char *mc = (unsigned char *)t.m + i, *vc = (unsigned char *)t.v + i;
+        if (aligned && i + 4 <= t.count) {
+            *(Vec<T, 4> *)p = h.p;
+            *(Vec<unsigned char, 4> *)mc = h.m;
+            *(Vec<unsigned char, 4> *)vc = h.v;
         } else {
-            for (int e = 0; e < n; ++e) {
-                p[e] = pv.v[e];
-                mc[e] = mv.v[e];
-                vc[e] = vv.v[e];
+            for (int e = 0; e < 4 && i + e < t.count; ++e) {
+                p[e] = h.p.v[e];
+                mc[e] = h.m.v[e];
+                vc[e] = h.v.v[e];
             }
         }
         if (lane == 0) {
@@ -290,7 +311,6 @@ int in_batches(const artemis_ops_tensor *tensors, int n, const char *what, F lau
 {
     Batch b;
     b.n = 0;
-    b.place = 0;
     long long blocks = 0;
     unsigned place = 0;
     constexpr long long kMost = 1 << 22;
@@ -308,7 +328,7 @@ int in_batches(const artemis_ops_tensor *tensors, int n, const char *what, F lau
         const long long need = (t.count + kShare - 1) / kShare;
         if (b.n == kTensors || blocks + need > kMost)
             if (int rc = flush()) return rc;
-        if (b.n == 0) b.place = place;
+        b.place[b.n] = place;
         b.t[b.n] = t;
         b.first[b.n] = (int)blocks;
         ++b.n;

@@ -5,11 +5,34 @@
 namespace aops {
 namespace {
 
-// by_head[head][entry] = table[entry][head] * log2(e)
-__global__ void bias_rows(const float *__restrict__ table, float *__restrict__ by_head, int entries, int heads)
+// bias[head][entry] = table[entry][head] * log2(e), and every head's entries in reverse
+__global__ __launch_bounds__(256) void bias_rows(const float *__restrict__ table, float *__restrict__ bias,
+                                                 float *__restrict__ rev, int entries, int heads)
 {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < entries * heads) by_head[(size_t)(i % heads) * entries + i / heads] = table[i] * kLog2e;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= entries * heads) return;
+    const int e = i / heads, head = i % heads;
+    const float v = table[i] * kLog2e;
+    bias[(size_t)head * entries + e] = v;
+    rev[(size_t)head * entries + entries - 1 - e] = v;
+}
+
+// Long windows: where the tokens of a window lie, and what the tiles of 64 tokens hold.  A wave for a tile.
+__global__ __launch_bounds__(256) void places_of(const WindowArgs a, const int *__restrict__ labels, int tiles,
+                                                 PlaceAt *__restrict__ places, TileAt *__restrict__ tiles_at)
+{
+    const long long tile = blockIdx.x * 4LL + threadIdx.x / 64;
+    if (tile >= a.windows * tiles) return;  // (a whole wave)
+    const int lane = threadIdx.x % 64, t = (int)(tile % tiles) * 64 + lane;
+    PlaceAt p{-1, 0, -1, 0};
+    if (t < a.n) {
+        const Place at = place_of(a, labels, tile / tiles, t);
+        p = PlaceAt{at.token, corner(a, t), at.label, at.wrap};
+    }
+    places[tile * 64 + lane] = p;
+    const int label = __shfl(p.label, 0), wrap = __shfl(p.wrap, 0);
+    const bool even = __all(p.label >= 0 && p.label == label && p.wrap == wrap), dead = __all(p.label < 0);
+    if (lane == 0) tiles_at[tile] = TileAt{dead ? kDead : even ? kEven : kMixed, label, wrap, 0};
 }
 
 // dense[head][e] = the sum of the shares of the workgroups that have that head, in a fixed order: 16 elements for a
@@ -58,7 +81,41 @@ __global__ __launch_bounds__(256) void table_small(const WindowArgs a, const flo
     if (lane == 0) dtable[(size_t)e * a.heads + head] = s;
 }
 
-// dtable[e][head] for long windows: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
+// dtable[e][head] for long windows that tiles of ed x eh x ew = 64 tokens divide: dense is [chunk][distance of tiles]
+// [head][64][64] (long_bwd_pairs).  For each query of a tile the key at this distance is one token of one tile: 64 terms for
+// each chunk.  Neighbouring lanes have neighbouring distances: they read neighbouring keys.
+__global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const PairWork w, const float *__restrict__ dense,
+                                                   float *__restrict__ dtable, int distances)
+{
+    const int e = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
+    if (e >= a.entries) return;
+    const int ed = a.wd / w.gd, eh = a.wh / w.gh, ew = a.ww / w.gw;
+    const int dw = e % a.rh - (a.ww - 1), dh = e / a.rh % (2 * a.wh - 1) - (a.wh - 1), dd = e / a.rd - (a.wd - 1);
+    // distance d of tokens i - k: tiles D = (d - i + k) / e apart, with k = (i - d) mod e
+    auto split = [](int i, int d, int size, int &k, int &D) {
+        int r = (i - d) % size;
+        k = r < 0 ? r + size : r;
+        D = (d - i + k) / size;
+    };
+    auto fold = [](int D) { return D > 0 ? 2 * D - 1 : -2 * D; };  // 0, 1, -1, 2, -2, ... -> 0, 1, 2, 3, 4
+    float s = 0.f;
+    for (int chunk = 0; chunk < w.chunks; ++chunk) {
+#pragma unroll 8
+        for (int q = 0; q < 64; ++q) {
+            const int x = q % ew, y = q / ew % eh, z = q / ew / eh;
+            int kx, ky, kz, Dx, Dy, Dz;
+            split(x, dw, ew, kx, Dx);
+            split(y, dh, eh, ky, Dy);
+            split(z, dd, ed, kz, Dz);
+            if (abs(Dx) >= w.gw || abs(Dy) >= w.gh || abs(Dz) >= w.gd) continue;  // out of the window for every tile
+            const int at = (fold(Dz) * (2 * w.gh - 1) + fold(Dy)) * (2 * w.gw - 1) + fold(Dx);
+            s += dense[((((size_t)chunk * distances + at) * a.heads + head) * 64 + q) * 64 + (kz * eh + ky) * ew + kx];
+        }
+    }
+    dtable[(size_t)e * a.heads + head] = s;
+}
+
+// dtable[e][head] for other long windows, from dense [head][n][n]: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
 // lane has one dw, so that neighbouring lanes read neighbouring keys.  Four waves take every fourth row.
 __global__ __launch_bounds__(256) void table_long(const WindowArgs a, const float *__restrict__ dense,
                                                   float *__restrict__ dtable)
@@ -147,8 +204,29 @@ int make_args(const char *what, const artemis_ops_window *w, WindowArgs &a)
     return a.windows == 0 ? -1 : 0;
 }
 
+// How the table's gradient goes through a long window's pairs (long_bwd_pairs): 64 tokens in a row of the raster that fill
+// whole rows, or whole planes, evenly; and shares of the windows until there is work for about 2048 workgroups.
+PairWork pair_work(const WindowArgs &a)
+{
+    PairWork w{0, 0, 0, 1};
+    const int plane = a.wh * a.ww;
+    if (a.ww % 64 == 0)
+        w = {a.wd, a.wh, a.ww / 64, 1};
+    else if (64 % a.ww == 0 && a.wh % (64 / a.ww) == 0)
+        w = {a.wd, a.wh / (64 / a.ww), 1, 1};
+    else if (64 % plane == 0 && a.wd % (64 / plane) == 0)
+        w = {a.wd / (64 / plane), 1, 1, 1};
+    if (w.gd) {
+        const long long groups = (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads;
+        const long long want = 2048 / groups;
+        w.chunks = (int)(want < 1 ? 1 : want < a.windows ? want : a.windows);
+    }
+    return w;
+}
+
 struct Layout {
-    size_t bias, pairs, dense, delta, total;
+    size_t bias, rev, places, tiles, pairs, dense, delta, total;
+    PairWork work;
 };
 Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool table)
 {
@@ -159,17 +237,25 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
         at += round16(bytes);
         return here;
     };
-    const bool is_long = a.n > 64;
-    const int nb = small_nb(a.n);
-    if (is_long && table) l.bias = take((size_t)a.entries * a.heads * 4);
-    if (backward && is_long) l.delta = take((size_t)a.windows * a.heads * a.n * 4);
-    if (backward && need_dtable) {
-        if (is_long) {
-            l.dense = take((size_t)a.heads * a.n * a.n * 4);
-        } else {
-            l.pairs = take((size_t)bwd_groups(a) * 64 * 16 * nb * 4);
-            l.dense = take((size_t)a.heads * 64 * 16 * nb * 4);
+    if (a.n > 64) {
+        const size_t tiles = (size_t)(a.n + 63) / 64;
+        l.places = take(a.windows * tiles * 64 * sizeof(PlaceAt));
+        l.tiles = take(a.windows * tiles * sizeof(TileAt));
+        if (table) {
+            l.bias = take((size_t)a.entries * a.heads * 4);
+            l.rev = take((size_t)a.entries * a.heads * 4);
         }
+        if (backward) l.delta = take((size_t)a.windows * a.heads * a.n * 4);
+        if (backward && need_dtable) {
+            l.work = pair_work(a);
+            const PairWork &w = l.work;
+            l.dense = take(w.gd ? (size_t)w.chunks * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
+                                : (size_t)a.heads * a.n * a.n * 4);
+        }
+    } else if (backward && need_dtable) {
+        const int nb = small_nb(a.n);
+        l.pairs = take((size_t)bwd_groups(a) * 64 * 16 * nb * 4);
+        l.dense = take((size_t)a.heads * 64 * 16 * nb * 4);
     }
     l.total = at;
     return l;
@@ -177,11 +263,25 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
 
 bool aligned4(const void *p, int dtype) { return ((size_t)p & (dtype == ARTEMIS_OPS_F32 ? 15 : 7)) == 0; }
 
-int rows_of_bias(const WindowArgs &a, const float *table, float *by_head, hipStream_t st)
+// Long windows: fills the maps in the workspace
+LongMap long_map(const WindowArgs &a, const Layout &l, const float *table, const int *labels, char *ws, hipStream_t st)
 {
-    const int n = a.entries * a.heads;
-    hipLaunchKernelGGL(bias_rows, dim3((n + 255) / 256), dim3(256), 0, st, table, by_head, a.entries, a.heads);
-    return 0;
+    LongMap m{};
+    m.tiles = (a.n + 63) / 64;
+    PlaceAt *places = (PlaceAt *)(ws + l.places);
+    TileAt *tiles = (TileAt *)(ws + l.tiles);
+    m.places = places;
+    m.tiles_at = tiles;
+    hipLaunchKernelGGL(places_of, dim3((unsigned)((a.windows * m.tiles + 3) / 4)), dim3(256), 0, st, a, labels, m.tiles, places,
+                       tiles);
+    if (table) {
+        float *bias = (float *)(ws + l.bias), *rev = (float *)(ws + l.rev);
+        const int n = a.entries * a.heads;
+        hipLaunchKernelGGL(bias_rows, dim3((n + 255) / 256), dim3(256), 0, st, table, bias, rev, a.entries, a.heads);
+        m.bias = bias;
+        m.rev = rev;
+    }
+    return m;
 }
 
 }  // namespace
@@ -227,10 +327,7 @@ int artemis_ops_window_attention_forward(const artemis_ops_window *w, const void
     b.out = out;
     b.lse = lse;
     b.groups = a.n <= 64 ? fwd_groups(a) : 0;
-    if (a.n > 64 && table) {
-        b.bias_by_head = (float *)((char *)workspace + l.bias);
-        rows_of_bias(a, table, (float *)((char *)workspace + l.bias), st);
-    }
+    if (a.n > 64) b.map = long_map(a, l, table, labels, (char *)workspace, st);
     if (w->dtype == ARTEMIS_OPS_F32)
         launch_attention_fwd<float>(a, b, st);
     else if (w->dtype == ARTEMIS_OPS_BF16)
@@ -278,17 +375,19 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
         b.dense = (float *)(ws + l.dense);
         if (!is_long) b.pairs = (float *)(ws + l.pairs);
     }
-    if (is_long && table) {
-        b.bias_by_head = (float *)(ws + l.bias);
-        rows_of_bias(a, table, (float *)(ws + l.bias), st);
-    }
+    if (is_long) b.map = long_map(a, l, table, labels, ws, st);
+    b.work = l.work;
     if (w->dtype == ARTEMIS_OPS_F32)
         launch_attention_bwd<float>(a, b, st);
     else if (w->dtype == ARTEMIS_OPS_BF16)
         launch_attention_bwd<__bf16>(a, b, st);
     else
         launch_attention_bwd<_Float16>(a, b, st);
-    if (dtable && is_long) {
+    if (dtable && is_long && b.work.gd) {
+        const int distances = (2 * b.work.gd - 1) * (2 * b.work.gh - 1) * (2 * b.work.gw - 1);
+        hipLaunchKernelGGL(table_tiled, dim3((a.entries + 255) / 256, a.heads), dim3(256), 0, st, a, b.work, b.dense, dtable,
+                           distances);
+    } else if (dtable && is_long) {
         hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st,
                            a, b.dense, dtable);
     } else if (dtable) {

@@ -41,6 +41,10 @@ struct Mma<float> {
         c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[2], b[2], c, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_16x16x4f32(a[3], b[3], c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 run2(Frag a0, Frag a1, Frag b0, Frag b1, f32x4 c)
+    {
+        return run(a1, b1, run(a0, b0, c));
+    }
     static __device__ __forceinline__ Frag frag(f32x4 v) { return v; }
 };
 template <>
@@ -49,6 +53,12 @@ struct Mma<__bf16> {
     static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    }
+    // two block products at once, depth 32: any order of the contraction will do, as long as a and b share it
+    static __device__ __forceinline__ f32x4 run2(Frag a0, Frag a1, Frag b0, Frag b1, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7),
+                                                       __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7), c, 0, 0, 0);
     }
     static __device__ __forceinline__ Frag frag(f32x4 v)
     {
@@ -61,6 +71,11 @@ struct Mma<_Float16> {
     static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 run2(Frag a0, Frag a1, Frag b0, Frag b1, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7),
+                                                      __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7), c, 0, 0, 0);
     }
     static __device__ __forceinline__ Frag frag(f32x4 v)
     {
@@ -450,105 +465,225 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
 
 // ================================================================================================
 // Longer windows (65 .. 4096 tokens): tiles of 64 queries against tiles of 64 keys, with the running maximum and sum
-// of a softmax over the key tiles.  The bias comes from a copy of the table with one head's entries in a row.
+// of a softmax over the key tiles.  A head's scores take about nine vector instructions for each pair beside its
+// products (scale and bias, maximum, exponential, sum, rounding), against 4 hd / 1024 matrix instructions: for the
+// model's 32 channels the vector units bound it, so the pair loop holds nothing else --
+//  * where tokens lie and what region they are of is written once for each call (`places`, `tiles`): a pair of
+//    tiles of one region needs no mask, one of two regions that never meet is skipped with its loads;
+//  * the bias comes from a copy of the table with one head's entries in a row, forwards and backwards, so that four
+//    neighbouring keys (or queries) have neighbouring entries: one load of 16 bytes where rows of the window are
+//    multiples of 4;
+//  * the next tile's rows are in flight while this one is used, and what is contracted over tokens lies in LDS
+//    transposed, so that an operand is one read.
 // ================================================================================================
+
+struct PlaceAt {
+    int token, corner, label, wrap;  // token -1: none (behind the window's end); label < 0: padding
+};
+struct TileAt {
+    int state, label, wrap, unused;  // kMixed; kEven: 64 live tokens of one region; kDead: no live token
+};
+constexpr int kMixed = 0, kEven = 1, kDead = 2;
+
+struct LongMap {
+    const PlaceAt *places;   // (windows, tiles * 64)
+    const TileAt *tiles_at;  // (windows, tiles)
+    const float *bias;       // (heads, entries) * log2 e, or NULL
+    const float *rev;        // the same, every head's entries in reverse
+    int tiles;               // of 64 tokens in a window, at most 64
+};
 
 struct LongTile {
     long long window;
-    int head, first;  // the tile's first token
+    int head, tile;
 };
-__device__ __forceinline__ LongTile long_tile(const WindowArgs &a)
+__device__ __forceinline__ LongTile long_tile(const WindowArgs &a, int tiles)
 {
-    const unsigned tiles = (unsigned)(a.n + 63) / 64;
-    const unsigned t = blockIdx.x % tiles, r = blockIdx.x / tiles;
-    return {(long long)(r / (unsigned)a.heads), (int)(r % (unsigned)a.heads), (int)t * 64};
+    const unsigned t = blockIdx.x % (unsigned)tiles, r = blockIdx.x / (unsigned)tiles;
+    return {(long long)(r / (unsigned)a.heads), (int)(r % (unsigned)a.heads), (int)t};
 }
 
-struct TokenRow {
-    int token[64], label[64], wrap[64], corner[64];
-    __device__ __forceinline__ void fill(const WindowArgs &a, const int *labels, long long window, int first, int s)
+// Which tiles a tile meets, one bit each (every lane of a wave looks at one tile)
+struct Meets {
+    unsigned long long any, mixed;
+};
+__device__ __forceinline__ Meets meets(const LongMap &m, long long window, int tile, float outside2)
+{
+    const TileAt *row = m.tiles_at + window * m.tiles;
+    const TileAt own = row[tile];
+    const int lane = threadIdx.x % 64;
+    TileAt other{kDead, 0, 0, 0};
+    if (lane < m.tiles) other = row[lane];
+    const bool even = own.state == kEven && other.state == kEven;
+    const bool same = own.label == other.label && own.wrap == other.wrap;
+    const bool any = own.state != kDead && other.state != kDead && !(even && !same && outside2 == -INFINITY);
+    return {__ballot(any), __ballot(any && !(even && same))};
+}
+
+// 64 rows on their way to LDS: HD / 16 pieces of four channels in each thread
+template <class T, int HD>
+struct Rows {
+    using Frag = typename Mma<T>::Frag;
+    static constexpr int kPieces = HD / 16, kRowStep = kAttnThreads / (HD / 4);
+    Frag f[kPieces];
+    static __device__ __forceinline__ int row(int m) { return threadIdx.x / (HD / 4) + m * kRowStep; }
+    static __device__ __forceinline__ int channel() { return threadIdx.x % (HD / 4) * 4; }
+    __device__ __forceinline__ void load(const T *__restrict__ base, long long stride, const int (&token)[kPieces], int hd)
     {
-        Place p{-1, -1, 0};
-        int c = 0;
-        if (first + s < a.n) {
-            p = place_of(a, labels, window, first + s);
-            c = ::aops::corner(a, first + s);
-        }
-        token[s] = p.token;
-        label[s] = p.token < 0 ? -1 : p.label;
-        wrap[s] = p.wrap;
-        corner[s] = c;
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) f[m] = load4<T>(base, stride, token[m], channel(), hd);
+    }
+    __device__ __forceinline__ void store_rows(T *tile) const  // [64][HD + 4]
+    {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) *(Frag *)&tile[row(m) * (HD + 4) + channel()] = f[m];
+    }
+    __device__ __forceinline__ void store_columns(T *tile) const  // [HD][64 + 4]
+    {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tile[(channel() + e) * 68 + row(m)] = f[m][e];
     }
 };
 
+// the tokens of a tile's rows as a thread stages them (-1: zeros)
 template <class T, int HD>
-__device__ __forceinline__ void stage(T *tile, const T *__restrict__ base, long long stride, const TokenRow &row, int hd)
+__device__ __forceinline__ void tokens_of(const PlaceAt *tile, int (&token)[Rows<T, HD>::kPieces])
 {
-    constexpr int STRIDE = HD + 4;
-    for (int k = threadIdx.x; k < 64 * (HD / 4); k += kAttnThreads) {
-        const int s = k / (HD / 4), c = k % (HD / 4) * 4;
-        *(typename Mma<T>::Frag *)&tile[s * STRIDE + c] = load4<T>(base, stride, row.label[s] < 0 ? -1 : row.token[s], c, hd);
+#pragma unroll
+    for (int m = 0; m < Rows<T, HD>::kPieces; ++m) {
+        const PlaceAt p = tile[Rows<T, HD>::row(m)];
+        token[m] = p.label < 0 ? -1 : p.token;
     }
 }
 
+// D[token 4g ..][column i] for a block of 16 rows of a row-major tile against a lane's operand: contraction over channels
 template <class T, int HD>
-__global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, const T *__restrict__ qkv,
-                                                         const float *__restrict__ bias_by_head,
-                                                         const int *__restrict__ labels, T *__restrict__ out,
-                                                         float *__restrict__ lse)
+__device__ __forceinline__ f32x4 over_channels(const T *rows, int first, const typename Mma<T>::Frag *own)
+{
+    using M = Mma<T>;
+    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+    const T *p = rows + (first + i) * (HD + 4) + 4 * g;
+    f32x4 acc{};
+    if constexpr (HD >= 32) {
+#pragma unroll
+        for (int c = 0; c < HD / 16; c += 2) acc = M::run2(row4<T>(p + c * 16), row4<T>(p + c * 16 + 16), own[c], own[c + 1], acc);
+    } else {
+        acc = M::run(row4<T>(p), own[0], acc);
+    }
+    return acc;
+}
+
+// acc[c] += columns^T (channels c * 16 ..) times four blocks of B operands: contraction over 64 tokens
+template <class T, int HD>
+__device__ __forceinline__ void over_tokens(f32x4 (&acc)[HD / 16], const T *columns, const typename Mma<T>::Frag (&b)[4])
+{
+    using M = Mma<T>;
+    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) {
+        const T *p = columns + (c * 16 + i) * 68 + 4 * g;
+        acc[c] = M::run2(row4<T>(p), row4<T>(p + 16), b[0], b[1], acc[c]);
+        acc[c] = M::run2(row4<T>(p + 32), row4<T>(p + 48), b[2], b[3], acc[c]);
+    }
+}
+
+// Four neighbouring bias entries.  VEC: they lie behind each other in `table` (rows of the window are multiples of 4).
+template <bool VEC>
+__device__ __forceinline__ f32x4 four_biases(const float *__restrict__ table, int own, const PlaceAt *at)
+{
+    f32x4 b{};
+    if (!table) return b;
+    if constexpr (VEC) {
+        struct __attribute__((packed, aligned(4))) Loose {
+            f32x4 v;
+        };
+        b = ((const Loose *)(table + own + at[0].corner))->v;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[r] = table[own + at[r].corner];
+    }
+    return b;
+}
+
+// the scores of four pairs in the exponent of 2
+__device__ __forceinline__ f32x4 scores(f32x4 acc, float scale2, f32x4 bias, bool mixed, const PlaceAt &own, const PlaceAt *at,
+                                        float outside2)
+{
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = acc[r] * scale2 + bias[r];
+    if (mixed) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = masked(x[r], own.label, own.wrap, at[r].label, at[r].wrap, outside2);
+    }
+    return x;
+}
+
+template <class T, int HD, bool VEC>
+__global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, const LongMap map, const T *__restrict__ qkv,
+                                                         T *__restrict__ out, float *__restrict__ lse)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int STRIDE = HD + 4;
+    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
-    __shared__ __align__(16) T Ks[64 * STRIDE];
-    __shared__ __align__(16) T Vs[64 * STRIDE];
-    __shared__ TokenRow qrow, krow;
+    __shared__ __align__(16) T Ks[64 * (HD + 4)];
+    __shared__ __align__(16) T Vt[HD * 68];
+    __shared__ __align__(16) PlaceAt at_s[64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
-    const LongTile lt = long_tile(a);
+    const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
-    const float *bias = bias_by_head ? bias_by_head + (size_t)lt.head * a.entries : nullptr;
-    if (threadIdx.x < 64) qrow.fill(a, labels, lt.window, lt.first, threadIdx.x);
-    __syncthreads();
-    const int mine = qrow.token[q], ql = qrow.label[q], qr = qrow.wrap[q], qc = qrow.corner[q] + middle(a);
+    const float *rev = map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr;
+    const PlaceAt *window = map.places + lt.window * map.tiles * 64;
+    const PlaceAt own = window[lt.tile * 64 + q];
+    const int at0 = middle(a) - own.corner;  // entry of the reversed row: middle - corner(q) + corner(k)
     Frag qf[CB];
 #pragma unroll
-    for (int c = 0; c < CB; ++c) qf[c] = load4<T>(base, stride, ql < 0 ? -1 : mine, c * 16 + 4 * g, a.hd);
+    for (int c = 0; c < CB; ++c) qf[c] = load4<T>(base, stride, own.label < 0 ? -1 : own.token, c * 16 + 4 * g, a.hd);
     const float scale2 = a.scale * kLog2e;
     float top = -INFINITY, sum = 0.f;
     f32x4 o[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) o[c] = f32x4{};
-    for (int k0 = 0; k0 < a.n; k0 += 64) {
+    const Meets meet = meets(map, lt.window, lt.tile, a.outside2);
+    unsigned long long todo = meet.any;
+    R kr, vr;
+    PlaceAt at{};
+    int token[R::kPieces];
+    auto fetch = [&](int t) {
+        tokens_of<T, HD>(window + t * 64, token);
+        kr.load(base + C, stride, token, a.hd);
+        vr.load(base + 2 * C, stride, token, a.hd);
+        if (threadIdx.x < 64) at = window[t * 64 + threadIdx.x];
+    };
+    if (todo) fetch(__builtin_ctzll(todo));
+    while (todo) {
+        const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
+        todo &= todo - 1;
+        __syncthreads();  // the tile before has been used
+        kr.store_rows(Ks);
+        vr.store_columns(Vt);
+        if (threadIdx.x < 64) at_s[threadIdx.x] = at;
+        if (todo) fetch(__builtin_ctzll(todo));
         __syncthreads();
-        if (threadIdx.x < 64) krow.fill(a, labels, lt.window, k0, threadIdx.x);
-        __syncthreads();
-        stage<T, HD>(Ks, base + C, stride, krow, a.hd);
-        stage<T, HD>(Vs, base + 2 * C, stride, krow, a.hd);
-        __syncthreads();
-        f32x4 s[4];
-        float high = -INFINITY;
+        f32x4 s[4], bias[4];
+        float high = top;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = four_biases<VEC>(rev, at0, &at_s[j * 16 + 4 * g]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 acc{};
+            s[j] = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g], a.outside2);
 #pragma unroll
-            for (int c = 0; c < CB; ++c) acc = M::run(row4<T>(&Ks[(j * 16 + i) * STRIDE + c * 16 + 4 * g]), qf[c], acc);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = j * 16 + 4 * g + r;
-                float x = acc[r] * scale2;
-                if (bias) x += bias[qc - krow.corner[key]];
-                x = masked(x, ql, qr, krow.label[key], krow.wrap[key], a.outside2);
-                s[j][r] = x;
-                high = fmaxf(high, x);
-            }
+            for (int r = 0; r < 4; ++r) high = fmaxf(high, s[j][r]);
         }
-        high = fmaxf(fold_max(high), top);
-        const float at = high == -INFINITY ? 0.f : high;
-        const float fade = exp2f(top - at);
+        high = fold_max(high);
+        const float base2 = high == -INFINITY ? 0.f : high;
+        const float fade = __builtin_amdgcn_exp2f(top - base2);
         top = high;
         float part = 0.f;
         Frag p[4];
@@ -556,59 +691,55 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[j][r] = exp2f(s[j][r] - at);
+                s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - base2);
                 part += s[j][r];
             }
-            p[j] = M::frag(s[j]);
+            p[j] = M::frag(s[j]);  // 16 bit: rounded as the product takes it, the sum is of the unrounded ones
         }
         sum = sum * fade + part;
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-            o[c] *= fade;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[c] = M::run(column<T, STRIDE>(Vs, j * 16 + 4 * g, c * 16 + i), p[j], o[c]);
-        }
+        for (int c = 0; c < CB; ++c) o[c] *= fade;
+        over_tokens<T, HD>(o, Vt, p);
     }
     sum = fold_sum(sum);
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-    if (mine < 0) return;
+    if (own.token < 0) return;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
         if (c * 16 + 4 * g < a.hd)
-            *(Frag *)(out + (size_t)mine * C + lt.head * a.hd + c * 16 + 4 * g) = M::frag(o[c] * inv);
+            *(Frag *)(out + (size_t)own.token * C + lt.head * a.hd + c * 16 + 4 * g) = M::frag(o[c] * inv);
     // log2 of the row's sum of 2^x; +inf for an empty row, so that its P is 0 in the backward pass
     if (lse && g == 0)
-        lse[((size_t)lt.window * a.heads + lt.head) * a.n + lt.first + q] = top == -INFINITY ? INFINITY : top + log2f(sum);
+        lse[((size_t)lt.window * a.heads + lt.head) * a.n + lt.tile * 64 + q] = top == -INFINITY ? INFINITY : top + log2f(sum);
 }
 
 // dQ, and delta = sum over keys of P dP for each query.  delta is also the product of out and dout; in 16 bits `out` is
 // rounded, so that product c is only near: dS = P (dP - c) serves dQ, which is rounded as coarsely itself, and
 // c + sum P (dP - c), summed here in fp32, is the delta that the table's gradient and dK are computed with.
-template <class T, int HD>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, const T *__restrict__ qkv,
-                                                           const float *__restrict__ bias_by_head,
-                                                           const int *__restrict__ labels, const T *__restrict__ out,
-                                                           const float *__restrict__ lse, const T *__restrict__ dout,
-                                                           T *__restrict__ dqkv, float *__restrict__ delta)
+template <class T, int HD, bool VEC>
+__global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, const LongMap map, const T *__restrict__ qkv,
+                                                           const T *__restrict__ out, const float *__restrict__ lse,
+                                                           const T *__restrict__ dout, T *__restrict__ dqkv,
+                                                           float *__restrict__ delta)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int STRIDE = HD + 4;
+    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
-    __shared__ __align__(16) T Ks[64 * STRIDE];
-    __shared__ __align__(16) T Vs[64 * STRIDE];
-    __shared__ TokenRow qrow, krow;
+    __shared__ __align__(16) T Ks[64 * (HD + 4)];
+    __shared__ __align__(16) T Kt[HD * 68];
+    __shared__ __align__(16) T Vs[64 * (HD + 4)];
+    __shared__ __align__(16) PlaceAt at_s[64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
-    const LongTile lt = long_tile(a);
+    const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
-    const float *bias = bias_by_head ? bias_by_head + (size_t)lt.head * a.entries : nullptr;
-    if (threadIdx.x < 64) qrow.fill(a, labels, lt.window, lt.first, threadIdx.x);
-    __syncthreads();
-    const int mine = qrow.token[q], ql = qrow.label[q], qr = qrow.wrap[q], qc = qrow.corner[q] + middle(a);
-    const int live = ql < 0 ? -1 : mine;
+    const float *rev = map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr;
+    const PlaceAt *window = map.places + lt.window * map.tiles * 64;
+    const PlaceAt own = window[lt.tile * 64 + q];
+    const int at0 = middle(a) - own.corner, live = own.label < 0 ? -1 : own.token;
     Frag qf[CB], gf[CB];
     float near = 0.f;
 #pragma unroll
@@ -620,84 +751,92 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
         for (int r = 0; r < 4; ++r) near += (float)of[r] * (float)gf[c][r];
     }
     near = fold_sum(near);
-    const size_t line = ((size_t)lt.window * a.heads + lt.head) * a.n + lt.first + q;
-    const float shift = mine >= 0 ? lse[line] : INFINITY;
+    const size_t line = ((size_t)lt.window * a.heads + lt.head) * a.n + lt.tile * 64 + q;
+    const float shift = own.token >= 0 ? lse[line] : INFINITY;
     const float scale2 = a.scale * kLog2e;
     float rest = 0.f;
     f32x4 dq[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
-    for (int k0 = 0; k0 < a.n; k0 += 64) {
+    const Meets meet = meets(map, lt.window, lt.tile, a.outside2);
+    unsigned long long todo = meet.any;
+    R kr, vr;
+    PlaceAt at{};
+    int token[R::kPieces];
+    auto fetch = [&](int t) {
+        tokens_of<T, HD>(window + t * 64, token);
+        kr.load(base + C, stride, token, a.hd);
+        vr.load(base + 2 * C, stride, token, a.hd);
+        if (threadIdx.x < 64) at = window[t * 64 + threadIdx.x];
+    };
+    if (todo) fetch(__builtin_ctzll(todo));
+    while (todo) {
+        const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
+        todo &= todo - 1;
         __syncthreads();
-        if (threadIdx.x < 64) krow.fill(a, labels, lt.window, k0, threadIdx.x);
+        kr.store_rows(Ks);
+        kr.store_columns(Kt);
+        vr.store_rows(Vs);
+        if (threadIdx.x < 64) at_s[threadIdx.x] = at;
+        if (todo) fetch(__builtin_ctzll(todo));
         __syncthreads();
-        stage<T, HD>(Ks, base + C, stride, krow, a.hd);
-        stage<T, HD>(Vs, base + 2 * C, stride, krow, a.hd);
-        __syncthreads();
+        f32x4 bias[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = four_biases<VEC>(rev, at0, &at_s[j * 16 + 4 * g]);
         Frag ds[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 acc{}, acc2{};
-#pragma unroll
-            for (int c = 0; c < CB; ++c) {
-                const int at = (j * 16 + i) * STRIDE + c * 16 + 4 * g;
-                acc = M::run(row4<T>(&Ks[at]), qf[c], acc);
-                acc2 = M::run(row4<T>(&Vs[at]), gf[c], acc2);
-            }
+            const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
+                                   a.outside2);
+            const f32x4 dp = over_channels<T, HD>(Vs, j * 16, gf);
             f32x4 d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int key = j * 16 + 4 * g + r;
-                float x = acc[r] * scale2;
-                if (bias) x += bias[qc - krow.corner[key]];
-                x = masked(x, ql, qr, krow.label[key], krow.wrap[key], a.outside2);
-                d[r] = x == -INFINITY ? 0.f : exp2f(x - shift) * (acc2[r] - near);
+                // (an empty row: -inf against +inf)
+                const float p = __builtin_amdgcn_exp2f(x[r] - shift);
+                d[r] = p * (dp[r] - near);
                 rest += d[r];
             }
             ds[j] = M::frag(d);
         }
-#pragma unroll
-        for (int c = 0; c < CB; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dq[c] = M::run(column<T, STRIDE>(Ks, j * 16 + 4 * g, c * 16 + i), ds[j], dq[c]);
+        over_tokens<T, HD>(dq, Kt, ds);
     }
     rest = fold_sum(rest);
-    if (mine < 0) return;
+    if (own.token < 0) return;
     if (g == 0) delta[line] = near + rest;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
         if (c * 16 + 4 * g < a.hd)
-            *(Frag *)(dqkv + (size_t)mine * stride + lt.head * a.hd + c * 16 + 4 * g) = M::frag(dq[c] * a.scale);
+            *(Frag *)(dqkv + (size_t)own.token * stride + lt.head * a.hd + c * 16 + 4 * g) = M::frag(dq[c] * a.scale);
 }
 
 // dK and dV: wave w has 16 keys and goes through the queries, S = Q K^T (rows: queries, lane: key), so that P and dS have the
 // layout of the B operands of dV^T = dO^T P and dK^T = Q^T dS.
-template <class T, int HD>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, const T *__restrict__ qkv,
-                                                            const float *__restrict__ bias_by_head,
-                                                            const int *__restrict__ labels,
+template <class T, int HD, bool VEC>
+__global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, const LongMap map, const T *__restrict__ qkv,
                                                             const float *__restrict__ lse, const T *__restrict__ dout,
                                                             T *__restrict__ dqkv, const float *__restrict__ delta)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int STRIDE = HD + 4;
+    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
-    __shared__ __align__(16) T Qs[64 * STRIDE];
-    __shared__ __align__(16) T Gs[64 * STRIDE];
-    __shared__ TokenRow qrow, krow;
-    __shared__ float lse_s[64], delta_s[64];
+    __shared__ __align__(16) T Qs[64 * (HD + 4)];
+    __shared__ __align__(16) T Qt[HD * 68];
+    __shared__ __align__(16) T Gs[64 * (HD + 4)];
+    __shared__ __align__(16) T Gt[HD * 68];
+    __shared__ __align__(16) PlaceAt at_s[64];
+    __shared__ __align__(16) float lse_s[64], delta_s[64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, k = wave * 16 + i;
-    const LongTile lt = long_tile(a);
+    const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
-    const T *base = qkv + (size_t)lt.head * a.hd;
-    const float *bias = bias_by_head ? bias_by_head + (size_t)lt.head * a.entries : nullptr;
-    if (threadIdx.x < 64) krow.fill(a, labels, lt.window, lt.first, threadIdx.x);
-    __syncthreads();
-    const int mine = krow.token[k], kl = krow.label[k], kr = krow.wrap[k], kc = middle(a) - krow.corner[k];
-    const int live = kl < 0 ? -1 : mine;
+    const T *base = qkv + (size_t)lt.head * a.hd, *gbase = dout + (size_t)lt.head * a.hd;
+    const float *bias_row = map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr;
+    const PlaceAt *window = map.places + lt.window * map.tiles * 64;
+    const PlaceAt own = window[lt.tile * 64 + k];
+    const int at0 = middle(a) - own.corner, live = own.label < 0 ? -1 : own.token;  // entry: corner(q) + middle - corner(k)
     Frag kf[CB], vf[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) {
@@ -709,136 +848,230 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     f32x4 dk[CB], dv[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
-    for (int q0 = 0; q0 < a.n; q0 += 64) {
-        __syncthreads();
+    const Meets meet = meets(map, lt.window, lt.tile, a.outside2);
+    unsigned long long todo = meet.any;
+    R qr, gr;
+    PlaceAt at{};
+    float shift = 0.f, del = 0.f;
+    int token[R::kPieces];
+    auto fetch = [&](int t) {
+        tokens_of<T, HD>(window + t * 64, token);
+        qr.load(base, stride, token, a.hd);
+        gr.load(gbase, C, token, a.hd);
         if (threadIdx.x < 64) {
-            qrow.fill(a, labels, lt.window, q0, threadIdx.x);
-            const bool in = q0 + (int)threadIdx.x < a.n;
-            lse_s[threadIdx.x] = in ? lse[lines + q0 + threadIdx.x] : INFINITY;
-            delta_s[threadIdx.x] = in ? delta[lines + q0 + threadIdx.x] : 0.f;
+            at = window[t * 64 + threadIdx.x];
+            const bool in = at.token >= 0;
+            shift = in ? lse[lines + t * 64 + threadIdx.x] : INFINITY;
+            del = in ? delta[lines + t * 64 + threadIdx.x] : 0.f;
         }
+    };
+    if (todo) fetch(__builtin_ctzll(todo));
+    while (todo) {
+        const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
+        todo &= todo - 1;
         __syncthreads();
-        stage<T, HD>(Qs, base, stride, qrow, a.hd);
-        stage<T, HD>(Gs, dout + (size_t)lt.head * a.hd, C, qrow, a.hd);
+        qr.store_rows(Qs);
+        qr.store_columns(Qt);
+        gr.store_rows(Gs);
+        gr.store_columns(Gt);
+        if (threadIdx.x < 64) {
+            at_s[threadIdx.x] = at;
+            lse_s[threadIdx.x] = shift;
+            delta_s[threadIdx.x] = del;
+        }
+        if (todo) fetch(__builtin_ctzll(todo));
         __syncthreads();
+        f32x4 bias[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = four_biases<VEC>(bias_row, at0, &at_s[j * 16 + 4 * g]);
+        Frag p[4], ds[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 acc{}, acc2{};
-#pragma unroll
-            for (int c = 0; c < CB; ++c) {
-                const int at = (j * 16 + i) * STRIDE + c * 16 + 4 * g;
-                acc = M::run(row4<T>(&Qs[at]), kf[c], acc);
-                acc2 = M::run(row4<T>(&Gs[at]), vf[c], acc2);
-            }
-            f32x4 p, d;
+            const f32x4 x = scores(over_channels<T, HD>(Qs, j * 16, kf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
+                                   a.outside2);
+            const f32x4 dp = over_channels<T, HD>(Gs, j * 16, vf);
+            const f32x4 l = *(const f32x4 *)&lse_s[j * 16 + 4 * g], del4 = *(const f32x4 *)&delta_s[j * 16 + 4 * g];
+            f32x4 pv, d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int q = j * 16 + 4 * g + r;
-                float x = acc[r] * scale2;
-                if (bias) x += bias[qrow.corner[q] + kc];
-                x = masked(x, qrow.label[q], qrow.wrap[q], kl, kr, a.outside2);
-                p[r] = x == -INFINITY ? 0.f : exp2f(x - lse_s[q]);
-                d[r] = p[r] * (acc2[r] - delta_s[q]);
+                pv[r] = __builtin_amdgcn_exp2f(x[r] - l[r]);
+                d[r] = pv[r] * (dp[r] - del4[r]);
             }
-            const Frag pf = M::frag(p), df = M::frag(d);
-#pragma unroll
-            for (int c = 0; c < CB; ++c) {
-                dv[c] = M::run(column<T, STRIDE>(Gs, j * 16 + 4 * g, c * 16 + i), pf, dv[c]);
-                dk[c] = M::run(column<T, STRIDE>(Qs, j * 16 + 4 * g, c * 16 + i), df, dk[c]);
-            }
+            p[j] = M::frag(pv);
+            ds[j] = M::frag(d);
         }
+        over_tokens<T, HD>(dv, Gt, p);
+        over_tokens<T, HD>(dk, Qt, ds);
     }
-    if (mine < 0) return;
+    if (own.token < 0) return;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
         if (c * 16 + 4 * g < a.hd) {
-            T *to = dqkv + (size_t)mine * stride + lt.head * a.hd + c * 16 + 4 * g;
+            T *to = dqkv + (size_t)own.token * stride + lt.head * a.hd + c * 16 + 4 * g;
             *(Frag *)(to + C) = M::frag(dk[c] * a.scale);
             *(Frag *)(to + 2 * C) = M::frag(dv[c]);
         }
 }
 
-// dense[head][query][key] = the sum of dS over the windows, for one tile of 64 x 64 pairs of one head
+// The table's gradient sums dS over all pairs of one distance.  Where 64 tokens tile the window evenly (ed x eh x ew tokens,
+// all three dividing the window's), the distances of a pair of tiles depend on the tiles' own distance alone: a
+// workgroup takes one distance of tiles and one head, goes through all such pairs of tiles of its share of the windows, and
+// adds their dS up in registers, where the bias is kept too.  64 x 64 sums for each distance of tiles are left.
+// Windows that 64 tokens do not tile: a workgroup takes one pair of tiles, and the sums are of n x n pairs.
+struct PairWork {
+    int gd, gh, gw;    // tiles along the axes; 0: not tiled evenly
+    int chunks;        // shares of the windows
+};
+
 template <class T, int HD>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs a, const T *__restrict__ qkv,
-                                                               const float *__restrict__ bias_by_head,
-                                                               const int *__restrict__ labels,
-                                                               const float *__restrict__ lse, const T *__restrict__ dout,
-                                                               const float *__restrict__ delta, float *__restrict__ dense)
+__global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs a, const LongMap map, const PairWork w,
+                                                               const T *__restrict__ qkv, const float *__restrict__ lse,
+                                                               const T *__restrict__ dout, const float *__restrict__ delta,
+                                                               float *__restrict__ dense)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int STRIDE = HD + 4;
+    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
-    __shared__ __align__(16) T Ks[64 * STRIDE];
-    __shared__ __align__(16) T Vs[64 * STRIDE];
-    __shared__ TokenRow qrow, krow;
+    __shared__ __align__(16) T Ks[64 * (HD + 4)];
+    __shared__ __align__(16) T Vs[64 * (HD + 4)];
+    __shared__ __align__(16) PlaceAt at_s[64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
-    const unsigned tiles = (unsigned)(a.n + 63) / 64;
-    const int k0 = (int)(blockIdx.x % tiles) * 64, q0 = (int)(blockIdx.x / tiles % tiles) * 64;
-    const int head = (int)(blockIdx.x / tiles / tiles);
+    const bool even = w.gd > 0;
+    // which tiles: query tile (z0 + z, y0 + y, x0 + x) against key tile (kz + z, ...), z < nz and so on
+    unsigned id = blockIdx.x;
+    const int chunk = (int)(id % (unsigned)w.chunks);
+    id /= (unsigned)w.chunks;
+    const int head = (int)(id % (unsigned)a.heads);
+    id /= (unsigned)a.heads;
+    int qt0, kt0, nz = 1, ny = 1, nx = 1;
+    if (even) {
+        // distances in the order 0, 1, -1, 2, -2, ...: the ones with most pairs first
+        auto unfold = [&](int n) {
+            const int u = (int)(id % (unsigned)(2 * n - 1));
+            id /= (unsigned)(2 * n - 1);
+            return u & 1 ? (u + 1) / 2 : -(u / 2);
+        };
+        const int dx = unfold(w.gw), dy = unfold(w.gh), dz = unfold(w.gd);
+        nz = w.gd - abs(dz), ny = w.gh - abs(dy), nx = w.gw - abs(dx);
+        qt0 = (max(dz, 0) * w.gh + max(dy, 0)) * w.gw + max(dx, 0);
+        kt0 = (max(-dz, 0) * w.gh + max(-dy, 0)) * w.gw + max(-dx, 0);
+    } else {
+        kt0 = (int)(id % (unsigned)map.tiles);
+        qt0 = (int)(id / (unsigned)map.tiles);
+    }
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
-    const T *base = qkv + (size_t)head * a.hd;
-    const float *bias = bias_by_head ? bias_by_head + (size_t)head * a.entries : nullptr;
+    const T *base = qkv + (size_t)head * a.hd, *gbase = dout + (size_t)head * a.hd;
     const float scale2 = a.scale * kLog2e;
-    f32x4 sum[4];
+    f32x4 sum[4], bias[4];
+    {
+        const float *row = map.bias ? map.bias + (size_t)head * a.entries : nullptr;
+        const PlaceAt *first = map.places;  // any window's: corners are the same in all
+        const int cq = first[qt0 * 64 + q].corner + middle(a);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = f32x4{};
-    for (long long window = 0; window < a.windows; ++window) {
-        __syncthreads();
-        if (threadIdx.x < 64)
-            qrow.fill(a, labels, window, q0, threadIdx.x);
-        else if (threadIdx.x < 128)
-            krow.fill(a, labels, window, k0, threadIdx.x - 64);
-        __syncthreads();
-        stage<T, HD>(Ks, base + C, stride, krow, a.hd);
-        stage<T, HD>(Vs, base + 2 * C, stride, krow, a.hd);
-        const int mine = qrow.token[q], ql = qrow.label[q], qr = qrow.wrap[q], qc = qrow.corner[q] + middle(a);
-        const int live = ql < 0 ? -1 : mine;
-        Frag qf[CB], gf[CB];
+        for (int j = 0; j < 4; ++j) {
+            sum[j] = f32x4{};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                bias[j][r] = row ? row[cq - first[kt0 * 64 + j * 16 + 4 * g + r].corner] : 0.f;
+        }
+    }
+    const long long w0 = a.windows * chunk / w.chunks, w1 = a.windows * (chunk + 1) / w.chunks;
+    const long long pairs = (w1 - w0) * nz * ny * nx;
+    // one pair of tiles after the other, their rows a pair ahead
+    struct Pair {
+        long long window;
+        int qt, kt;
+    };
+    auto pair_at = [&](long long k) {
+        const unsigned per = (unsigned)(nz * ny * nx);
+        const unsigned u = (unsigned)(k % per);
+        const unsigned x = u % (unsigned)nx, y = u / (unsigned)nx % (unsigned)ny, z = u / (unsigned)nx / (unsigned)ny;
+        const int step = ((int)z * w.gh + (int)y) * w.gw + (int)x;
+        return Pair{w0 + k / per, qt0 + step, kt0 + step};
+    };
+    R kr, vr;
+    Frag qf[CB], gf[CB], qn[CB], gn[CB];
+    PlaceAt at{}, own{}, own_n{};
+    float shift = 0.f, del = 0.f, shift_n = 0.f, del_n = 0.f;
+    bool mixed = false, mixed_n = false;
+    int token[R::kPieces];
+    auto fetch = [&](const Pair &p) {
+        const PlaceAt *window = map.places + p.window * map.tiles * 64;
+        tokens_of<T, HD>(window + p.kt * 64, token);
+        kr.load(base + C, stride, token, a.hd);
+        vr.load(base + 2 * C, stride, token, a.hd);
+        if (threadIdx.x < 64) at = window[p.kt * 64 + threadIdx.x];
+        own_n = window[p.qt * 64 + q];
+        const int live = own_n.label < 0 ? -1 : own_n.token;
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
-            qf[c] = load4<T>(base, stride, live, c * 16 + 4 * g, a.hd);
-            gf[c] = load4<T>(dout + (size_t)head * a.hd, C, live, c * 16 + 4 * g, a.hd);
+            qn[c] = load4<T>(base, stride, live, c * 16 + 4 * g, a.hd);
+            gn[c] = load4<T>(gbase, C, live, c * 16 + 4 * g, a.hd);
         }
-        const size_t line = ((size_t)window * a.heads + head) * a.n + q0 + q;
-        const float shift = mine >= 0 ? lse[line] : INFINITY, del = mine >= 0 ? delta[line] : 0.f;
+        const size_t line = ((size_t)p.window * a.heads + head) * a.n + p.qt * 64 + q;
+        shift_n = own_n.token >= 0 ? lse[line] : INFINITY;
+        del_n = own_n.token >= 0 ? delta[line] : 0.f;
+    };
+    // the next pair from k on that has anything to add; pairs when there is none
+    auto next = [&](long long k) {
+        for (; k < pairs; ++k) {
+            const Pair p = pair_at(k);
+            const TileAt *row = map.tiles_at + p.window * map.tiles;
+            const TileAt tq = row[p.qt], tk = row[p.kt];
+            const bool both = tq.state == kEven && tk.state == kEven;
+            const bool same = tq.label == tk.label && tq.wrap == tk.wrap;
+            mixed_n = !(both && same);
+            if (tq.state != kDead && tk.state != kDead && !(both && !same && a.outside2 == -INFINITY)) break;
+        }
+        return k;
+    };
+    long long k = next(0);
+    if (k < pairs) fetch(pair_at(k));
+    while (k < pairs) {
+        __syncthreads();
+        kr.store_rows(Ks);
+        vr.store_rows(Vs);
+        if (threadIdx.x < 64) at_s[threadIdx.x] = at;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) qf[c] = qn[c], gf[c] = gn[c];
+        own = own_n, shift = shift_n, del = del_n, mixed = mixed_n;
+        k = next(k + 1);
+        if (k < pairs) fetch(pair_at(k));
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 acc{}, acc2{};
+            const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
+                                   a.outside2);
+            const f32x4 dp = over_channels<T, HD>(Vs, j * 16, gf);
 #pragma unroll
-            for (int c = 0; c < CB; ++c) {
-                const int at = (j * 16 + i) * STRIDE + c * 16 + 4 * g;
-                acc = M::run(row4<T>(&Ks[at]), qf[c], acc);
-                acc2 = M::run(row4<T>(&Vs[at]), gf[c], acc2);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = j * 16 + 4 * g + r;
-                float x = acc[r] * scale2;
-                if (bias) x += bias[qc - krow.corner[key]];
-                x = masked(x, ql, qr, krow.label[key], krow.wrap[key], a.outside2);
-                if (x != -INFINITY) sum[j][r] += exp2f(x - shift) * (acc2[r] - del);
-            }
+            for (int r = 0; r < 4; ++r) sum[j][r] += __builtin_amdgcn_exp2f(x[r] - shift) * (dp[r] - del);
         }
     }
-    if (q0 + q >= a.n) return;
-    float *to = dense + ((size_t)head * a.n + q0 + q) * a.n + k0;
+    if (even) {  // [chunk][distance of tiles][head][64][64]
+        float *to = dense + (((size_t)chunk * (gridDim.x / (unsigned)(w.chunks * a.heads)) + blockIdx.x / (unsigned)(w.chunks * a.heads)) *
+                                 a.heads + head) * 4096 + q * 64;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(f32x4 *)&to[j * 16 + 4 * g] = sum[j];
+        return;
+    }
+    if (qt0 * 64 + q >= a.n) return;
+    float *to = dense + ((size_t)head * a.n + qt0 * 64 + q) * a.n + kt0 * 64;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (k0 + j * 16 + 4 * g + r < a.n) to[j * 16 + 4 * g + r] = sum[j][r];
+            if (kt0 * 64 + j * 16 + 4 * g + r < a.n) to[j * 16 + 4 * g + r] = sum[j][r];
 }
 
 // launchers, one translation unit for each element type
 struct AttnBuffers {
     const void *qkv;
     const float *table;         // as given
-    const float *bias_by_head;  // long windows: the copy
+    LongMap map;                // long windows
+    PairWork work;
     const int *labels;
     const void *out_in;
     void *out;

@@ -33,6 +33,16 @@ void with_nb(int n, F f)
 
 unsigned long_grid(const WindowArgs &a) { return (unsigned)(a.windows * a.heads * ((a.n + 63) / 64)); }
 
+// rows of the window that are multiples of 4: four neighbours' bias entries lie behind each other
+template <class F>
+void with_vec(int ww, F f)
+{
+    if (ww % 4 == 0)
+        f(std::true_type{});
+    else
+        f(std::false_type{});
+}
+
 }  // namespace
 
 template <>
@@ -46,8 +56,10 @@ void launch_attention_fwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
                                    b.table, b.labels, (T *)b.out);
             });
         else
-            hipLaunchKernelGGL((long_fwd<T, HD>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, (const T *)b.qkv,
-                               b.bias_by_head, b.labels, (T *)b.out, b.lse);
+            with_vec(a.ww, [&](auto VEC) {
+                hipLaunchKernelGGL((long_fwd<T, HD, VEC>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, b.map,
+                                   (const T *)b.qkv, (T *)b.out, b.lse);
+            });
     });
 }
 
@@ -63,14 +75,17 @@ void launch_attention_bwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
             });
             return;
         }
-        hipLaunchKernelGGL((long_bwd_q<T, HD>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, (const T *)b.qkv,
-                           b.bias_by_head, b.labels, (const T *)b.out_in, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
-        hipLaunchKernelGGL((long_bwd_kv<T, HD>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, (const T *)b.qkv,
-                           b.bias_by_head, b.labels, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
+        with_vec(a.ww, [&](auto VEC) {
+            hipLaunchKernelGGL((long_bwd_q<T, HD, VEC>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, b.map,
+                               (const T *)b.qkv, (const T *)b.out_in, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
+            hipLaunchKernelGGL((long_bwd_kv<T, HD, VEC>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, b.map,
+                               (const T *)b.qkv, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
+        });
         if (b.dense) {
-            const unsigned tiles = (unsigned)(a.n + 63) / 64;
-            hipLaunchKernelGGL((long_bwd_pairs<T, HD>), dim3(tiles * tiles * a.heads), dim3(kAttnThreads), 0, st, a,
-                               (const T *)b.qkv, b.bias_by_head, b.labels, b.lse, (const T *)b.dout, b.delta, b.dense);
+            const PairWork &w = b.work;
+            const unsigned distances = w.gd ? (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) : b.map.tiles * b.map.tiles;
+            hipLaunchKernelGGL((long_bwd_pairs<T, HD>), dim3(distances * a.heads * w.chunks), dim3(kAttnThreads), 0, st, a, b.map, w,
+                               (const T *)b.qkv, b.lse, (const T *)b.dout, b.delta, b.dense);
         }
     });
 }

@@ -18,63 +18,97 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// VEC parameters of column j * VEC .., as vectors of four where they are aligned (the row's type has VEC of 4 or 8;
+// VEC = 1: single ones); `none` where there are no parameters.
+template <int VEC>
+__device__ __forceinline__ void load_params(float (&to)[VEC], const float *__restrict__ p, int j, bool in, float none)
+{
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) to[e] = none;
+    if (!p || !in) return;
+    if constexpr (VEC % 4 == 0) {
+        if (((size_t)p & 15) == 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const f32x4 v = *(const f32x4 *)(p + j * VEC + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[e + k] = v[k];
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) to[e] = p[j * VEC + e];
+}
+
 // Rows of `cols` elements as NV vectors of VEC elements in each of L lanes; lane i holds the vectors i, i + L, ...
-template <class T, int VEC, int L, int NV>
+// R rows are in flight at once: one row's 16 bytes for a lane, read, summed and written in turn, leave the memory
+// waiting for the sums (rows of 64 fp32: 96 us; ROWS in flight: see the table of measurements below).
+template <class T, int VEC, int L, int NV, int R>
 __global__ __launch_bounds__(kThreads) void norm_fwd(const T *__restrict__ x, const float *__restrict__ w,
                                                      const float *__restrict__ b, T *__restrict__ y,
                                                      float *__restrict__ mean_out, float *__restrict__ rstd_out,
                                                      long long rows, int cols, float eps)
 {
+    constexpr int G = kThreads / L;
     const int lane = threadIdx.x % L;
     const int nvec = cols / VEC;
     const float inv = 1.0f / (float)cols;
     // (whole groups of L lanes leave the loop together: the sums below stay within a group)
-    for (long long row = (long long)blockIdx.x * (kThreads / L) + threadIdx.x / L; row < rows;
-         row += (long long)gridDim.x * (kThreads / L)) {
-    const Vec<T, VEC> *xr = (const Vec<T, VEC> *)(x + row * cols);
-    float xv[NV][VEC];
-    float s = 0.f;
+    for (long long row0 = (long long)blockIdx.x * (G * R) + threadIdx.x / L; row0 < rows;
+         row0 += (long long)gridDim.x * (G * R)) {
+        Vec<T, VEC> t[R][NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = lane + i * L;
-        Vec<T, VEC> t{};
-        if (j < nvec) t = xr[j];
+        for (int k = 0; k < R; ++k) {
+            const long long row = row0 + k * G;
+            const Vec<T, VEC> *xr = (const Vec<T, VEC> *)(x + row * cols);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            xv[i][e] = to_f32(t.v[e]);
-            s += xv[i][e];
-        }
-    }
-    const float mean = group_sum<L>(s) * inv;
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (lane + i * L < nvec)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                xv[i][e] -= mean;
-                q += xv[i][e] * xv[i][e];
+            for (int i = 0; i < NV; ++i) {
+                t[k][i] = Vec<T, VEC>{};
+                if (row < rows && lane + i * L < nvec) t[k][i] = xr[lane + i * L];
             }
-    const float rstd = 1.0f / sqrtf(group_sum<L>(q) * inv + eps);
-    if (lane == 0 && mean_out) {
-        mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
-    Vec<T, VEC> *yr = (Vec<T, VEC> *)(y + row * cols);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = lane + i * L;
-        if (j >= nvec) continue;
-        Vec<T, VEC> t;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float v = xv[i][e] * rstd;
-            if (w) v *= w[j * VEC + e];
-            if (b) v += b[j * VEC + e];
-            t.v[e] = from_f32<T>(v);
         }
-        yr[j] = t;
-    }
+        float wv[NV][VEC], bv[NV][VEC];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            load_params<VEC>(wv[i], w, lane + i * L, lane + i * L < nvec, 1.f);
+            load_params<VEC>(bv[i], b, lane + i * L, lane + i * L < nvec, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const long long row = row0 + k * G;
+            if (row >= rows) break;
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s += to_f32(t[k][i].v[e]);
+            const float mean = group_sum<L>(s) * inv;
+            float q = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (lane + i * L < nvec)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float d = to_f32(t[k][i].v[e]) - mean;
+                        q += d * d;
+                    }
+            const float rstd = 1.0f / sqrtf(group_sum<L>(q) * inv + eps);
+            if (lane == 0 && mean_out) {
+                mean_out[row] = mean;
+                rstd_out[row] = rstd;
+            }
+            Vec<T, VEC> *yr = (Vec<T, VEC> *)(y + row * cols);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (lane + i * L >= nvec) continue;
+                Vec<T, VEC> o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    o.v[e] = from_f32<T>((to_f32(t[k][i].v[e]) - mean) * rstd * wv[i][e] + bv[i][e]);
+                yr[lane + i * L] = o;
+            }
+        }
     }
 }
 
@@ -137,10 +171,10 @@ __global__ __launch_bounds__(kThreads) void norm_bwd(const T *__restrict__ x, co
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const int c = (lane + i * L) * VEC + e;
-            wv[i][e] = c < cols && w ? w[c] : 1.0f;
             dw[i][e] = db[i][e] = 0.f;
         }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_params<VEC>(wv[i], w, lane + i * L, lane + i * L < nvec, 1.f);
     for (long long row = (long long)blockIdx.x * G + group; row < rows; row += (long long)gridDim.x * G) {
         const Vec<T, VEC> *xr = (const Vec<T, VEC> *)(x + row * cols);
         const Vec<T, VEC> *gr = (const Vec<T, VEC> *)(dy + row * cols);
@@ -247,21 +281,25 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_wide(const T *__restrict__ 
     }
 }
 
-// dw and db from the workgroups' shares: 16 columns for a workgroup, 16 threads on each, joined in order.
-__global__ __launch_bounds__(kThreads) void norm_fold(const float *__restrict__ partial, float *__restrict__ dw,
-                                                      float *__restrict__ db, int parts, int cols)
+// dw and db from the workgroups' shares: 16 columns for a workgroup, 64 threads on each, joined in order.  (16 threads
+// on each: 17 us for 1024 shares of 2 x 64 columns, all of it waiting for 64 loads in a row.)
+constexpr int kFold = 1024;
+__global__ __launch_bounds__(kFold) void norm_fold(const float *__restrict__ partial, float *__restrict__ dw,
+                                                   float *__restrict__ db, int parts, int cols)
 {
-    __shared__ float fold[16][17];
+    __shared__ float fold[kFold / 16][17];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const long long c = (long long)blockIdx.x * 16 + tx;  // of 2 * cols
     float s = 0.f;
-    if (c < 2LL * cols)
-        for (int p = ty; p < parts; p += 16) s += partial[(size_t)p * 2 * cols + c];
+    if (c < 2LL * cols) {
+#pragma unroll 8
+        for (int p = ty; p < parts; p += kFold / 16) s += partial[(size_t)p * 2 * cols + c];
+    }
     fold[ty][tx] = s;
     __syncthreads();
-    if (ty == 0 && c < 2LL * cols) {
+    if (threadIdx.x < 16 && c < 2LL * cols) {
         float t = 0.f;
-        for (int k = 0; k < 16; ++k) t += fold[k][tx];
+        for (int k = 0; k < kFold / 16; ++k) t += fold[k][tx];
         if (c < cols) {
             if (dw) dw[c] = t;
         } else if (db) {
@@ -340,7 +378,9 @@ int run_fwd(const void *x, const float *w, const float *b, void *y, float *mean,
 {
     const Shape s = shape_for(cols, dtype, aligned16(x) && aligned16(y));
     if (!with_shape<T>(s, [&](auto V, auto L, auto N) {
-            hipLaunchKernelGGL((norm_fwd<T, V, L, N>), dim3(fwd_blocks(rows, kThreads / L)), dim3(kThreads), 0, st, (const T *)x, w, b,
+            // rows in flight: as many as 64 bytes for a lane make
+            constexpr int R = N == 1 ? 4 : N == 2 ? 2 : 1;
+            hipLaunchKernelGGL((norm_fwd<T, V, L, N, R>), dim3(fwd_blocks(rows, kThreads / L * R)), dim3(kThreads), 0, st, (const T *)x, w, b,
                                (T *)y, mean, rstd, rows, cols, eps);
         }))
         hipLaunchKernelGGL((norm_fwd_wide<T>), dim3(fwd_blocks(rows, 1)), dim3(kThreads), 0, st, (const T *)x, w, b,
@@ -361,7 +401,7 @@ int run_bwd(const void *x, const void *dy, const float *w, const float *mean, co
         hipLaunchKernelGGL((norm_bwd_wide<T>), dim3(parts), dim3(kThreads), 0, st, (const T *)x, (const T *)dy, w,
                            mean, rstd, (T *)dx, partial, rows, cols);
     if (partial)
-        hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2LL * cols + 15) / 16)), dim3(kThreads), 0, st, partial,
+        hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2LL * cols + 15) / 16)), dim3(kFold), 0, st, partial,
                            dw, db, parts, cols);
     return check_launch("artemis_ops_layer_norm_backward");
 }
@@ -426,7 +466,7 @@ int artemis_ops_layer_norm_backward(const void *x, const void *dy, const float *
     const bool sums = dweight || dbias;
     if (rows == 0) {  // sums over nothing
         if (sums)
-            hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2 * cols + 15) / 16)), dim3(kThreads), 0, st,
+            hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2 * cols + 15) / 16)), dim3(kFold), 0, st,
                                (const float *)nullptr, dweight, dbias, 0, (int)cols);
         return check_launch(what);
     }
