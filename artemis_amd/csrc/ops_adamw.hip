@@ -4,8 +4,8 @@
 //   p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Elementwise, so bound by memory: 28 bytes for an fp32 parameter with 32-bit moments, 16 with 8-bit ones.  A
-// launch takes the addresses of up to kTensors tensors as its arguments (no copy of a table, nothing kept
-// between calls); a workgroup finds its tensor and its share of 4096 elements by a search in the shares' prefix sums.
+// launch takes the addresses of up to 90 tensors (8 bit: 59) as its arguments (no copy of a table, nothing kept
+// between calls); a workgroup finds its tensor and its share of 1024 elements by a search in the shares' prefix sums.
 //
 // 8-bit moments.  A positive fp32 number's bit pattern orders as the number does; its top 11 bits are 8 of
 // exponent and 3 of mantissa.  256 elements share a base, and a code counts those 11 bits up from it: v, which
@@ -21,22 +21,38 @@ namespace aops {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kShare = 4096;  // elements a workgroup takes
+// Elements a workgroup takes: four a thread.  Short-lived workgroups keep loads and stores of different ones in flight
+// together: 29.1 M fp32 parameters with 32-bit moments take 163 us (5.0 TB/s) at 1024, 174 at 2048, 190 at 4096; with
+// 8-bit ones 120, 140 and 174 us.
+constexpr int kShare = 1024;
 constexpr int kGroup = 256;   // elements that share a base
-constexpr int kTensors = 62;  // 62 * 64 bytes: within the 4 KB of a launch's arguments
 
-struct Tensor {
+// A launch's tensors, as many as its 4 KB of arguments hold
+struct Tensor32 {
+    static constexpr int kMost = 90;
+    void *p;
+    const void *g;
+    void *m, *v;
+    long long count;
+    Tensor32() = default;
+    Tensor32(const artemis_ops_tensor &t, unsigned) : p(t.param), g(t.grad), m(t.m), v(t.v), count(t.count) {}
+};
+struct Tensor8 {
+    static constexpr int kMost = 59;
     void *p;
     const void *g;
     void *m, *v;
     int *mb, *vb;
     long long count;
+    unsigned place;  // among all tensors, in groups of kGroup
+    Tensor8() = default;
+    Tensor8(const artemis_ops_tensor &t, unsigned at)
+        : p(t.param), g(t.grad), m(t.m), v(t.v), mb(t.m_base), vb(t.v_base), count(t.count), place(at) {}
 };
-
+template <class Tensor>
 struct Batch {
-    Tensor t[kTensors];
-    int first[kTensors];       // the first workgroup of each tensor
-    unsigned place[kTensors];  // its place among all tensors, in groups of kGroup
+    Tensor t[Tensor::kMost];
+    int first[Tensor::kMost];  // the first workgroup of each tensor
     int n;
 };
 
@@ -61,7 +77,8 @@ __device__ __forceinline__ void update(float &p, float g, float &m, float &v, co
     p = p - (m * c.step) / (sqrtf(v) * c.unbias + c.eps);
 }
 
-__device__ __forceinline__ int find(const Batch &b)
+template <class Tensor>
+__device__ __forceinline__ int find(const Batch<Tensor> &b)
 {
     int lo = 0, hi = b.n - 1;  // the last tensor whose first workgroup is not behind this one
     while (lo < hi) {
@@ -75,10 +92,10 @@ __device__ __forceinline__ int find(const Batch &b)
 }
 
 template <class T>
-__global__ __launch_bounds__(kThreads) void adamw32(const Batch b, const Coef c)
+__global__ __launch_bounds__(kThreads) void adamw32(const Batch<Tensor32> b, const Coef c)
 {
     const int which = find(b);
-    const Tensor t = b.t[which];
+    const Tensor32 t = b.t[which];
     const long long at = (long long)(blockIdx.x - b.first[which]) * kShare;
     T *p = (T *)t.p + at;
     const T *g = (const T *)t.g + at;
@@ -196,14 +213,14 @@ struct Held {
 
 // A wave takes groups of 256 elements, four neighbours in each lane; all groups' loads are in front of the first store.
 template <class T>
-__global__ __launch_bounds__(kThreads) void adamw8(const Batch b, const Coef c)
+__global__ __launch_bounds__(kThreads) void adamw8(const Batch<Tensor8> b, const Coef c)
 {
     constexpr int K = kShare / kGroup / (kThreads / 64);
     const int which = find(b);
-    const Tensor t = b.t[which];
+    const Tensor8 t = b.t[which];
     const long long at = (long long)(blockIdx.x - b.first[which]) * kShare;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const unsigned place = b.place[which];
+    const unsigned place = t.place;
     const bool aligned = ((size_t)t.p % (4 * sizeof(T)) | (size_t)t.g % (4 * sizeof(T)) |
                           ((size_t)t.m & 3) | ((size_t)t.v & 3)) == 0;
     Held<T> held[K];
@@ -278,10 +295,10 @@ __global__ __launch_bounds__(kThreads) void adamw8(const Batch b, const Coef c)
 }
 
 template <bool SIGNED>
-__global__ __launch_bounds__(kThreads) void moments_from_8bit(const Batch b)
+__global__ __launch_bounds__(kThreads) void moments_from_8bit(const Batch<Tensor8> b)
 {
     const int which = find(b);
-    const Tensor t = b.t[which];
+    const Tensor8 t = b.t[which];
     const long long at = (long long)(blockIdx.x - b.first[which]) * kShare;
     float *out = (float *)t.p;
     const unsigned char *codes = (const unsigned char *)t.m;
@@ -304,16 +321,17 @@ __global__ __launch_bounds__(kThreads) void moments_from_8bit(const Batch b)
     }
 }
 
-// Calls launch(batch, workgroups) for every batch of tensors: as many as fit the arguments and 2^22 workgroups
+// Calls launch(batch, workgroups) for every batch of tensors: as many as fit the arguments and 2^23 workgroups
 // (check_tensors holds each of them to that; a launch has at most 2^32 threads).
-template <class F>
+template <class Tensor, class F>
 int in_batches(const artemis_ops_tensor *tensors, int n, const char *what, F launch)
 {
-    Batch b;
+    static_assert(sizeof(Batch<Tensor>) + sizeof(Coef) <= 4096, "a launch's arguments");
+    Batch<Tensor> b;
     b.n = 0;
     long long blocks = 0;
     unsigned place = 0;
-    constexpr long long kMost = 1 << 22;
+    constexpr long long kMost = 1 << 23;
     auto flush = [&]() -> int {
         if (b.n == 0) return 0;
         launch(b, (unsigned)blocks);
@@ -322,18 +340,16 @@ int in_batches(const artemis_ops_tensor *tensors, int n, const char *what, F lau
         return check_launch(what);
     };
     for (int i = 0; i < n; ++i) {
-        Tensor t{tensors[i].param, tensors[i].grad, tensors[i].m, tensors[i].v, tensors[i].m_base,
-                 tensors[i].v_base, tensors[i].count};
-        if (t.count == 0) continue;
-        const long long need = (t.count + kShare - 1) / kShare;
-        if (b.n == kTensors || blocks + need > kMost)
+        const long long count = tensors[i].count;
+        if (count == 0) continue;
+        const long long need = (count + kShare - 1) / kShare;
+        if (b.n == Tensor::kMost || blocks + need > kMost)
             if (int rc = flush()) return rc;
-        b.place[b.n] = place;
-        b.t[b.n] = t;
+        b.t[b.n] = Tensor(tensors[i], place);
         b.first[b.n] = (int)blocks;
         ++b.n;
         blocks += need;
-        place += (unsigned)((t.count + kGroup - 1) / kGroup);
+        place += (unsigned)((count + kGroup - 1) / kGroup);
     }
     return flush();
 }
@@ -345,8 +361,8 @@ int check_tensors(const artemis_ops_tensor *tensors, int n, bool grads, bool bas
     long long groups = 0;
     for (int i = 0; i < n; ++i) {
         const artemis_ops_tensor &t = tensors[i];
-        if (t.count < 0 || t.count > ((1LL << 22) * kShare))
-            return fail(hipErrorInvalidValue, "%s: tensor %d has %lld elements (0 .. 2^34)", what, i, t.count);
+        if (t.count < 0 || t.count > ((1LL << 23) * kShare))
+            return fail(hipErrorInvalidValue, "%s: tensor %d has %lld elements (0 .. 2^33)", what, i, t.count);
         groups += (t.count + kGroup - 1) / kGroup;
         if (t.count == 0) continue;
         if (!t.param || !t.m || (grads && (!t.grad || !t.v)) || (bases && (!t.m_base || (grads && !t.v_base))))
@@ -390,23 +406,24 @@ int artemis_ops_adamw(const artemis_ops_tensor *tensors, int n_tensors, int dtyp
     c.eps = (float)eps;
     c.key = seed * 0x9E3779B1u + (unsigned)step * 0x6A09E667u;
     hipStream_t st = (hipStream_t)stream;
-    return in_batches(tensors, n_tensors, what, [&](const Batch &b, unsigned blocks) {
-        const dim3 grid(blocks), block(kThreads);
-        if (bits == 32) {
+    if (bits == 32)
+        return in_batches<Tensor32>(tensors, n_tensors, what, [&](const Batch<Tensor32> &b, unsigned blocks) {
+            const dim3 grid(blocks), block(kThreads);
             if (dtype == ARTEMIS_OPS_F32)
                 hipLaunchKernelGGL((adamw32<float>), grid, block, 0, st, b, c);
             else if (dtype == ARTEMIS_OPS_BF16)
                 hipLaunchKernelGGL((adamw32<__bf16>), grid, block, 0, st, b, c);
             else
                 hipLaunchKernelGGL((adamw32<_Float16>), grid, block, 0, st, b, c);
-        } else {
-            if (dtype == ARTEMIS_OPS_F32)
-                hipLaunchKernelGGL((adamw8<float>), grid, block, 0, st, b, c);
-            else if (dtype == ARTEMIS_OPS_BF16)
-                hipLaunchKernelGGL((adamw8<__bf16>), grid, block, 0, st, b, c);
-            else
-                hipLaunchKernelGGL((adamw8<_Float16>), grid, block, 0, st, b, c);
-        }
+        });
+    return in_batches<Tensor8>(tensors, n_tensors, what, [&](const Batch<Tensor8> &b, unsigned blocks) {
+        const dim3 grid(blocks), block(kThreads);
+        if (dtype == ARTEMIS_OPS_F32)
+            hipLaunchKernelGGL((adamw8<float>), grid, block, 0, st, b, c);
+        else if (dtype == ARTEMIS_OPS_BF16)
+            hipLaunchKernelGGL((adamw8<__bf16>), grid, block, 0, st, b, c);
+        else
+            hipLaunchKernelGGL((adamw8<_Float16>), grid, block, 0, st, b, c);
     });
 }
 
@@ -415,7 +432,7 @@ int artemis_ops_moments_from_8bit(const artemis_ops_tensor *tensors, int n_tenso
     const char *what = "artemis_ops_moments_from_8bit";
     if (int rc = check_tensors(tensors, n_tensors, false, true, what)) return rc;
     hipStream_t st = (hipStream_t)stream;
-    return in_batches(tensors, n_tensors, what, [&](const Batch &b, unsigned blocks) {
+    return in_batches<Tensor8>(tensors, n_tensors, what, [&](const Batch<Tensor8> &b, unsigned blocks) {
         if (is_signed)
             hipLaunchKernelGGL((moments_from_8bit<true>), dim3(blocks), dim3(kThreads), 0, st, b);
         else

@@ -108,7 +108,7 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w /* HOST */
  *             generator: (seed, step, the element's place), where the tensors follow each other at
  *             multiples of 256 elements.  A gradient that is not finite spoils the 256 elements of its
  *             group.
- * step >= 1.  bits = 8 holds at most 2^32 places, counted in groups of 256. */
+ * step >= 1; a tensor has at most 2^33 elements.  bits = 8 holds at most 2^32 places, counted in groups of 256. */
 typedef struct artemis_ops_tensor {
     void *param;
     const void *grad;
