@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void places_of(const WindowArgs a, const int *
     const int lane = threadIdx.x % 64, t = (int)(tile % tiles) * 64 + lane;
     PlaceAt p{-1, 0, -1, 0};
     if (t < a.n) {
-        const Place at = place_of(a, labels, tile / tiles, t);
+        const Place at = place_of(a, labels, tile / tiles, t / a.ww / a.wh, t / a.ww % a.wh, t % a.ww);
         p = PlaceAt{at.token, corner(a, t), at.label, at.wrap};
     }
     places[tile * 64 + lane] = p;
@@ -197,8 +197,9 @@ int make_args(const char *what, const artemis_ops_window *w, WindowArgs &a)
         return fail(hipErrorInvalidValue, "%s: too many tokens or windows * heads", what);
     a = WindowArgs{w->B, w->D, w->H, w->W, w->heads, w->head_dim, w->wd, w->wh, w->ww, n, w->shift_d, w->shift_h,
                    w->shift_w, w->D / w->wd, w->H / w->wh, w->W / w->ww, w->label_maps, (2 * w->wh - 1) * (2 * w->ww - 1),
-                   2 * w->ww - 1, (2 * w->wd - 1) * (2 * w->wh - 1) * (2 * w->ww - 1), 0, w->scale, 0.f};
+                   2 * w->ww - 1, (2 * w->wd - 1) * (2 * w->wh - 1) * (2 * w->ww - 1), 0, Divider(), Divider(), Divider(), w->scale, 0.f};
     a.windows = (long long)w->B * a.nd * a.nh * a.nw;
+    if (a.windows) a.by_nd = Divider(a.nd), a.by_nh = Divider(a.nh), a.by_nw = Divider(a.nw);
     // a finite `outside` stays finite in the exponent of 2; beyond -1e30 nothing else counts beside it anyway
     a.outside2 = w->outside == -INFINITY ? -INFINITY : (w->outside < -1e30f ? -1e30f : w->outside) * kLog2e;
     return a.windows == 0 ? -1 : 0;

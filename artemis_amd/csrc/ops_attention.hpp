@@ -15,6 +15,19 @@ namespace aops {
 constexpr int kAttnThreads = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Division of numbers below 2^31 by a constant d: q = (mulhi(x, m) + x) >> s with m = floor(2^32 (2^s - d) / d) + 1,
+// s = ceil(log2 d) -- the reciprocal rounded up to 33 bits, whose top one is the added x.
+struct Divider {
+    unsigned m = 1, s = 0;
+    Divider() = default;
+    explicit Divider(unsigned d)
+    {
+        while ((1ull << s) < d) ++s;
+        m = (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+    }
+    __device__ __forceinline__ unsigned of(unsigned x) const { return (__umulhi(x, m) + x) >> s; }
+};
+
 struct WindowArgs {
     int B, D, H, W;
     int heads, hd;           // head_dim
@@ -25,6 +38,7 @@ struct WindowArgs {
     int rd, rh;              // radices of the bias index: (2wh-1)(2ww-1), 2ww-1
     int entries;             // of the bias table
     long long windows;       // B * nd * nh * nw
+    Divider by_nd, by_nh, by_nw;
     float scale, outside2;   // outside * log2(e); -inf: never
 };
 
@@ -83,38 +97,30 @@ struct Mma<_Float16> {
     }
 };
 
-// a column of four rows of a row-major LDS tile: the A operand (row = channel, contraction over tokens)
-template <class T, int STRIDE>
-__device__ __forceinline__ typename Mma<T>::Frag column(const T *tile, int token, int channel)
-{
-    typename Mma<T>::Frag f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] = tile[(token + r) * STRIDE + channel];
-    return f;
-}
+// four neighbours of an LDS tile as an operand
 template <class T>
 __device__ __forceinline__ typename Mma<T>::Frag row4(const T *p)
 {
     return *(const typename Mma<T>::Frag *)p;
 }
 
-// Where a token of a window lies, and its region.  `live`: it exists and is not padding.
+// Where a token of a window lies, and its region.
 struct Place {
     int token;   // on the (B, D, H, W) map, -1: none
-    int label;
+    int label;   // < 0: padding
     int wrap;    // which axes the shift wrapped around, one bit each
 };
 
-__device__ __forceinline__ Place place_of(const WindowArgs &a, const int *__restrict__ labels, long long window, int t)
+// `td`, `th`, `tw`: the token's coordinates in the window
+__device__ __forceinline__ Place place_of(const WindowArgs &a, const int *__restrict__ labels, long long window, int td, int th,
+                                          int tw)
 {
     Place r{-1, -1, 0};
     if (window >= a.windows) return r;
     const unsigned w = (unsigned)window;
-    const unsigned kw = w % (unsigned)a.nw, w1 = w / (unsigned)a.nw;
-    const unsigned kh = w1 % (unsigned)a.nh, w2 = w1 / (unsigned)a.nh;
-    const unsigned kd = w2 % (unsigned)a.nd, b = w2 / (unsigned)a.nd;
-    const unsigned tw = (unsigned)t % (unsigned)a.ww, t1 = (unsigned)t / (unsigned)a.ww;
-    const unsigned th = t1 % (unsigned)a.wh, td = t1 / (unsigned)a.wh;
+    const unsigned w1 = a.by_nw.of(w), kw = w - w1 * a.nw;
+    const unsigned w2 = a.by_nh.of(w1), kh = w1 - w2 * a.nh;
+    const unsigned b = a.by_nd.of(w2), kd = w2 - b * a.nd;
     int d = (int)(kd * a.wd + td) + a.sd, h = (int)(kh * a.wh + th) + a.sh, x = (int)(kw * a.ww + tw) + a.sw;
     if (d >= a.D) d -= a.D, r.wrap |= 1;
     if (h >= a.H) h -= a.H, r.wrap |= 2;
@@ -151,6 +157,83 @@ __device__ __forceinline__ typename Mma<T>::Frag load4(const T *__restrict__ bas
     typename Mma<T>::Frag f{};
     if (token >= 0 && c < hd) f = *(const typename Mma<T>::Frag *)(base + (long long)token * stride + c);
     return f;
+}
+
+// 64 rows on their way to LDS: HD / 16 pieces of four channels in each thread
+template <class T, int HD>
+struct Rows {
+    using Frag = typename Mma<T>::Frag;
+    static constexpr int kPieces = HD / 16, kRowStep = kAttnThreads / (HD / 4);
+    Frag f[kPieces];
+    static __device__ __forceinline__ int row(int m) { return threadIdx.x / (HD / 4) + m * kRowStep; }
+    static __device__ __forceinline__ int channel() { return threadIdx.x % (HD / 4) * 4; }
+    __device__ __forceinline__ void load(const T *__restrict__ base, long long stride, const int (&token)[kPieces], int hd)
+    {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) f[m] = load4<T>(base, stride, token[m], channel(), hd);
+    }
+    __device__ __forceinline__ void store_rows(T *tile) const  // [64][HD + 4]
+    {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) *(Frag *)&tile[row(m) * (HD + 4) + channel()] = f[m];
+    }
+    __device__ __forceinline__ void store_columns(T *tile) const  // [HD][64 + 4]
+    {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tile[(channel() + e) * 68 + row(m)] = f[m][e];
+    }
+};
+
+// D[token 4g ..][column i] for a block of 16 rows of a row-major tile against a lane's operand: contraction over channels
+template <class T, int HD>
+__device__ __forceinline__ f32x4 over_channels(const T *rows, int first, const typename Mma<T>::Frag *own)
+{
+    using M = Mma<T>;
+    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+    const T *p = rows + (first + i) * (HD + 4) + 4 * g;
+    f32x4 acc{};
+    if constexpr (HD >= 32) {
+#pragma unroll
+        for (int c = 0; c < HD / 16; c += 2) acc = M::run2(row4<T>(p + c * 16), row4<T>(p + c * 16 + 16), own[c], own[c + 1], acc);
+    } else {
+        acc = M::run(row4<T>(p), own[0], acc);
+    }
+    return acc;
+}
+
+// The A operand of a contraction over tokens (row: channel c * 16 + i; tokens at + 4g ..): one read of a tile stored by
+// columns, four of one stored by rows
+template <class T, int HD, bool BY_ROWS>
+__device__ __forceinline__ typename Mma<T>::Frag column(const T *tile, int c, int at)
+{
+    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+    if constexpr (BY_ROWS) {
+        typename Mma<T>::Frag f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = tile[(at + 4 * g + r) * (HD + 4) + c * 16 + i];
+        return f;
+    }
+    return row4<T>(tile + (c * 16 + i) * 68 + at + 4 * g);
+}
+
+// acc[c] += tile^T (channels c * 16 .., tokens first ..) times N blocks of B operands: contraction over 16 N tokens
+template <class T, int HD, int N, bool BY_ROWS = false>
+__device__ __forceinline__ void over_tokens(f32x4 (&acc)[HD / 16], const T *tile, int first,
+                                            const typename Mma<T>::Frag (&b)[N])
+{
+    using M = Mma<T>;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) {
+        if constexpr (N == 1)
+            acc[c] = M::run(column<T, HD, BY_ROWS>(tile, c, first), b[0], acc[c]);
+        else
+#pragma unroll
+            for (int j = 0; j < N; j += 2)
+                acc[c] = M::run2(column<T, HD, BY_ROWS>(tile, c, first + j * 16),
+                                 column<T, HD, BY_ROWS>(tile, c, first + j * 16 + 16), b[j], b[j + 1], acc[c]);
+    }
 }
 
 // ================================================================================================
@@ -214,6 +297,87 @@ __device__ __forceinline__ float masked(float x, int ql, int qr, int kl, int kr,
     return outside2 == -INFINITY ? -INFINITY : x + outside2;
 }
 
+// What the 64 slots of a tile hold.  `mixed`: some are of different regions, or padding.
+struct Spots {
+    int token[64], label[64], wrap[64], mixed;
+};
+
+// The slot of this thread (the first wave's), and the spots of one tile after the other
+template <int NB>
+struct Spotter {
+    int window, t, td, th, tw;
+    __device__ __forceinline__ explicit Spotter(const WindowArgs &a)
+    {
+        Slots<NB>::of(a, threadIdx.x % 64, window, t);
+        const int u = t < 0 ? 0 : t, u1 = u / a.ww;
+        tw = u % a.ww, th = u1 % a.wh, td = u1 / a.wh;
+    }
+    __device__ __forceinline__ Place look(const WindowArgs &a, const int *labels, long long first) const
+    {
+        return t < 0 ? Place{-1, -1, 0} : place_of(a, labels, first + window, td, th, tw);
+    }
+    // (only pairs within a window meet, but one comparison serves all windows of the tile)
+    __device__ __forceinline__ void write(Spots &to, const Place &p) const
+    {
+        const int s = threadIdx.x;
+        to.token[s] = p.token;
+        to.label[s] = p.label;
+        to.wrap[s] = p.wrap;
+        const int label = __shfl(p.label, 0), wrap = __shfl(p.wrap, 0);
+        const bool mixed = !__all(t < 0 || p.token < 0 || (p.label >= 0 && p.label == label && p.wrap == wrap));
+        if (s == 0) to.mixed = mixed;
+    }
+};
+
+template <class T, int HD>
+__device__ __forceinline__ void tokens_at(const Spots &at, int (&token)[Rows<T, HD>::kPieces])
+{
+#pragma unroll
+    for (int m = 0; m < Rows<T, HD>::kPieces; ++m) {
+        const int s = Rows<T, HD>::row(m);
+        token[m] = at.label[s] < 0 ? -1 : at.token[s];
+    }
+}
+
+// Windows that share a block of 16 slots meet in its products, where an operand 0 does not undo an infinity or a NaN of
+// another window's tokens.  Where a tile holds any (kept in a flag beside it), the products over tokens are made
+// window by window instead, with the other windows' tokens taken for 0, and each lane keeps its own window's.
+template <class T, int HD, int NB, bool BY_ROWS = false>
+__device__ __forceinline__ void over_unit(f32x4 (&acc)[HD / 16], const T *tile, int first,
+                                          const typename Mma<T>::Frag (&b)[NB], bool odd, int n)
+{
+    if constexpr (NB == 1) {
+        if (odd) {
+            using M = Mma<T>;
+            const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+            for (int w = 0; w < 16 / n; ++w)
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    typename M::Frag f = column<T, HD, BY_ROWS>(tile, c, first), e = b[0];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if ((4 * g + r) / n != w) f[r] = (T)0.f, e[r] = (T)0.f;
+                    const f32x4 o = M::run(f, e, f32x4{});
+                    if (i / n == w) acc[c] += o;
+                }
+            return;
+        }
+    }
+    over_tokens<T, HD, NB, BY_ROWS>(acc, tile, first, b);
+}
+
+// whether a thread's pieces hold an infinity or a NaN
+template <class T, int HD>
+__device__ __forceinline__ bool not_finite(const Rows<T, HD> &r)
+{
+    float x = 0.f;
+#pragma unroll
+    for (int m = 0; m < Rows<T, HD>::kPieces; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x += (float)r.f[m][e] * 0.f;
+    return x != 0.f;  // 0, or NaN
+}
+
 template <class T, int HD, int NB>
 __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, const T *__restrict__ qkv,
                                                            const float *__restrict__ table,
@@ -221,11 +385,12 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int STRIDE = HD + 4;  // rows 4 elements apart from a power of two: 16 rows on different banks
+    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
-    __shared__ __align__(16) T Ks[64 * STRIDE];
-    __shared__ __align__(16) T Vs[64 * STRIDE];
-    __shared__ int token_s[64], label_s[64], wrap_s[64];
+    __shared__ __align__(16) T Ks[64 * (HD + 4)];
+    __shared__ __align__(16) T Vt[HD * 68];
+    __shared__ Spots spots[3];
+    __shared__ int odd_s[3];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16;
     const Walk walk = walk_of(a.heads);
@@ -234,52 +399,70 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
     const T *base = qkv + (size_t)walk.head * a.hd;
     const int per = Slots<NB>::per_tile(a.n);
     const long long tiles = (a.windows + per - 1) / per;
-    const bool mask = labels || a.sd || a.sh || a.sw;
+    if (walk.tile >= tiles) return;
     const int kb0 = wave / NB * NB;  // the first key block of this wave's unit
     const int q = wave * 16 + i;
     f32x4 bias[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) bias[j] = pair_bias<NB>(a, table, walk.head, q, (kb0 + j) * 16 + 4 * g);
     const float scale2 = a.scale * kLog2e;
-
+    const Spotter<NB> spotter(a);
+    const bool first_wave = threadIdx.x < 64;
+    if (first_wave) {
+        spotter.write(spots[0], spotter.look(a, labels, walk.tile * per));
+        spotter.write(spots[1], spotter.look(a, labels, (walk.tile + walk.step) * per));
+    }
+    if (threadIdx.x < 3) odd_s[threadIdx.x] = 0;
+    __syncthreads();
+    R kr, vr;
+    Frag qn[CB];
+    auto fetch = [&](const Spots &at) {
+        int token[R::kPieces];
+        tokens_at<T, HD>(at, token);
+        kr.load(base + C, stride, token, a.hd);
+        vr.load(base + 2 * C, stride, token, a.hd);
+        const int t = at.label[q] < 0 ? -1 : at.token[q];
+#pragma unroll
+        for (int c = 0; c < CB; ++c) qn[c] = load4<T>(base, stride, t, c * 16 + 4 * g, a.hd);
+    };
+    fetch(spots[0]);
+    int now = 0;  // of three spots: this tile's, the next one's, and the one being looked up
     for (long long tile = walk.tile; tile < tiles; tile += walk.step) {
+        const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
         __syncthreads();  // the tile before has been used
-        if (threadIdx.x < 64) {
-            int w, t;
-            Slots<NB>::of(a, threadIdx.x, w, t);
-            Place p{-1, -1, 0};
-            if (t >= 0) p = place_of(a, labels, tile * per + w, t);
-            token_s[threadIdx.x] = p.token;
-            label_s[threadIdx.x] = p.label;
-            wrap_s[threadIdx.x] = p.wrap;
+        kr.store_rows(Ks);
+        vr.store_columns(Vt);
+        if constexpr (NB == 1) {
+            if (not_finite(vr)) odd_s[now] = 1;
         }
-        __syncthreads();
-        for (int k = threadIdx.x; k < 64 * (HD / 4); k += kAttnThreads) {
-            const int s = k / (HD / 4), c = k % (HD / 4) * 4;
-            const int t = label_s[s] < 0 ? -1 : token_s[s];
-            *(Frag *)&Ks[s * STRIDE + c] = load4<T>(base + C, stride, t, c, a.hd);
-            *(Frag *)&Vs[s * STRIDE + c] = load4<T>(base + 2 * C, stride, t, c, a.hd);
-        }
-        const int mine = token_s[q], ql = label_s[q], qr = wrap_s[q];
         Frag qf[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) qf[c] = load4<T>(base, stride, ql < 0 ? -1 : mine, c * 16 + 4 * g, a.hd);
+        for (int c = 0; c < CB; ++c) qf[c] = qn[c];
         __syncthreads();
+        const Spots &at = spots[now];
+        const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
+        const bool mixed = at.mixed;
+        if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
+        if (tile + walk.step < tiles) fetch(spots[next]);
+        Place coming;
+        if (first_wave) coming = spotter.look(a, labels, (tile + 2 * walk.step) * per);
         f32x4 s[NB];
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            f32x4 acc{};
-#pragma unroll
-            for (int c = 0; c < CB; ++c) acc = M::run(row4<T>(&Ks[((kb0 + j) * 16 + i) * STRIDE + c * 16 + 4 * g]), qf[c], acc);
-            const int key = (kb0 + j) * 16 + 4 * g;
+            const f32x4 acc = over_channels<T, HD>(Ks, (kb0 + j) * 16, qf);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = bias[j][r] == -INFINITY ? -INFINITY : acc[r] * scale2 + bias[j][r];
-                if (mask) x = masked(x, ql, qr, label_s[key + r], wrap_s[key + r], a.outside2);
-                s[j][r] = x;
-                top = fmaxf(top, x);
+                s[j][r] = acc[r] * scale2 + bias[j][r];
+                if (NB == 1 && bias[j][r] == -INFINITY) s[j][r] = -INFINITY;  // (of another window: whatever it is)
             }
+            if (mixed) {
+                const int key = (kb0 + j) * 16 + 4 * g;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[j][r]);
         }
         top = fold_max(top);
         if (top == -INFINITY) top = 0.f;
@@ -288,7 +471,7 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
         for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[j][r] = exp2f(s[j][r] - top);
+                s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - top);
                 sum += s[j][r];
             }
         sum = fold_sum(sum);
@@ -296,15 +479,16 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
         Frag p[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) p[j] = M::frag(s[j] * inv);  // 16 bit: rounded once, as the product takes it
+        f32x4 o[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-            f32x4 o{};
+        for (int c = 0; c < CB; ++c) o[c] = f32x4{};
+        over_unit<T, HD, NB>(o, Vt, kb0 * 16, p, NB == 1 && odd_s[now], a.n);
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
-                o = M::run(column<T, STRIDE>(Vs, (kb0 + j) * 16 + 4 * g, c * 16 + i), p[j], o);
+        for (int c = 0; c < CB; ++c)
             if (mine >= 0 && c * 16 + 4 * g < a.hd)
-                *(Frag *)(out + (size_t)mine * C + walk.head * a.hd + c * 16 + 4 * g) = M::frag(o);
-        }
+                *(Frag *)(out + (size_t)mine * C + walk.head * a.hd + c * 16 + 4 * g) = M::frag(o[c]);
+        if (first_wave) spotter.write(spots[after], coming);
+        now = next;
     }
 }
 
@@ -321,26 +505,29 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    constexpr int STRIDE = HD + 4;
+    using R = Rows<T, HD>;
     constexpr int PS = 16 * NB + 4;
     constexpr int CB = HD / 16;
-    constexpr int TILE = 64 * STRIDE, PAIRS = 2 * 64 * PS;
-    __shared__ __align__(16) T Qs[TILE];
-    __shared__ __align__(16) T Ks[TILE];
-    __shared__ __align__(16) T Gs[TILE];
-    __shared__ __align__(16) T Vs[TILE > PAIRS ? TILE : PAIRS];  // V, then P and dS
+    constexpr int ROWS = 64 * (HD + 4), COLUMNS = HD * 68, PAIRS = 2 * 64 * PS;
+    // K by rows and (128 fp32 channels: no room) by columns, Q and dO by columns; V by rows, then P and dS by keys
+    constexpr bool K_BY_ROWS = HD * sizeof(T) > 256;
+    __shared__ __align__(16) T Ks[ROWS];
+    __shared__ __align__(16) T Kt[K_BY_ROWS ? 1 : COLUMNS];
+    __shared__ __align__(16) T Qt[COLUMNS];
+    __shared__ __align__(16) T Gt[COLUMNS];
+    __shared__ __align__(16) T Vs[ROWS > PAIRS ? ROWS : PAIRS];
     T *const Ps = Vs, *const Ss = Vs + 64 * PS;
-    __shared__ int token_s[64], label_s[64], wrap_s[64];
+    __shared__ Spots spots[3];
+    __shared__ int odd_s[3];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16;
     const Walk walk = walk_of(a.heads);
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
-    const T *base = qkv + (size_t)walk.head * a.hd;
+    const T *base = qkv + (size_t)walk.head * a.hd, *gbase = dout + (size_t)walk.head * a.hd;
     T *dbase = dqkv + (size_t)walk.head * a.hd;
     const int per = Slots<NB>::per_tile(a.n);
     const long long tiles = (a.windows + per - 1) / per;
-    const bool mask = labels || a.sd || a.sh || a.sw;
     const int kb0 = wave / NB * NB;
     const int q = wave * 16 + i;
     f32x4 bias[NB], dbias[NB];
@@ -350,55 +537,70 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
         dbias[j] = f32x4{};
     }
     const float scale2 = a.scale * kLog2e;
-
+    const Spotter<NB> spotter(a);
+    const bool first_wave = threadIdx.x < 64;
+    if (first_wave) {
+        spotter.write(spots[0], spotter.look(a, labels, walk.tile * per));
+        spotter.write(spots[1], spotter.look(a, labels, (walk.tile + walk.step) * per));
+    }
+    if (threadIdx.x < 3) odd_s[threadIdx.x] = 0;
+    __syncthreads();
+    R qr_, kr, vr, gr;
+    auto fetch = [&](const Spots &at) {
+        int token[R::kPieces];
+        tokens_at<T, HD>(at, token);
+        qr_.load(base, stride, token, a.hd);
+        kr.load(base + C, stride, token, a.hd);
+        vr.load(base + 2 * C, stride, token, a.hd);
+        gr.load(gbase, C, token, a.hd);
+    };
+    if (walk.tile < tiles) fetch(spots[0]);
+    int now = 0;
     for (long long tile = walk.tile; tile < tiles; tile += walk.step) {
+        const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
         __syncthreads();
-        if (threadIdx.x < 64) {
-            int w, t;
-            Slots<NB>::of(a, threadIdx.x, w, t);
-            Place p{-1, -1, 0};
-            if (t >= 0) p = place_of(a, labels, tile * per + w, t);
-            token_s[threadIdx.x] = p.token;
-            label_s[threadIdx.x] = p.label;
-            wrap_s[threadIdx.x] = p.wrap;
+        qr_.store_columns(Qt);
+        kr.store_rows(Ks);
+        if constexpr (!K_BY_ROWS) kr.store_columns(Kt);
+        vr.store_rows(Vs);
+        gr.store_columns(Gt);
+        if constexpr (NB == 1) {
+            if (not_finite(qr_) || not_finite(kr) || not_finite(vr) || not_finite(gr)) odd_s[now] = 1;
         }
         __syncthreads();
-        for (int k = threadIdx.x; k < 64 * (HD / 4); k += kAttnThreads) {
-            const int s = k / (HD / 4), c = k % (HD / 4) * 4;
-            const int t = label_s[s] < 0 ? -1 : token_s[s];
-            *(Frag *)&Qs[s * STRIDE + c] = load4<T>(base, stride, t, c, a.hd);
-            *(Frag *)&Ks[s * STRIDE + c] = load4<T>(base + C, stride, t, c, a.hd);
-            *(Frag *)&Vs[s * STRIDE + c] = load4<T>(base + 2 * C, stride, t, c, a.hd);
-            *(Frag *)&Gs[s * STRIDE + c] = load4<T>(dout + (size_t)walk.head * a.hd, C, t, c, a.hd);
-        }
-        const int mine = token_s[q], ql = label_s[q], qr = wrap_s[q];
-        __syncthreads();
+        const Spots &at = spots[now];
+        const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
+        const bool mixed = at.mixed, odd = NB == 1 && odd_s[now];
+        if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
+        if (tile + walk.step < tiles) fetch(spots[next]);
+        Place coming;
+        if (first_wave) coming = spotter.look(a, labels, (tile + 2 * walk.step) * per);
         Frag qf[CB], gf[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-            qf[c] = row4<T>(&Qs[q * STRIDE + c * 16 + 4 * g]);
-            gf[c] = row4<T>(&Gs[q * STRIDE + c * 16 + 4 * g]);
-        }
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                qf[c][r] = Qt[(c * 16 + 4 * g + r) * 68 + q];
+                gf[c][r] = Gt[(c * 16 + 4 * g + r) * 68 + q];
+            }
         f32x4 s[NB], dp[NB];
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            f32x4 acc{}, acc2{};
-#pragma unroll
-            for (int c = 0; c < CB; ++c) {
-                const int at = ((kb0 + j) * 16 + i) * STRIDE + c * 16 + 4 * g;
-                acc = M::run(row4<T>(&Ks[at]), qf[c], acc);
-                acc2 = M::run(row4<T>(&Vs[at]), gf[c], acc2);
-            }
-            dp[j] = acc2;
-            const int key = (kb0 + j) * 16 + 4 * g;
+            const f32x4 acc = over_channels<T, HD>(Ks, (kb0 + j) * 16, qf);
+            dp[j] = over_channels<T, HD>(Vs, (kb0 + j) * 16, gf);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = bias[j][r] == -INFINITY ? -INFINITY : acc[r] * scale2 + bias[j][r];
-                if (mask) x = masked(x, ql, qr, label_s[key + r], wrap_s[key + r], a.outside2);
-                s[j][r] = x;
-                top = fmaxf(top, x);
+                s[j][r] = acc[r] * scale2 + bias[j][r];
+                if (NB == 1 && bias[j][r] == -INFINITY) s[j][r] = -INFINITY, dp[j][r] = 0.f;
             }
+            if (mixed) {
+                const int key = (kb0 + j) * 16 + 4 * g;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[j][r]);
         }
         top = fold_max(top);
         if (top == -INFINITY) top = 0.f;
@@ -407,7 +609,7 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
         for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[j][r] = exp2f(s[j][r] - top);
+                s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - top);
                 sum += s[j][r];
                 delta += s[j][r] * dp[j][r];
             }
@@ -417,51 +619,62 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
         Frag ds[NB], p[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const f32x4 pv = s[j] * inv;
-            const f32x4 d = pv * (dp[j] - delta);
+            f32x4 pv = s[j] * inv;
+            f32x4 d = pv * (dp[j] - delta);
+            if constexpr (NB == 1) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (bias[j][r] == -INFINITY) pv[r] = d[r] = 0.f;
+            }
             dbias[j] += d;
             p[j] = M::frag(pv);
             ds[j] = M::frag(d);  // 16 bit: rounded once, as the products take it; the table's gradient sums it unrounded
         }
+        f32x4 acc[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-            f32x4 dq{};
+        for (int c = 0; c < CB; ++c) acc[c] = f32x4{};
+        over_unit<T, HD, NB, K_BY_ROWS>(acc, K_BY_ROWS ? Ks : Kt, kb0 * 16, ds, odd, a.n);
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
-                dq = M::run(column<T, STRIDE>(Ks, (kb0 + j) * 16 + 4 * g, c * 16 + i), ds[j], dq);
+        for (int c = 0; c < CB; ++c)
             if (mine >= 0 && c * 16 + 4 * g < a.hd)
-                *(Frag *)(dbase + (size_t)mine * stride + c * 16 + 4 * g) = M::frag(dq * a.scale);
-        }
+                *(Frag *)(dbase + (size_t)mine * stride + c * 16 + 4 * g) = M::frag(acc[c] * a.scale);
         __syncthreads();  // V has been used
+        const int ql_ = wave % NB * 16 + i;  // this lane's query within its unit
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = (kb0 + j) * 16 + 4 * g + r;
+                Ps[key * PS + ql_] = p[j][r];
+                Ss[key * PS + ql_] = ds[j][r];
+            }
+        __syncthreads();
+        // now slot q is this lane's key
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            *(Frag *)&Ps[q * PS + j * 16 + 4 * g] = p[j];
-            *(Frag *)&Ss[q * PS + j * 16 + 4 * g] = ds[j];
+            p[j] = row4<T>(&Ps[q * PS + j * 16 + 4 * g]);
+            ds[j] = row4<T>(&Ss[q * PS + j * 16 + 4 * g]);
         }
-        __syncthreads();
-        const int kc = wave % NB * 16 + i;  // this lane's key within the unit
+        f32x4 dv[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) {
-            f32x4 dv{}, dk{};
+        for (int c = 0; c < CB; ++c) acc[c] = dv[c] = f32x4{};
+        over_unit<T, HD, NB>(dv, Gt, kb0 * 16, p, odd, a.n);
+        over_unit<T, HD, NB>(acc, Qt, kb0 * 16, ds, odd, a.n);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const int qb = (kb0 + j) * 16 + 4 * g;
-                dv = M::run(column<T, STRIDE>(Gs, qb, c * 16 + i), column<T, PS>(Ps, qb, kc), dv);
-                dk = M::run(column<T, STRIDE>(Qs, qb, c * 16 + i), column<T, PS>(Ss, qb, kc), dk);
-            }
-            if (mine >= 0 && c * 16 + 4 * g < a.hd) {  // (slot q is also this lane's key)
+        for (int c = 0; c < CB; ++c)
+            if (mine >= 0 && c * 16 + 4 * g < a.hd) {
                 T *to = dbase + (size_t)mine * stride + c * 16 + 4 * g;
-                *(Frag *)(to + C) = M::frag(dk * a.scale);
-                *(Frag *)(to + 2 * C) = M::frag(dv);
+                *(Frag *)(to + C) = M::frag(acc[c] * a.scale);
+                *(Frag *)(to + 2 * C) = M::frag(dv[c]);
             }
-        }
+        if (first_wave) spotter.write(spots[after], coming);
+        now = next;
     }
     if (!pairs) return;
     float *to = pairs + (size_t)blockIdx.x * 64 * 16 * NB;
 #pragma unroll
     for (int j = 0; j < NB; ++j) *(f32x4 *)&to[q * 16 * NB + j * 16 + 4 * g] = dbias[j];
 }
-
 
 // ================================================================================================
 // Longer windows (65 .. 4096 tokens): tiles of 64 queries against tiles of 64 keys, with the running maximum and sum
@@ -520,33 +733,6 @@ __device__ __forceinline__ Meets meets(const LongMap &m, long long window, int t
     return {__ballot(any), __ballot(any && !(even && same))};
 }
 
-// 64 rows on their way to LDS: HD / 16 pieces of four channels in each thread
-template <class T, int HD>
-struct Rows {
-    using Frag = typename Mma<T>::Frag;
-    static constexpr int kPieces = HD / 16, kRowStep = kAttnThreads / (HD / 4);
-    Frag f[kPieces];
-    static __device__ __forceinline__ int row(int m) { return threadIdx.x / (HD / 4) + m * kRowStep; }
-    static __device__ __forceinline__ int channel() { return threadIdx.x % (HD / 4) * 4; }
-    __device__ __forceinline__ void load(const T *__restrict__ base, long long stride, const int (&token)[kPieces], int hd)
-    {
-#pragma unroll
-        for (int m = 0; m < kPieces; ++m) f[m] = load4<T>(base, stride, token[m], channel(), hd);
-    }
-    __device__ __forceinline__ void store_rows(T *tile) const  // [64][HD + 4]
-    {
-#pragma unroll
-        for (int m = 0; m < kPieces; ++m) *(Frag *)&tile[row(m) * (HD + 4) + channel()] = f[m];
-    }
-    __device__ __forceinline__ void store_columns(T *tile) const  // [HD][64 + 4]
-    {
-#pragma unroll
-        for (int m = 0; m < kPieces; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tile[(channel() + e) * 68 + row(m)] = f[m][e];
-    }
-};
-
 // the tokens of a tile's rows as a thread stages them (-1: zeros)
 template <class T, int HD>
 __device__ __forceinline__ void tokens_of(const PlaceAt *tile, int (&token)[Rows<T, HD>::kPieces])
@@ -555,37 +741,6 @@ __device__ __forceinline__ void tokens_of(const PlaceAt *tile, int (&token)[Rows
     for (int m = 0; m < Rows<T, HD>::kPieces; ++m) {
         const PlaceAt p = tile[Rows<T, HD>::row(m)];
         token[m] = p.label < 0 ? -1 : p.token;
-    }
-}
-
-// D[token 4g ..][column i] for a block of 16 rows of a row-major tile against a lane's operand: contraction over channels
-template <class T, int HD>
-__device__ __forceinline__ f32x4 over_channels(const T *rows, int first, const typename Mma<T>::Frag *own)
-{
-    using M = Mma<T>;
-    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
-    const T *p = rows + (first + i) * (HD + 4) + 4 * g;
-    f32x4 acc{};
-    if constexpr (HD >= 32) {
-#pragma unroll
-        for (int c = 0; c < HD / 16; c += 2) acc = M::run2(row4<T>(p + c * 16), row4<T>(p + c * 16 + 16), own[c], own[c + 1], acc);
-    } else {
-        acc = M::run(row4<T>(p), own[0], acc);
-    }
-    return acc;
-}
-
-// acc[c] += columns^T (channels c * 16 ..) times four blocks of B operands: contraction over 64 tokens
-template <class T, int HD>
-__device__ __forceinline__ void over_tokens(f32x4 (&acc)[HD / 16], const T *columns, const typename Mma<T>::Frag (&b)[4])
-{
-    using M = Mma<T>;
-    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
-#pragma unroll
-    for (int c = 0; c < HD / 16; ++c) {
-        const T *p = columns + (c * 16 + i) * 68 + 4 * g;
-        acc[c] = M::run2(row4<T>(p), row4<T>(p + 16), b[0], b[1], acc[c]);
-        acc[c] = M::run2(row4<T>(p + 32), row4<T>(p + 48), b[2], b[3], acc[c]);
     }
 }
 
@@ -699,7 +854,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
         sum = sum * fade + part;
 #pragma unroll
         for (int c = 0; c < CB; ++c) o[c] *= fade;
-        over_tokens<T, HD>(o, Vt, p);
+        over_tokens<T, HD>(o, Vt, 0, p);
     }
     sum = fold_sum(sum);
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
@@ -799,7 +954,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
             }
             ds[j] = M::frag(d);
         }
-        over_tokens<T, HD>(dq, Kt, ds);
+        over_tokens<T, HD>(dq, Kt, 0, ds);
     }
     rest = fold_sum(rest);
     if (own.token < 0) return;
@@ -900,8 +1055,8 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
             p[j] = M::frag(pv);
             ds[j] = M::frag(d);
         }
-        over_tokens<T, HD>(dv, Gt, p);
-        over_tokens<T, HD>(dk, Qt, ds);
+        over_tokens<T, HD>(dv, Gt, 0, p);
+        over_tokens<T, HD>(dk, Qt, 0, ds);
     }
     if (own.token < 0) return;
 #pragma unroll

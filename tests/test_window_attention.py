@@ -112,14 +112,25 @@ def test_padding_is_not_read(window):
 
 
 @pytest.mark.gpu
-def test_not_finite_scores_spread_no_further_than_their_window():
-    shape, window = (1, 1, 16, 16), (1, 8, 8)
-    qkv, table, dout = data(shape, window, 2, 32, torch.float32, 9)
-    clean, _ = run(qkv, table, window, 2, dout)
-    qkv[0, 0, 3, 3] = float("nan")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("part", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("window", [(1, 8, 8), (4, 1, 1), (1, 2, 2), (3, 1, 1), (2, 4, 4), (4, 8, 8)])
+def test_what_is_not_finite_stays_in_its_window(window, part, dtype):
+    """Also where windows share a block of 16 slots."""
+    shape = (2, 12, 16, 16)
+    qkv, table, dout = data(shape, window, 2, 32, dtype, 9)
+    clean, (clean_grad, _) = run(qkv, table, window, 2, dout)
+    at = (1, 5, 9, 3)
+    if part == "dout":
+        dout[at] = float("nan")
+    else:
+        qkv[at][64 * "qkv".index(part):][:64] = float("inf") if part == "v" else float("nan")
     out, (dqkv, _) = run(qkv, table, window, 2, dout)
-    assert out[:, :, :8, :8].isnan().all() and dqkv[:, :, :8, :8].isnan().any()
-    assert torch.equal(out[:, :, 8:], clean[:, :, 8:]) and torch.equal(out[:, :, :, 8:], clean[:, :, :, 8:])
+    inside = torch.zeros(shape, dtype=torch.bool)
+    inside[(1, *(slice(p // w * w, p // w * w + w) for p, w in zip(at[1:], window)))] = True
+    inside = inside.to(DEV)
+    assert torch.equal(out[~inside], clean[~inside]) and torch.equal(dqkv[~inside], clean_grad[~inside])
+    assert not dqkv[inside].isfinite().all() and (part == "dout" or not out[inside].isfinite().all())
 
 
 @pytest.mark.gpu
