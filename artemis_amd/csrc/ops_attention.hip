@@ -19,7 +19,8 @@ __global__ __launch_bounds__(256) void bias_rows(const float *__restrict__ table
 
 // Long windows: where the tokens of a window lie, and what the tiles of 64 tokens hold.  A wave for a tile.
 __global__ __launch_bounds__(256) void places_of(const WindowArgs a, const int *__restrict__ labels, int tiles,
-                                                 PlaceAt *__restrict__ places, TileAt *__restrict__ tiles_at)
+                                                 PlaceAt *__restrict__ places, int *__restrict__ live,
+                                                 TileAt *__restrict__ tiles_at)
 {
     const long long tile = blockIdx.x * 4LL + threadIdx.x / 64;
     if (tile >= a.windows * tiles) return;  // (a whole wave)
@@ -30,9 +31,10 @@ __global__ __launch_bounds__(256) void places_of(const WindowArgs a, const int *
         p = PlaceAt{at.token, corner(a, t), at.label, at.wrap};
     }
     places[tile * 64 + lane] = p;
+    live[tile * 64 + lane] = p.label < 0 ? -1 : p.token;
     const int label = __shfl(p.label, 0), wrap = __shfl(p.wrap, 0);
     const bool even = __all(p.label >= 0 && p.label == label && p.wrap == wrap), dead = __all(p.label < 0);
-    if (lane == 0) tiles_at[tile] = TileAt{dead ? kDead : even ? kEven : kMixed, label, wrap, 0};
+    if (lane == 0) tiles_at[tile] = TileAt{dead ? kDead : even ? kEven : kMixed, label, wrap, p.corner};
 }
 
 // dense[head][e] = the sum of the shares of the workgroups that have that head, in a fixed order: 16 elements for a
@@ -81,38 +83,51 @@ __global__ __launch_bounds__(256) void table_small(const WindowArgs a, const flo
     if (lane == 0) dtable[(size_t)e * a.heads + head] = s;
 }
 
-// dtable[e][head] for long windows that tiles of ed x eh x ew = 64 tokens divide: dense is [chunk][distance of tiles]
+// dtable[e][head] for long windows that tiles of ed x eh x ew = 64 tokens divide: dense is [share][distance of tiles]
 // [head][64][64] (long_bwd_pairs).  For each query of a tile the key at this distance is one token of one tile: 64 terms for
-// each chunk.  Neighbouring lanes have neighbouring distances: they read neighbouring keys.
+// each share, a quarter for each wave.  Neighbouring lanes have neighbouring distances: they read neighbouring keys.
 __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const PairWork w, const float *__restrict__ dense,
                                                    float *__restrict__ dtable, int distances)
 {
-    const int e = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
-    if (e >= a.entries) return;
-    const int ed = a.wd / w.gd, eh = a.wh / w.gh, ew = a.ww / w.gw;
+    __shared__ float fold[4][64];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, head = blockIdx.y;
+    const int e = min(blockIdx.x * 64 + lane, a.entries - 1);
     const int dw = e % a.rh - (a.ww - 1), dh = e / a.rh % (2 * a.wh - 1) - (a.wh - 1), dd = e / a.rd - (a.wd - 1);
-    // distance d of tokens i - k: tiles D = (d - i + k) / e apart, with k = (i - d) mod e
-    auto split = [](int i, int d, int size, int &k, int &D) {
-        int r = (i - d) % size;
-        k = r < 0 ? r + size : r;
-        D = (d - i + k) / size;
+    // One axis: tokens i of a query's tile, `size` long, at distance d.  With m = d mod size the key is i - m in the tile
+    // (d - m) / size away for i >= m, and i - m + size in the tile one further for i < m.
+    struct Axis {
+        int size, tiles, m, far;
+        __device__ Axis(int d, int tokens, int tiles) : size(tokens / tiles), tiles(tiles)
+        {
+            m = d % size;
+            if (m < 0) m += size;
+            far = (d - m) / size;
+        }
+        // the key, and the distance of tiles counted as 0, 1, -1, 2, -2, ...; -1: beyond the window for every tile
+        __device__ __forceinline__ int key(int i) const { return i < m ? i - m + size : i - m; }
+        __device__ __forceinline__ int distance(int i) const
+        {
+            const int D = i < m ? far + 1 : far;
+            return abs(D) >= tiles ? -1 : D > 0 ? 2 * D - 1 : -2 * D;
+        }
     };
-    auto fold = [](int D) { return D > 0 ? 2 * D - 1 : -2 * D; };  // 0, 1, -1, 2, -2, ... -> 0, 1, 2, 3, 4
+    const Axis x(dw, a.ww, w.gw), y(dh, a.wh, w.gh), z(dd, a.wd, w.gd);
     float s = 0.f;
-    for (int chunk = 0; chunk < w.chunks; ++chunk) {
+    for (int share = 0; share < w.chunks * w.subs; ++share) {
+        const float *from = dense + ((size_t)share * distances * a.heads + head) * 4096;
 #pragma unroll 8
-        for (int q = 0; q < 64; ++q) {
-            const int x = q % ew, y = q / ew % eh, z = q / ew / eh;
-            int kx, ky, kz, Dx, Dy, Dz;
-            split(x, dw, ew, kx, Dx);
-            split(y, dh, eh, ky, Dy);
-            split(z, dd, ed, kz, Dz);
-            if (abs(Dx) >= w.gw || abs(Dy) >= w.gh || abs(Dz) >= w.gd) continue;  // out of the window for every tile
-            const int at = (fold(Dz) * (2 * w.gh - 1) + fold(Dy)) * (2 * w.gw - 1) + fold(Dx);
-            s += dense[((((size_t)chunk * distances + at) * a.heads + head) * 64 + q) * 64 + (kz * eh + ky) * ew + kx];
+        for (int q = wave * 16; q < wave * 16 + 16; ++q) {  // (the same q in every lane: its coordinates are scalars)
+            const int ix = q % x.size, iy = q / x.size % y.size, iz = q / x.size / y.size;
+            const int dx = x.distance(ix), dy = y.distance(iy), dz = z.distance(iz);
+            if ((dx | dy | dz) >= 0)
+                s += from[(size_t)((dz * (2 * w.gh - 1) + dy) * (2 * w.gw - 1) + dx) * a.heads * 4096 + q * 64 +
+                          (z.key(iz) * y.size + y.key(iy)) * x.size + x.key(ix)];
         }
     }
-    dtable[(size_t)e * a.heads + head] = s;
+    fold[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && (int)blockIdx.x * 64 + lane < a.entries)
+        dtable[(size_t)e * a.heads + head] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
 }
 
 // dtable[e][head] for other long windows, from dense [head][n][n]: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
@@ -206,28 +221,46 @@ int make_args(const char *what, const artemis_ops_window *w, WindowArgs &a)
 }
 
 // How the table's gradient goes through a long window's pairs (long_bwd_pairs): 64 tokens in a row of the raster that fill
-// whole rows, or whole planes, evenly; and shares of the windows until there is work for about 2048 workgroups.
+// whole rows, or whole planes, evenly; and shares of the windows, then of a window's pairs (at most 64), until there is work
+// for about 2048 workgroups or four pairs are left for each on average.
+#ifndef OPS_PAIR_TARGET
+#define OPS_PAIR_TARGET 2048
+#endif
 PairWork pair_work(const WindowArgs &a)
 {
-    PairWork w{0, 0, 0, 1};
+    PairWork w{0, 0, 0, 1, 1};
     const int plane = a.wh * a.ww;
     if (a.ww % 64 == 0)
-        w = {a.wd, a.wh, a.ww / 64, 1};
+        w = {a.wd, a.wh, a.ww / 64, 1, 1};
     else if (64 % a.ww == 0 && a.wh % (64 / a.ww) == 0)
-        w = {a.wd, a.wh / (64 / a.ww), 1, 1};
+        w = {a.wd, a.wh / (64 / a.ww), 1, 1, 1};
     else if (64 % plane == 0 && a.wd % (64 / plane) == 0)
-        w = {a.wd / (64 / plane), 1, 1, 1};
+        w = {a.wd / (64 / plane), 1, 1, 1, 1};
     if (w.gd) {
-        const long long groups = (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads;
-        const long long want = 2048 / groups;
+        const long long distances = (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1), groups = distances * a.heads;
+        const long long tiles = w.gd * w.gh * w.gw, want = OPS_PAIR_TARGET / groups;
         w.chunks = (int)(want < 1 ? 1 : want < a.windows ? want : a.windows);
+        const long long more = OPS_PAIR_TARGET / (groups * w.chunks), most = tiles * tiles / distances / 4;
+        w.subs = (int)(more < 1 || most < 1 ? 1 : more < most ? more : most);
     }
     return w;
 }
 
+// Workgroups that share a tile's partners where there are few tiles: about 2048 in all, each with four partners at least.
+#ifndef OPS_SPLIT_TARGET
+#define OPS_SPLIT_TARGET 2048
+#endif
+int split_count(const WindowArgs &a)
+{
+    const long long tiles = (a.n + 63) / 64, groups = a.windows * a.heads * tiles;
+    const long long want = OPS_SPLIT_TARGET / groups, most = tiles / 4;
+    return (int)(want < 1 || most < 1 ? 1 : want < most ? want : most);
+}
+
 struct Layout {
-    size_t bias, rev, places, tiles, pairs, dense, delta, total;
+    size_t bias, rev, places, live, tiles, pairs, dense, delta, split_a, split_b, split_rows, total;
     PairWork work;
+    int splits;
 };
 Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool table)
 {
@@ -241,16 +274,24 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
     if (a.n > 64) {
         const size_t tiles = (size_t)(a.n + 63) / 64;
         l.places = take(a.windows * tiles * 64 * sizeof(PlaceAt));
+        l.live = take(a.windows * tiles * 64 * sizeof(int));
         l.tiles = take(a.windows * tiles * sizeof(TileAt));
         if (table) {
             l.bias = take((size_t)a.entries * a.heads * 4);
             l.rev = take((size_t)a.entries * a.heads * 4);
         }
-        if (backward) l.delta = take((size_t)a.windows * a.heads * a.n * 4);
+        const size_t lines = (size_t)a.windows * a.heads * tiles * 64;
+        if (backward) l.delta = take(lines * 4);
+        l.splits = split_count(a);
+        if (l.splits > 1) {
+            l.split_a = take(l.splits * lines * a.hd * 4);
+            if (backward) l.split_b = take(l.splits * lines * a.hd * 4);
+            l.split_rows = take(l.splits * lines * 2 * 4);
+        }
         if (backward && need_dtable) {
             l.work = pair_work(a);
             const PairWork &w = l.work;
-            l.dense = take(w.gd ? (size_t)w.chunks * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
+            l.dense = take(w.gd ? (size_t)w.chunks * w.subs * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
                                 : (size_t)a.heads * a.n * a.n * 4);
         }
     } else if (backward && need_dtable) {
@@ -264,17 +305,24 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
 
 bool aligned4(const void *p, int dtype) { return ((size_t)p & (dtype == ARTEMIS_OPS_F32 ? 15 : 7)) == 0; }
 
-// Long windows: fills the maps in the workspace
-LongMap long_map(const WindowArgs &a, const Layout &l, const float *table, const int *labels, char *ws, hipStream_t st)
+// Long windows: what the kernels find in the workspace; fills the maps
+void long_buffers(AttnBuffers &b, const WindowArgs &a, const Layout &l, const float *table, const int *labels, char *ws,
+                  hipStream_t st)
 {
+    const int last = 63;  // of a tile: how far its corners reach
+    const int reach = last / a.ww / a.wh * a.rd + last / a.ww % a.wh * a.rh + last % a.ww;
+    b.even = pair_work(a).gd > 0 && a.ww % 4 == 0 && 2 * reach + 4 <= kSpan;
+    b.split = Split{l.splits, (float *)(ws + l.split_a), (float *)(ws + l.split_b), (float *)(ws + l.split_rows)};
     LongMap m{};
     m.tiles = (a.n + 63) / 64;
     PlaceAt *places = (PlaceAt *)(ws + l.places);
     TileAt *tiles = (TileAt *)(ws + l.tiles);
     m.places = places;
     m.tiles_at = tiles;
+    int *live = (int *)(ws + l.live);
+    m.live = live;
     hipLaunchKernelGGL(places_of, dim3((unsigned)((a.windows * m.tiles + 3) / 4)), dim3(256), 0, st, a, labels, m.tiles, places,
-                       tiles);
+                       live, tiles);
     if (table) {
         float *bias = (float *)(ws + l.bias), *rev = (float *)(ws + l.rev);
         const int n = a.entries * a.heads;
@@ -282,7 +330,7 @@ LongMap long_map(const WindowArgs &a, const Layout &l, const float *table, const
         m.bias = bias;
         m.rev = rev;
     }
-    return m;
+    b.map = m;
 }
 
 }  // namespace
@@ -296,7 +344,7 @@ size_t artemis_ops_window_attention_lse_count(const artemis_ops_window *w)
 {
     WindowArgs a;
     if (make_args("artemis_ops_window_attention", w, a)) return 0;
-    return a.n > 64 ? (size_t)a.windows * a.heads * a.n : 0;
+    return a.n > 64 ? (size_t)a.windows * a.heads * ((a.n + 63) / 64) * 64 : 0;
 }
 
 size_t artemis_ops_window_attention_workspace_bytes(const artemis_ops_window *w, int backward, int need_dtable)
@@ -328,7 +376,7 @@ int artemis_ops_window_attention_forward(const artemis_ops_window *w, const void
     b.out = out;
     b.lse = lse;
     b.groups = a.n <= 64 ? fwd_groups(a) : 0;
-    if (a.n > 64) b.map = long_map(a, l, table, labels, (char *)workspace, st);
+    if (a.n > 64) long_buffers(b, a, l, table, labels, (char *)workspace, st);
     if (w->dtype == ARTEMIS_OPS_F32)
         launch_attention_fwd<float>(a, b, st);
     else if (w->dtype == ARTEMIS_OPS_BF16)
@@ -376,7 +424,7 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
         b.dense = (float *)(ws + l.dense);
         if (!is_long) b.pairs = (float *)(ws + l.pairs);
     }
-    if (is_long) b.map = long_map(a, l, table, labels, ws, st);
+    if (is_long) long_buffers(b, a, l, table, labels, ws, st);
     b.work = l.work;
     if (w->dtype == ARTEMIS_OPS_F32)
         launch_attention_bwd<float>(a, b, st);
@@ -386,7 +434,7 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
         launch_attention_bwd<_Float16>(a, b, st);
     if (dtable && is_long && b.work.gd) {
         const int distances = (2 * b.work.gd - 1) * (2 * b.work.gh - 1) * (2 * b.work.gw - 1);
-        hipLaunchKernelGGL(table_tiled, dim3((a.entries + 255) / 256, a.heads), dim3(256), 0, st, a, b.work, b.dense, dtable,
+        hipLaunchKernelGGL(table_tiled, dim3((a.entries + 63) / 64, a.heads), dim3(256), 0, st, a, b.work, b.dense, dtable,
                            distances);
     } else if (dtable && is_long) {
         hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st,

@@ -694,73 +694,124 @@ struct PlaceAt {
     int token, corner, label, wrap;  // token -1: none (behind the window's end); label < 0: padding
 };
 struct TileAt {
-    int state, label, wrap, unused;  // kMixed; kEven: 64 live tokens of one region; kDead: no live token
+    int state, label, wrap;  // kMixed; kEven: 64 live tokens of one region; kDead: no live token
+    int corner;              // of the tile's first token
 };
 constexpr int kMixed = 0, kEven = 1, kDead = 2;
 
 struct LongMap {
     const PlaceAt *places;   // (windows, tiles * 64)
+    const int *live;         // the same: the token, -1 for none and for padding
     const TileAt *tiles_at;  // (windows, tiles)
     const float *bias;       // (heads, entries) * log2 e, or NULL
     const float *rev;        // the same, every head's entries in reverse
     int tiles;               // of 64 tokens in a window, at most 64
 };
 
+// Few workgroups: `splits` of them share a tile's partners, and their sums are joined by a second kernel.
+struct Split {
+    int splits;
+    float *a, *b;  // [split][window, head, tile, 64][head_dim]: sums of the products over tokens
+    float *rows;   // [split][window, head, tile, 64][2]: forward: maximum and sum of the softmax; dQ: delta's share
+};
+
 struct LongTile {
     long long window;
     int head, tile;
 };
+// Workgroups 8 apart run on one XCD: each XCD takes a run of neighbouring tiles, head by head, so that its cache holds few
+// heads' rows and biases, and so that tiles with more to do than others (the last row of every plane padding, say) do not
+// all fall to one XCD, as they do where tile t goes to XCD t % 8.
 __device__ __forceinline__ LongTile long_tile(const WindowArgs &a, int tiles)
 {
-    const unsigned t = blockIdx.x % (unsigned)tiles, r = blockIdx.x / (unsigned)tiles;
+    const unsigned x = blockIdx.x % 8, each = gridDim.x / 8, more = gridDim.x % 8;
+    const unsigned id = x * each + (x < more ? x : more) + blockIdx.x / 8;
+    const unsigned t = id % (unsigned)tiles, r = id / (unsigned)tiles;
     return {(long long)(r / (unsigned)a.heads), (int)(r % (unsigned)a.heads), (int)t};
 }
 
-// Which tiles a tile meets, one bit each (every lane of a wave looks at one tile)
+// whether two tiles meet at all, and whether they need a mask
+__device__ __forceinline__ void relation(const TileAt &x, const TileAt &y, float outside2, bool &any, bool &mixed)
+{
+    const bool even = x.state == kEven && y.state == kEven;
+    const bool same = x.label == y.label && x.wrap == y.wrap;
+    any = x.state != kDead && y.state != kDead && !(even && !same && outside2 == -INFINITY);
+    mixed = any && !(even && same);
+}
+
+// Which tiles a tile meets, one bit each (every lane of a wave looks at one tile); of these, every splits-th is this
+// workgroup's.
 struct Meets {
-    unsigned long long any, mixed;
+    unsigned long long todo, mixed;
+    int corner;  // this lane's tile's first token's
 };
-__device__ __forceinline__ Meets meets(const LongMap &m, long long window, int tile, float outside2)
+__device__ __forceinline__ Meets meets(const LongMap &m, long long window, int tile, float outside2, int splits)
 {
     const TileAt *row = m.tiles_at + window * m.tiles;
     const TileAt own = row[tile];
     const int lane = threadIdx.x % 64;
     TileAt other{kDead, 0, 0, 0};
     if (lane < m.tiles) other = row[lane];
-    const bool even = own.state == kEven && other.state == kEven;
-    const bool same = own.label == other.label && own.wrap == other.wrap;
-    const bool any = own.state != kDead && other.state != kDead && !(even && !same && outside2 == -INFINITY);
-    return {__ballot(any), __ballot(any && !(even && same))};
+    bool any, mixed;
+    relation(own, other, outside2, any, mixed);
+    unsigned long long all = __ballot(any);
+    if (splits > 1) {
+        const int rank = __popcll(all & ((1ull << lane) - 1));
+        all = __ballot(any && rank % splits == (int)blockIdx.y);
+    }
+    return {all, __ballot(mixed), other.corner};
 }
 
-// the tokens of a tile's rows as a thread stages them (-1: zeros)
-template <class T, int HD>
-__device__ __forceinline__ void tokens_of(const PlaceAt *tile, int (&token)[Rows<T, HD>::kPieces])
-{
+// The bias of a tile's pairs.
+// EVEN (64 tokens tile the window, its rows are multiples of 4, and two tiles' distances span at most kSpan entries): the
+// entries of a pair of tiles are one run of the row, which the workgroup copies to LDS, a tile ahead; a lane's four lie
+// behind each other there.  (Loading them from the row itself is 16 bytes a lane at any alignment, and was a third of all
+// the work of the address units.)  Else: each by itself.
+constexpr int kSpan = 512;
+template <bool EVEN>
+struct Biases {
+    f32x4 now[4];
+    float ahead[2];
+    int at[4], start;
+    const float *row;  // this head's entries
+    // `sign`: an entry's place grows with +-corner(own); `own`, `partner`: corners of this lane's token and of the first tile's
+    __device__ __forceinline__ Biases(const float *head_row, const WindowArgs &a, int own, int own_tile, const PlaceAt *first_tile)
+        : row(head_row)
+    {
+        const int g = threadIdx.x % 64 / 16;
+        const int reach = EVEN ? first_tile[63].corner : 0;  // between the first and the last token of a tile
+        start = middle(a) - own_tile - reach;
 #pragma unroll
-    for (int m = 0; m < Rows<T, HD>::kPieces; ++m) {
-        const PlaceAt p = tile[Rows<T, HD>::row(m)];
-        token[m] = p.label < 0 ? -1 : p.token;
+        for (int j = 0; j < 4; ++j) {
+            now[j] = f32x4{};
+            at[j] = EVEN ? reach - (own - own_tile) + first_tile[j * 16 + 4 * g].corner : middle(a) - own;
+        }
     }
-}
-
-// Four neighbouring bias entries.  VEC: they lie behind each other in `table` (rows of the window are multiples of 4).
-template <bool VEC>
-__device__ __forceinline__ f32x4 four_biases(const float *__restrict__ table, int own, const PlaceAt *at)
-{
-    f32x4 b{};
-    if (!table) return b;
-    if constexpr (VEC) {
-        struct __attribute__((packed, aligned(4))) Loose {
-            f32x4 v;
-        };
-        b = ((const Loose *)(table + own + at[0].corner))->v;
-    } else {
+    __device__ __forceinline__ void fetch(const WindowArgs &a, int tile_corner)
+    {
+        if (!EVEN || !row) return;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) b[r] = table[own + at[r].corner];
+        for (int k = 0; k < 2; ++k) {
+            const int e = start + tile_corner + k * kAttnThreads + threadIdx.x;
+            ahead[k] = e >= 0 && e < a.entries ? row[e] : 0.f;
+        }
     }
-    return b;
-}
+    __device__ __forceinline__ void store(float *run)
+    {
+        if (!EVEN || !row) return;
+        run[threadIdx.x] = ahead[0];
+        run[threadIdx.x + kAttnThreads] = ahead[1];
+    }
+    __device__ __forceinline__ void take(const float *run, const PlaceAt *tile)
+    {
+        if (!row) return;
+        const int g = threadIdx.x % 64 / 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) now[j][r] = EVEN ? run[at[j] + r] : row[at[j] + tile[j * 16 + 4 * g + r].corner];
+    }
+};
 
 // the scores of four pairs in the exponent of 2
 __device__ __forceinline__ f32x4 scores(f32x4 acc, float scale2, f32x4 bias, bool mixed, const PlaceAt &own, const PlaceAt *at,
@@ -776,27 +827,62 @@ __device__ __forceinline__ f32x4 scores(f32x4 acc, float scale2, f32x4 bias, boo
     return x;
 }
 
-template <class T, int HD, bool VEC>
-__global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, const LongMap map, const T *__restrict__ qkv,
-                                                         T *__restrict__ out, float *__restrict__ lse)
+// What a thread has in flight of the tiles to come: the rows of the next one, the tokens of the one after it.
+template <class T, int HD>
+struct Ahead {
+    using R = Rows<T, HD>;
+    R x, y;        // rows of two tensors
+    PlaceAt at;    // of the tile's token threadIdx.x % 64
+    int token[R::kPieces];
+    __device__ __forceinline__ void tokens(const int *live, int t)
+    {
+#pragma unroll
+        for (int m = 0; m < R::kPieces; ++m) token[m] = live[t * 64 + R::row(m)];
+    }
+    __device__ __forceinline__ void rows(const T *xb, long long xs, const T *yb, long long ys, int hd)
+    {
+        x.load(xb, xs, token, hd);
+        y.load(yb, ys, token, hd);
+    }
+};
+
+template <class T, int HD, bool EVEN>
+__global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, const LongMap map, const Split split,
+                                                         const T *__restrict__ qkv, T *__restrict__ out,
+                                                         float *__restrict__ lse)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
     __shared__ __align__(16) T Ks[64 * (HD + 4)];
     __shared__ __align__(16) T Vt[HD * 68];
     __shared__ __align__(16) PlaceAt at_s[64];
+    __shared__ float bias_s[EVEN ? kSpan : 1];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
-    const float *rev = map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
+    const Meets meet = meets(map, lt.window, lt.tile, a.outside2, split.splits);
+    const int *live = map.live + lt.window * map.tiles * 64;
+    unsigned long long todo = meet.todo, later = todo & (todo - 1);
+    Ahead<T, HD> ahead;
+    auto rows = [&](int t) {
+        ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
+        if (threadIdx.x < 64 && (!EVEN || (meet.mixed >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
+    };
+    if (todo) ahead.tokens(live, __builtin_ctzll(todo));
     const PlaceAt own = window[lt.tile * 64 + q];
-    const int at0 = middle(a) - own.corner;  // entry of the reversed row: middle - corner(q) + corner(k)
+    // entry of the reversed row: middle - corner(q) + corner(k)
+    Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
+                      window[lt.tile * 64].corner, window);
+    if (todo) {
+        rows(__builtin_ctzll(todo));
+        bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
+        if (later) ahead.tokens(live, __builtin_ctzll(later));
+    }
     Frag qf[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) qf[c] = load4<T>(base, stride, own.label < 0 ? -1 : own.token, c * 16 + 4 * g, a.hd);
@@ -805,34 +891,27 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
     f32x4 o[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) o[c] = f32x4{};
-    const Meets meet = meets(map, lt.window, lt.tile, a.outside2);
-    unsigned long long todo = meet.any;
-    R kr, vr;
-    PlaceAt at{};
-    int token[R::kPieces];
-    auto fetch = [&](int t) {
-        tokens_of<T, HD>(window + t * 64, token);
-        kr.load(base + C, stride, token, a.hd);
-        vr.load(base + 2 * C, stride, token, a.hd);
-        if (threadIdx.x < 64) at = window[t * 64 + threadIdx.x];
-    };
-    if (todo) fetch(__builtin_ctzll(todo));
     while (todo) {
         const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
-        todo &= todo - 1;
+        todo = later;
+        later &= later - 1;
         __syncthreads();  // the tile before has been used
-        kr.store_rows(Ks);
-        vr.store_columns(Vt);
-        if (threadIdx.x < 64) at_s[threadIdx.x] = at;
-        if (todo) fetch(__builtin_ctzll(todo));
+        ahead.x.store_rows(Ks);
+        ahead.y.store_columns(Vt);
+        if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
+        bias.store(bias_s);
         __syncthreads();
-        f32x4 s[4], bias[4];
+        bias.take(bias_s, at_s);
+        if (todo) {
+            rows(__builtin_ctzll(todo));
+            bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
+            if (later) ahead.tokens(live, __builtin_ctzll(later));
+        }
+        f32x4 s[4];
         float high = top;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bias[j] = four_biases<VEC>(rev, at0, &at_s[j * 16 + 4 * g]);
-#pragma unroll
         for (int j = 0; j < 4; ++j) {
-            s[j] = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g], a.outside2);
+            s[j] = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias.now[j], mixed, own, &at_s[j * 16 + 4 * g], a.outside2);
 #pragma unroll
             for (int r = 0; r < 4; ++r) high = fmaxf(high, s[j][r]);
         }
@@ -857,6 +936,15 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
         over_tokens<T, HD>(o, Vt, 0, p);
     }
     sum = fold_sum(sum);
+    const size_t padded = (((size_t)lt.window * a.heads + lt.head) * map.tiles + lt.tile) * 64 + q;
+    if (split.splits > 1) {
+        const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + padded;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+            if (c * 16 + 4 * g < a.hd) *(f32x4 *)(split.a + line * a.hd + c * 16 + 4 * g) = o[c];
+        if (g == 0) split.rows[line * 2] = top, split.rows[line * 2 + 1] = sum;
+        return;
+    }
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
     if (own.token < 0) return;
 #pragma unroll
@@ -864,84 +952,119 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
         if (c * 16 + 4 * g < a.hd)
             *(Frag *)(out + (size_t)own.token * C + lt.head * a.hd + c * 16 + 4 * g) = M::frag(o[c] * inv);
     // log2 of the row's sum of 2^x; +inf for an empty row, so that its P is 0 in the backward pass
-    if (lse && g == 0)
-        lse[((size_t)lt.window * a.heads + lt.head) * a.n + lt.tile * 64 + q] = top == -INFINITY ? INFINITY : top + log2f(sum);
+    if (lse && g == 0) lse[padded] = top == -INFINITY ? INFINITY : top + log2f(sum);
+}
+
+// Joins the shares of a forward pass: hd / 4 threads for a query, each with four channels
+template <class T>
+__global__ __launch_bounds__(kAttnThreads) void long_fwd_join(const WindowArgs a, const LongMap map, const Split split,
+                                                              T *__restrict__ out, float *__restrict__ lse)
+{
+    const size_t lines = (size_t)a.windows * a.heads * map.tiles * 64;
+    const unsigned per = (unsigned)a.hd / 4;
+    const size_t id = (size_t)blockIdx.x * kAttnThreads + threadIdx.x, line = id / per;
+    const int c = (int)(id % per) * 4;
+    if (line >= lines) return;
+    const size_t r = line / ((size_t)map.tiles * 64);
+    const int head = (int)(r % (size_t)a.heads);
+    const PlaceAt own = map.places[r / (size_t)a.heads * (size_t)map.tiles * 64 + line % ((size_t)map.tiles * 64)];
+    if (own.token < 0) return;
+    float top = -INFINITY;
+    for (int k = 0; k < split.splits; ++k) top = fmaxf(top, split.rows[(k * lines + line) * 2]);
+    const float base2 = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    f32x4 o{};
+    for (int k = 0; k < split.splits; ++k) {
+        const float fade = __builtin_amdgcn_exp2f(split.rows[(k * lines + line) * 2] - base2);
+        sum += split.rows[(k * lines + line) * 2 + 1] * fade;
+        o += *(const f32x4 *)(split.a + (k * lines + line) * a.hd + c) * fade;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+    *(typename Mma<T>::Frag *)(out + (size_t)own.token * a.heads * a.hd + head * a.hd + c) = Mma<T>::frag(o * inv);
+    if (lse && c == 0) lse[line] = top == -INFINITY ? INFINITY : top + log2f(sum);
 }
 
 // dQ, and delta = sum over keys of P dP for each query.  delta is also the product of out and dout; in 16 bits `out` is
 // rounded, so that product c is only near: dS = P (dP - c) serves dQ, which is rounded as coarsely itself, and
 // c + sum P (dP - c), summed here in fp32, is the delta that the table's gradient and dK are computed with.
-template <class T, int HD, bool VEC>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, const LongMap map, const T *__restrict__ qkv,
-                                                           const T *__restrict__ out, const float *__restrict__ lse,
-                                                           const T *__restrict__ dout, T *__restrict__ dqkv,
-                                                           float *__restrict__ delta)
+template <class T, int HD, bool EVEN>
+__global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, const LongMap map, const Split split,
+                                                           const T *__restrict__ qkv, const T *__restrict__ out,
+                                                           const float *__restrict__ lse, const T *__restrict__ dout,
+                                                           T *__restrict__ dqkv, float *__restrict__ delta)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
     __shared__ __align__(16) T Ks[64 * (HD + 4)];
     __shared__ __align__(16) T Kt[HD * 68];
     __shared__ __align__(16) T Vs[64 * (HD + 4)];
     __shared__ __align__(16) PlaceAt at_s[64];
+    __shared__ float bias_s[EVEN ? kSpan : 1];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
-    const float *rev = map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
+    const Meets meet = meets(map, lt.window, lt.tile, a.outside2, split.splits);
+    const int *live = map.live + lt.window * map.tiles * 64;
+    unsigned long long todo = meet.todo, later = todo & (todo - 1);
+    Ahead<T, HD> ahead;
+    auto rows = [&](int t) {
+        ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
+        if (threadIdx.x < 64 && (!EVEN || (meet.mixed >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
+    };
+    if (todo) ahead.tokens(live, __builtin_ctzll(todo));
     const PlaceAt own = window[lt.tile * 64 + q];
-    const int at0 = middle(a) - own.corner, live = own.label < 0 ? -1 : own.token;
+    const int mine = own.label < 0 ? -1 : own.token;
+    Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
+                      window[lt.tile * 64].corner, window);
+    if (todo) {
+        rows(__builtin_ctzll(todo));
+        bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
+        if (later) ahead.tokens(live, __builtin_ctzll(later));
+    }
     Frag qf[CB], gf[CB];
     float near = 0.f;
 #pragma unroll
     for (int c = 0; c < CB; ++c) {
-        qf[c] = load4<T>(base, stride, live, c * 16 + 4 * g, a.hd);
-        gf[c] = load4<T>(dout + (size_t)lt.head * a.hd, C, live, c * 16 + 4 * g, a.hd);
-        const Frag of = load4<T>(out + (size_t)lt.head * a.hd, C, live, c * 16 + 4 * g, a.hd);
+        qf[c] = load4<T>(base, stride, mine, c * 16 + 4 * g, a.hd);
+        gf[c] = load4<T>(dout + (size_t)lt.head * a.hd, C, mine, c * 16 + 4 * g, a.hd);
+        const Frag of = load4<T>(out + (size_t)lt.head * a.hd, C, mine, c * 16 + 4 * g, a.hd);
 #pragma unroll
         for (int r = 0; r < 4; ++r) near += (float)of[r] * (float)gf[c][r];
     }
     near = fold_sum(near);
-    const size_t line = ((size_t)lt.window * a.heads + lt.head) * a.n + lt.tile * 64 + q;
-    const float shift = own.token >= 0 ? lse[line] : INFINITY;
+    const size_t padded = (((size_t)lt.window * a.heads + lt.head) * map.tiles + lt.tile) * 64 + q;
+    const float shift = own.token >= 0 ? lse[padded] : INFINITY;
     const float scale2 = a.scale * kLog2e;
     float rest = 0.f;
     f32x4 dq[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
-    const Meets meet = meets(map, lt.window, lt.tile, a.outside2);
-    unsigned long long todo = meet.any;
-    R kr, vr;
-    PlaceAt at{};
-    int token[R::kPieces];
-    auto fetch = [&](int t) {
-        tokens_of<T, HD>(window + t * 64, token);
-        kr.load(base + C, stride, token, a.hd);
-        vr.load(base + 2 * C, stride, token, a.hd);
-        if (threadIdx.x < 64) at = window[t * 64 + threadIdx.x];
-    };
-    if (todo) fetch(__builtin_ctzll(todo));
     while (todo) {
         const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
-        todo &= todo - 1;
+        todo = later;
+        later &= later - 1;
         __syncthreads();
-        kr.store_rows(Ks);
-        kr.store_columns(Kt);
-        vr.store_rows(Vs);
-        if (threadIdx.x < 64) at_s[threadIdx.x] = at;
-        if (todo) fetch(__builtin_ctzll(todo));
+        ahead.x.store_rows(Ks);
+        ahead.x.store_columns(Kt);
+        ahead.y.store_rows(Vs);
+        if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
+        bias.store(bias_s);
         __syncthreads();
-        f32x4 bias[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bias[j] = four_biases<VEC>(rev, at0, &at_s[j * 16 + 4 * g]);
+        bias.take(bias_s, at_s);
+        if (todo) {
+            rows(__builtin_ctzll(todo));
+            bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
+            if (later) ahead.tokens(live, __builtin_ctzll(later));
+        }
         Frag ds[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
+            const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias.now[j], mixed, own, &at_s[j * 16 + 4 * g],
                                    a.outside2);
             const f32x4 dp = over_channels<T, HD>(Vs, j * 16, gf);
             f32x4 d;
@@ -957,8 +1080,16 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
         over_tokens<T, HD>(dq, Kt, 0, ds);
     }
     rest = fold_sum(rest);
+    if (split.splits > 1) {
+        const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + padded;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+            if (c * 16 + 4 * g < a.hd) *(f32x4 *)(split.a + line * a.hd + c * 16 + 4 * g) = dq[c];
+        if (g == 0) split.rows[line * 2] = blockIdx.y == 0 ? near + rest : rest;
+        return;
+    }
     if (own.token < 0) return;
-    if (g == 0) delta[line] = near + rest;
+    if (g == 0) delta[padded] = near + rest;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
         if (c * 16 + 4 * g < a.hd)
@@ -967,20 +1098,21 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
 
 // dK and dV: wave w has 16 keys and goes through the queries, S = Q K^T (rows: queries, lane: key), so that P and dS have the
 // layout of the B operands of dV^T = dO^T P and dK^T = Q^T dS.
-template <class T, int HD, bool VEC>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, const LongMap map, const T *__restrict__ qkv,
-                                                            const float *__restrict__ lse, const T *__restrict__ dout,
-                                                            T *__restrict__ dqkv, const float *__restrict__ delta)
+template <class T, int HD, bool EVEN>
+__global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, const LongMap map, const Split split,
+                                                            const T *__restrict__ qkv, const float *__restrict__ lse,
+                                                            const T *__restrict__ dout, T *__restrict__ dqkv,
+                                                            const float *__restrict__ delta)
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
     __shared__ __align__(16) T Qs[64 * (HD + 4)];
     __shared__ __align__(16) T Qt[HD * 68];
     __shared__ __align__(16) T Gs[64 * (HD + 4)];
     __shared__ __align__(16) T Gt[HD * 68];
     __shared__ __align__(16) PlaceAt at_s[64];
+    __shared__ float bias_s[EVEN ? kSpan : 1];
     __shared__ __align__(16) float lse_s[64], delta_s[64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, k = wave * 16 + i;
@@ -988,61 +1120,69 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     const int C = a.heads * a.hd;
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd, *gbase = dout + (size_t)lt.head * a.hd;
-    const float *bias_row = map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
-    const PlaceAt own = window[lt.tile * 64 + k];
-    const int at0 = middle(a) - own.corner, live = own.label < 0 ? -1 : own.token;  // entry: corner(q) + middle - corner(k)
-    Frag kf[CB], vf[CB];
-#pragma unroll
-    for (int c = 0; c < CB; ++c) {
-        kf[c] = load4<T>(base + C, stride, live, c * 16 + 4 * g, a.hd);
-        vf[c] = load4<T>(base + 2 * C, stride, live, c * 16 + 4 * g, a.hd);
-    }
-    const float scale2 = a.scale * kLog2e;
-    const size_t lines = ((size_t)lt.window * a.heads + lt.head) * a.n;
-    f32x4 dk[CB], dv[CB];
-#pragma unroll
-    for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
-    const Meets meet = meets(map, lt.window, lt.tile, a.outside2);
-    unsigned long long todo = meet.any;
-    R qr, gr;
-    PlaceAt at{};
+    const size_t lines = ((size_t)lt.window * a.heads + lt.head) * map.tiles * 64;
+    const Meets meet = meets(map, lt.window, lt.tile, a.outside2, split.splits);
+    const int *live = map.live + lt.window * map.tiles * 64;
+    unsigned long long todo = meet.todo, later = todo & (todo - 1);
+    Ahead<T, HD> ahead;
     float shift = 0.f, del = 0.f;
-    int token[R::kPieces];
-    auto fetch = [&](int t) {
-        tokens_of<T, HD>(window + t * 64, token);
-        qr.load(base, stride, token, a.hd);
-        gr.load(gbase, C, token, a.hd);
+    auto rows = [&](int t) {
+        ahead.rows(base, stride, gbase, C, a.hd);
         if (threadIdx.x < 64) {
-            at = window[t * 64 + threadIdx.x];
-            const bool in = at.token >= 0;
+            if (!EVEN || (meet.mixed >> t & 1)) ahead.at = window[t * 64 + threadIdx.x];
+            const bool in = live[t * 64 + threadIdx.x] >= 0;
             shift = in ? lse[lines + t * 64 + threadIdx.x] : INFINITY;
             del = in ? delta[lines + t * 64 + threadIdx.x] : 0.f;
         }
     };
-    if (todo) fetch(__builtin_ctzll(todo));
+    if (todo) ahead.tokens(live, __builtin_ctzll(todo));
+    const PlaceAt own = window[lt.tile * 64 + k];
+    const int mine = own.label < 0 ? -1 : own.token;
+    // entry: corner(q) + middle - corner(k)
+    Biases<EVEN> bias(map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr, a, own.corner,
+                      window[lt.tile * 64].corner, window);
+    if (todo) {
+        rows(__builtin_ctzll(todo));
+        bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
+        if (later) ahead.tokens(live, __builtin_ctzll(later));
+    }
+    Frag kf[CB], vf[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+        kf[c] = load4<T>(base + C, stride, mine, c * 16 + 4 * g, a.hd);
+        vf[c] = load4<T>(base + 2 * C, stride, mine, c * 16 + 4 * g, a.hd);
+    }
+    const float scale2 = a.scale * kLog2e;
+    f32x4 dk[CB], dv[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
     while (todo) {
         const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
-        todo &= todo - 1;
+        todo = later;
+        later &= later - 1;
         __syncthreads();
-        qr.store_rows(Qs);
-        qr.store_columns(Qt);
-        gr.store_rows(Gs);
-        gr.store_columns(Gt);
+        ahead.x.store_rows(Qs);
+        ahead.x.store_columns(Qt);
+        ahead.y.store_rows(Gs);
+        ahead.y.store_columns(Gt);
         if (threadIdx.x < 64) {
-            at_s[threadIdx.x] = at;
+            at_s[threadIdx.x] = ahead.at;
             lse_s[threadIdx.x] = shift;
             delta_s[threadIdx.x] = del;
         }
-        if (todo) fetch(__builtin_ctzll(todo));
+        bias.store(bias_s);
         __syncthreads();
-        f32x4 bias[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bias[j] = four_biases<VEC>(bias_row, at0, &at_s[j * 16 + 4 * g]);
+        bias.take(bias_s, at_s);
+        if (todo) {
+            rows(__builtin_ctzll(todo));
+            bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
+            if (later) ahead.tokens(live, __builtin_ctzll(later));
+        }
         Frag p[4], ds[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const f32x4 x = scores(over_channels<T, HD>(Qs, j * 16, kf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
+            const f32x4 x = scores(over_channels<T, HD>(Qs, j * 16, kf), scale2, bias.now[j], mixed, own, &at_s[j * 16 + 4 * g],
                                    a.outside2);
             const f32x4 dp = over_channels<T, HD>(Gs, j * 16, vf);
             const f32x4 l = *(const f32x4 *)&lse_s[j * 16 + 4 * g], del4 = *(const f32x4 *)&delta_s[j * 16 + 4 * g];
@@ -1058,6 +1198,16 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
         over_tokens<T, HD>(dv, Gt, 0, p);
         over_tokens<T, HD>(dk, Qt, 0, ds);
     }
+    if (split.splits > 1) {
+        const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + lines + lt.tile * 64 + k;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+            if (c * 16 + 4 * g < a.hd) {
+                *(f32x4 *)(split.a + line * a.hd + c * 16 + 4 * g) = dk[c];
+                *(f32x4 *)(split.b + line * a.hd + c * 16 + 4 * g) = dv[c];
+            }
+        return;
+    }
     if (own.token < 0) return;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
@@ -1068,6 +1218,37 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
         }
 }
 
+// Joins the shares of a backward pass: hd / 4 threads for a token, each with four channels.  KV: dK and dV; else dQ and delta.
+template <class T, bool KV>
+__global__ __launch_bounds__(kAttnThreads) void long_bwd_join(const WindowArgs a, const LongMap map, const Split split,
+                                                              T *__restrict__ dqkv, float *__restrict__ delta)
+{
+    const size_t lines = (size_t)a.windows * a.heads * map.tiles * 64;
+    const unsigned per = (unsigned)a.hd / 4;
+    const size_t id = (size_t)blockIdx.x * kAttnThreads + threadIdx.x, line = id / per;
+    const int c = (int)(id % per) * 4;
+    if (line >= lines) return;
+    const size_t r = line / ((size_t)map.tiles * 64);
+    const int head = (int)(r % (size_t)a.heads), C = a.heads * a.hd;
+    const PlaceAt own = map.places[r / (size_t)a.heads * (size_t)map.tiles * 64 + line % ((size_t)map.tiles * 64)];
+    if (own.token < 0) return;
+    f32x4 x{}, y{};
+    float del = 0.f;
+    for (int k = 0; k < split.splits; ++k) {
+        x += *(const f32x4 *)(split.a + (k * lines + line) * a.hd + c);
+        if constexpr (KV)
+            y += *(const f32x4 *)(split.b + (k * lines + line) * a.hd + c);
+        else
+            del += split.rows[(k * lines + line) * 2];
+    }
+    T *to = dqkv + (size_t)own.token * 3 * C + head * a.hd + c;
+    *(typename Mma<T>::Frag *)(to + (KV ? C : 0)) = Mma<T>::frag(x * a.scale);
+    if constexpr (KV)
+        *(typename Mma<T>::Frag *)(to + 2 * C) = Mma<T>::frag(y);
+    else if (c == 0)
+        delta[line] = del;
+}
+
 // The table's gradient sums dS over all pairs of one distance.  Where 64 tokens tile the window evenly (ed x eh x ew tokens,
 // all three dividing the window's), the distances of a pair of tiles depend on the tiles' own distance alone: a
 // workgroup takes one distance of tiles and one head, goes through all such pairs of tiles of its share of the windows, and
@@ -1076,6 +1257,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
 struct PairWork {
     int gd, gh, gw;    // tiles along the axes; 0: not tiled evenly
     int chunks;        // shares of the windows
+    int subs;          // and of a window's pairs: every subs-th is one workgroup's
 };
 
 template <class T, int HD>
@@ -1086,7 +1268,6 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
 {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    using R = Rows<T, HD>;
     constexpr int CB = HD / 16;
     __shared__ __align__(16) T Ks[64 * (HD + 4)];
     __shared__ __align__(16) T Vs[64 * (HD + 4)];
@@ -1094,10 +1275,10 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const bool even = w.gd > 0;
-    // which tiles: query tile (z0 + z, y0 + y, x0 + x) against key tile (kz + z, ...), z < nz and so on
+    // which tiles: query tile qt0 + step against key tile kt0 + step, for nz * ny * nx <= 64 steps
     unsigned id = blockIdx.x;
-    const int chunk = (int)(id % (unsigned)w.chunks);
-    id /= (unsigned)w.chunks;
+    const int share = (int)(id % (unsigned)(w.chunks * w.subs)), chunk = share / w.subs, sub = share % w.subs;
+    id /= (unsigned)(w.chunks * w.subs);
     const int head = (int)(id % (unsigned)a.heads);
     id /= (unsigned)a.heads;
     int qt0, kt0, nz = 1, ny = 1, nx = 1;
@@ -1133,69 +1314,91 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
                 bias[j][r] = row ? row[cq - first[kt0 * 64 + j * 16 + 4 * g + r].corner] : 0.f;
         }
     }
-    const long long w0 = a.windows * chunk / w.chunks, w1 = a.windows * (chunk + 1) / w.chunks;
-    const long long pairs = (w1 - w0) * nz * ny * nx;
-    // one pair of tiles after the other, their rows a pair ahead
+    // lane u's step, and of the window in hand which steps meet, one bit each; the next window's tiles are loaded ahead
+    const int sx = lane % nx, sy = lane / nx % ny, sz = lane / nx / ny;
+    const bool in = lane < nz * ny * nx;
+    const int step = in ? (sz * w.gh + sy) * w.gw + sx : 0;
+    const long long w1 = a.windows * (chunk + 1) / w.chunks;
+    long long window = a.windows * chunk / w.chunks - 1;
+    unsigned long long todo = 0, mask = 0;
+    TileAt tq{kDead, 0, 0, 0}, tk{kDead, 0, 0, 0};
+    auto look = [&](long long at) {
+        if (at >= w1) return;
+        tq = map.tiles_at[at * map.tiles + qt0 + step];
+        tk = map.tiles_at[at * map.tiles + kt0 + step];
+    };
+    look(window + 1);
     struct Pair {
         long long window;
         int qt, kt;
+        bool mixed, some;
     };
-    auto pair_at = [&](long long k) {
-        const unsigned per = (unsigned)(nz * ny * nx);
-        const unsigned u = (unsigned)(k % per);
-        const unsigned x = u % (unsigned)nx, y = u / (unsigned)nx % (unsigned)ny, z = u / (unsigned)nx / (unsigned)ny;
-        const int step = ((int)z * w.gh + (int)y) * w.gw + (int)x;
-        return Pair{w0 + k / per, qt0 + step, kt0 + step};
+    auto advance = [&]() {
+        while (!todo) {
+            if (++window >= w1) return Pair{0, 0, 0, false, false};
+            bool any, mixed;
+            relation(tq, tk, a.outside2, any, mixed);
+            todo = __ballot(any && in);
+            if (w.subs > 1) todo = __ballot(any && in && __popcll(todo & ((1ull << lane) - 1)) % w.subs == sub);
+            mask = __ballot(mixed);
+            look(window + 1);
+        }
+        const int u = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int by = __builtin_amdgcn_readlane(step, u);
+        return Pair{window, qt0 + by, kt0 + by, (bool)(mask >> u & 1), true};
     };
-    R kr, vr;
-    Frag qf[CB], gf[CB], qn[CB], gn[CB];
-    PlaceAt at{}, own{}, own_n{};
-    float shift = 0.f, del = 0.f, shift_n = 0.f, del_n = 0.f;
-    bool mixed = false, mixed_n = false;
-    int token[R::kPieces];
-    auto fetch = [&](const Pair &p) {
-        const PlaceAt *window = map.places + p.window * map.tiles * 64;
-        tokens_of<T, HD>(window + p.kt * 64, token);
-        kr.load(base + C, stride, token, a.hd);
-        vr.load(base + 2 * C, stride, token, a.hd);
-        if (threadIdx.x < 64) at = window[p.kt * 64 + threadIdx.x];
-        own_n = window[p.qt * 64 + q];
-        const int live = own_n.label < 0 ? -1 : own_n.token;
+    Ahead<T, HD> ahead;
+    Frag qn[CB], gn[CB];
+    PlaceAt own_next{};
+    int mine_later = -1;
+    float shift_next = 0.f, del_next = 0.f;
+    auto tokens = [&](const Pair &p) {
+        const int *live = map.live + p.window * map.tiles * 64;
+        ahead.tokens(live, p.kt);
+        mine_later = live[p.qt * 64 + q];
+    };
+    auto rows = [&](const Pair &p) {
+        ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
-            qn[c] = load4<T>(base, stride, live, c * 16 + 4 * g, a.hd);
-            gn[c] = load4<T>(gbase, C, live, c * 16 + 4 * g, a.hd);
+            qn[c] = load4<T>(base, stride, mine_later, c * 16 + 4 * g, a.hd);
+            gn[c] = load4<T>(gbase, C, mine_later, c * 16 + 4 * g, a.hd);
         }
-        const size_t line = ((size_t)p.window * a.heads + head) * a.n + p.qt * 64 + q;
-        shift_n = own_n.token >= 0 ? lse[line] : INFINITY;
-        del_n = own_n.token >= 0 ? delta[line] : 0.f;
-    };
-    // the next pair from k on that has anything to add; pairs when there is none
-    auto next = [&](long long k) {
-        for (; k < pairs; ++k) {
-            const Pair p = pair_at(k);
-            const TileAt *row = map.tiles_at + p.window * map.tiles;
-            const TileAt tq = row[p.qt], tk = row[p.kt];
-            const bool both = tq.state == kEven && tk.state == kEven;
-            const bool same = tq.label == tk.label && tq.wrap == tk.wrap;
-            mixed_n = !(both && same);
-            if (tq.state != kDead && tk.state != kDead && !(both && !same && a.outside2 == -INFINITY)) break;
+        if (p.mixed) {
+            const PlaceAt *window = map.places + p.window * map.tiles * 64;
+            own_next = window[p.qt * 64 + q];
+            if (threadIdx.x < 64) ahead.at = window[p.kt * 64 + threadIdx.x];
         }
-        return k;
+        const size_t line = (((size_t)p.window * a.heads + head) * map.tiles + p.qt) * 64 + q;
+        shift_next = mine_later >= 0 ? lse[line] : INFINITY;
+        del_next = mine_later >= 0 ? delta[line] : 0.f;
     };
-    long long k = next(0);
-    if (k < pairs) fetch(pair_at(k));
-    while (k < pairs) {
+    Pair now = advance(), next{};
+    if (now.some) {
+        tokens(now);
+        rows(now);
+        next = advance();
+        if (next.some) tokens(next);
+    }
+    while (now.some) {
+        const bool mixed = now.mixed;
+        Frag qf[CB], gf[CB];
         __syncthreads();
-        kr.store_rows(Ks);
-        vr.store_rows(Vs);
-        if (threadIdx.x < 64) at_s[threadIdx.x] = at;
+        ahead.x.store_rows(Ks);
+        ahead.y.store_rows(Vs);
+        if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
 #pragma unroll
         for (int c = 0; c < CB; ++c) qf[c] = qn[c], gf[c] = gn[c];
-        own = own_n, shift = shift_n, del = del_n, mixed = mixed_n;
-        k = next(k + 1);
-        if (k < pairs) fetch(pair_at(k));
+        const PlaceAt own = own_next;
+        const float shift = shift_next, del = del_next;
         __syncthreads();
+        now = next;
+        if (now.some) {
+            rows(now);
+            next = advance();
+            if (next.some) tokens(next);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
@@ -1205,9 +1408,9 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
             for (int r = 0; r < 4; ++r) sum[j][r] += __builtin_amdgcn_exp2f(x[r] - shift) * (dp[r] - del);
         }
     }
-    if (even) {  // [chunk][distance of tiles][head][64][64]
-        float *to = dense + (((size_t)chunk * (gridDim.x / (unsigned)(w.chunks * a.heads)) + blockIdx.x / (unsigned)(w.chunks * a.heads)) *
-                                 a.heads + head) * 4096 + q * 64;
+    if (even) {  // [share][distance of tiles][head][64][64]
+        const unsigned each = (unsigned)(w.chunks * w.subs * a.heads);
+        float *to = dense + (((size_t)share * (gridDim.x / each) + blockIdx.x / each) * a.heads + head) * 4096 + q * 64;
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(f32x4 *)&to[j * 16 + 4 * g] = sum[j];
         return;
@@ -1226,6 +1429,8 @@ struct AttnBuffers {
     const void *qkv;
     const float *table;         // as given
     LongMap map;                // long windows
+    bool even;                  // see Biases
+    Split split;
     PairWork work;
     const int *labels;
     const void *out_in;

@@ -31,13 +31,19 @@ void with_nb(int n, F f)
         f(integral_constant<int, 4>{});
 }
 
-unsigned long_grid(const WindowArgs &a) { return (unsigned)(a.windows * a.heads * ((a.n + 63) / 64)); }
-
-// rows of the window that are multiples of 4: four neighbours' bias entries lie behind each other
-template <class F>
-void with_vec(int ww, F f)
+dim3 long_grid(const WindowArgs &a, const AttnBuffers &b)
 {
-    if (ww % 4 == 0)
+    return dim3((unsigned)(a.windows * a.heads * b.map.tiles), b.split.splits);
+}
+unsigned join_grid(const WindowArgs &a, const AttnBuffers &b)
+{
+    return (unsigned)((a.windows * a.heads * b.map.tiles * 64 * (a.hd / 4) + kAttnThreads - 1) / kAttnThreads);
+}
+
+template <class F>
+void with_even(bool even, F f)
+{
+    if (even)
         f(std::true_type{});
     else
         f(std::false_type{});
@@ -56,11 +62,14 @@ void launch_attention_fwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
                                    b.table, b.labels, (T *)b.out);
             });
         else
-            with_vec(a.ww, [&](auto VEC) {
-                hipLaunchKernelGGL((long_fwd<T, HD, VEC>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, b.map,
+            with_even(b.even, [&](auto EVEN) {
+                hipLaunchKernelGGL((long_fwd<T, HD, EVEN>), long_grid(a, b), dim3(kAttnThreads), 0, st, a, b.map, b.split,
                                    (const T *)b.qkv, (T *)b.out, b.lse);
             });
     });
+    if (a.n > 64 && b.split.splits > 1)
+        hipLaunchKernelGGL((long_fwd_join<T>), dim3(join_grid(a, b)), dim3(kAttnThreads), 0, st, a, b.map, b.split, (T *)b.out,
+                           b.lse);
 }
 
 template <>
@@ -75,16 +84,21 @@ void launch_attention_bwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
             });
             return;
         }
-        with_vec(a.ww, [&](auto VEC) {
-            hipLaunchKernelGGL((long_bwd_q<T, HD, VEC>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, b.map,
-                               (const T *)b.qkv, (const T *)b.out_in, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
-            hipLaunchKernelGGL((long_bwd_kv<T, HD, VEC>), dim3(long_grid(a)), dim3(kAttnThreads), 0, st, a, b.map,
-                               (const T *)b.qkv, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
+        const dim3 grid = long_grid(a, b), join(join_grid(a, b)), block(kAttnThreads);
+        with_even(b.even, [&](auto EVEN) {
+            hipLaunchKernelGGL((long_bwd_q<T, HD, EVEN>), grid, block, 0, st, a, b.map, b.split, (const T *)b.qkv,
+                               (const T *)b.out_in, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
+            if (b.split.splits > 1)
+                hipLaunchKernelGGL((long_bwd_join<T, false>), join, block, 0, st, a, b.map, b.split, (T *)b.dqkv, b.delta);
+            hipLaunchKernelGGL((long_bwd_kv<T, HD, EVEN>), grid, block, 0, st, a, b.map, b.split, (const T *)b.qkv, b.lse,
+                               (const T *)b.dout, (T *)b.dqkv, b.delta);
+            if (b.split.splits > 1)
+                hipLaunchKernelGGL((long_bwd_join<T, true>), join, block, 0, st, a, b.map, b.split, (T *)b.dqkv, b.delta);
         });
         if (b.dense) {
             const PairWork &w = b.work;
             const unsigned distances = w.gd ? (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) : b.map.tiles * b.map.tiles;
-            hipLaunchKernelGGL((long_bwd_pairs<T, HD>), dim3(distances * a.heads * w.chunks), dim3(kAttnThreads), 0, st, a, b.map, w,
+            hipLaunchKernelGGL((long_bwd_pairs<T, HD>), dim3(distances * a.heads * w.chunks * w.subs), dim3(kAttnThreads), 0, st, a, b.map, w,
                                (const T *)b.qkv, b.lse, (const T *)b.dout, b.delta, b.dense);
         }
     });
