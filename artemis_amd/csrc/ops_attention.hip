@@ -32,9 +32,8 @@ __global__ __launch_bounds__(256) void places_of(const WindowArgs a, const int *
     }
     places[tile * 64 + lane] = p;
     live[tile * 64 + lane] = p.label < 0 ? -1 : p.token;
-    const int label = __shfl(p.label, 0), wrap = __shfl(p.wrap, 0);
-    const bool even = __all(p.label >= 0 && p.label == label && p.wrap == wrap), dead = __all(p.label < 0);
-    if (lane == 0) tiles_at[tile] = TileAt{dead ? kDead : even ? kEven : kMixed, label, wrap, p.corner};
+    const TileAt what = tile_of(p, __shfl(p.corner, 0));
+    if (lane == 0) tiles_at[tile] = what;
 }
 
 // dense[head][e] = the sum of the shares of the workgroups that have that head, in a fixed order: 16 elements for a
@@ -94,34 +93,36 @@ __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const Pai
     const int e = min(blockIdx.x * 64 + lane, a.entries - 1);
     const int dw = e % a.rh - (a.ww - 1), dh = e / a.rh % (2 * a.wh - 1) - (a.wh - 1), dd = e / a.rd - (a.wd - 1);
     // One axis: tokens i of a query's tile, `size` long, at distance d.  With m = d mod size the key is i - m in the tile
-    // (d - m) / size away for i >= m, and i - m + size in the tile one further for i < m.
+    // (d - m) / size away for i >= m, and i - m + size in the tile one further for i < m: two cases, each with what it adds
+    // to the distance's number (distances are counted as 0, 1, -1, 2, -2, ...) and to the key's place.
     struct Axis {
-        int size, tiles, m, far;
-        __device__ Axis(int d, int tokens, int tiles) : size(tokens / tiles), tiles(tiles)
+        int size, m, far[2], key[2];
+        __device__ Axis(int d, int tokens, int tiles, int distances, int pitch) : size(tokens / tiles)
         {
             m = d % size;
             if (m < 0) m += size;
-            far = (d - m) / size;
-        }
-        // the key, and the distance of tiles counted as 0, 1, -1, 2, -2, ...; -1: beyond the window for every tile
-        __device__ __forceinline__ int key(int i) const { return i < m ? i - m + size : i - m; }
-        __device__ __forceinline__ int distance(int i) const
-        {
-            const int D = i < m ? far + 1 : far;
-            return abs(D) >= tiles ? -1 : D > 0 ? 2 * D - 1 : -2 * D;
+            for (int k = 0; k < 2; ++k) {
+                const int D = (d - m) / size + k;
+                far[k] = abs(D) >= tiles ? -(1 << 24) : (D > 0 ? 2 * D - 1 : -2 * D) * distances;  // beyond the window
+                key[k] = (k * size - m) * pitch;
+            }
         }
     };
-    const Axis x(dw, a.ww, w.gw), y(dh, a.wh, w.gh), z(dd, a.wd, w.gd);
+    const int ew = a.ww / w.gw, eh = a.wh / w.gh;
+    const Axis x(dw, a.ww, w.gw, 1, 1), y(dh, a.wh, w.gh, 2 * w.gw - 1, ew);
+    const Axis z(dd, a.wd, w.gd, (2 * w.gh - 1) * (2 * w.gw - 1), ew * eh);
+    const unsigned stride = (unsigned)a.heads * 4096;
     float s = 0.f;
     for (int share = 0; share < w.chunks * w.subs; ++share) {
         const float *from = dense + ((size_t)share * distances * a.heads + head) * 4096;
 #pragma unroll 8
         for (int q = wave * 16; q < wave * 16 + 16; ++q) {  // (the same q in every lane: its coordinates are scalars)
-            const int ix = q % x.size, iy = q / x.size % y.size, iz = q / x.size / y.size;
-            const int dx = x.distance(ix), dy = y.distance(iy), dz = z.distance(iz);
-            if ((dx | dy | dz) >= 0)
-                s += from[(size_t)((dz * (2 * w.gh - 1) + dy) * (2 * w.gw - 1) + dx) * a.heads * 4096 + q * 64 +
-                          (z.key(iz) * y.size + y.key(iy)) * x.size + x.key(ix)];
+            const int ix = q % ew, iy = q / ew % eh, iz = q / ew / eh;
+            const int bx = ix < x.m, by = iy < y.m, bz = iz < z.m;
+            const int far = (bx ? x.far[1] : x.far[0]) + (by ? y.far[1] : y.far[0]) + (bz ? z.far[1] : z.far[0]);
+            const int key = (bx ? x.key[1] : x.key[0]) + (by ? y.key[1] : y.key[0]) + (bz ? z.key[1] : z.key[0]);
+            // (the key's coordinates are the query's plus these: the query's place in the tile is q itself)
+            if (far >= 0) s += from[(unsigned long long)(unsigned)far * stride + (unsigned)(q * 65 + key)];
         }
     }
     fold[wave][lane] = s;

@@ -694,10 +694,10 @@ struct PlaceAt {
     int token, corner, label, wrap;  // token -1: none (behind the window's end); label < 0: padding
 };
 struct TileAt {
-    int state, label, wrap;  // kMixed; kEven: 64 live tokens of one region; kDead: no live token
-    int corner;              // of the tile's first token
+    int state, label, wrap;  // kEven: live tokens of one region; kPadded: of one region beside padding; kDead: no live
+    int corner;              // token; kMixed: of several regions.  corner: of the tile's first token
 };
-constexpr int kMixed = 0, kEven = 1, kDead = 2;
+constexpr int kMixed = 0, kEven = 1, kPadded = 2, kDead = 3;
 
 struct LongMap {
     const PlaceAt *places;   // (windows, tiles * 64)
@@ -730,36 +730,51 @@ __device__ __forceinline__ LongTile long_tile(const WindowArgs &a, int tiles)
     return {(long long)(r / (unsigned)a.heads), (int)(r % (unsigned)a.heads), (int)t};
 }
 
-// whether two tiles meet at all, and whether they need a mask
+// Whether tokens `x` meet tile `y` at all, and whether they need a mask.  Padding among x needs none: its row is cleared
+// at the end; PADDING_OK: padding among y neither (queries: their lse is infinite, their P 0).
+template <bool PADDING_OK>
 __device__ __forceinline__ void relation(const TileAt &x, const TileAt &y, float outside2, bool &any, bool &mixed)
 {
-    const bool even = x.state == kEven && y.state == kEven;
+    const bool single = x.state != kMixed && y.state != kMixed;
     const bool same = x.label == y.label && x.wrap == y.wrap;
-    any = x.state != kDead && y.state != kDead && !(even && !same && outside2 == -INFINITY);
-    mixed = any && !(even && same);
+    any = x.state != kDead && y.state != kDead && !(single && !same && outside2 == -INFINITY);
+    mixed = any && !(single && same && (PADDING_OK || y.state == kEven));
 }
 
-// Which tiles a tile meets, one bit each (every lane of a wave looks at one tile); of these, every splits-th is this
-// workgroup's.
+// what the lanes of a wave hold: a token each
+__device__ __forceinline__ TileAt tile_of(const PlaceAt &p, int corner)
+{
+    const unsigned long long live = __ballot(p.label >= 0);
+    const int first = live ? __builtin_ctzll(live) : 0;
+    const int label = __shfl(p.label, first), wrap = __shfl(p.wrap, first);
+    const bool one = __all(p.label < 0 || (p.label == label && p.wrap == wrap));
+    return {live == 0 ? kDead : !one ? kMixed : live == ~0ull ? kEven : kPadded, label, wrap, corner};
+}
+
+// Which tiles a wave's 16 tokens meet, one bit each (every lane looks at one tile); the workgroup goes through those that any
+// of its waves meets, or every splits-th of them.
 struct Meets {
-    unsigned long long todo, mixed;
+    unsigned long long todo, any, mixed, masks;  // masks: `mixed` of any wave
     int corner;  // this lane's tile's first token's
 };
-__device__ __forceinline__ Meets meets(const LongMap &m, long long window, int tile, float outside2, int splits)
+template <bool PADDING_OK>
+__device__ __forceinline__ Meets meets(const LongMap &m, long long window, const PlaceAt &own, float outside2, int splits)
 {
-    const TileAt *row = m.tiles_at + window * m.tiles;
-    const TileAt own = row[tile];
+    constexpr int W = kAttnThreads / 64;
+    __shared__ unsigned long long bits[2 * W];
     const int lane = threadIdx.x % 64;
     TileAt other{kDead, 0, 0, 0};
-    if (lane < m.tiles) other = row[lane];
+    if (lane < m.tiles) other = m.tiles_at[window * m.tiles + lane];
     bool any, mixed;
-    relation(own, other, outside2, any, mixed);
-    unsigned long long all = __ballot(any);
-    if (splits > 1) {
-        const int rank = __popcll(all & ((1ull << lane) - 1));
-        all = __ballot(any && rank % splits == (int)blockIdx.y);
-    }
-    return {all, __ballot(mixed), other.corner};
+    relation<PADDING_OK>(tile_of(own, 0), other, outside2, any, mixed);
+    const unsigned long long mine = __ballot(any), masked = __ballot(mixed);
+    if (lane == 0) bits[threadIdx.x / 64] = mine, bits[W + threadIdx.x / 64] = masked;
+    __syncthreads();
+    unsigned long long all = 0, masks = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) all |= bits[k], masks |= bits[W + k];
+    if (splits > 1) all = __ballot((all >> lane & 1) && __popcll(all & ((1ull << lane) - 1)) % splits == (int)blockIdx.y);
+    return {all, mine, masked, masks, other.corner};
 }
 
 // The bias of a tile's pairs.
@@ -865,16 +880,16 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
-    const Meets meet = meets(map, lt.window, lt.tile, a.outside2, split.splits);
+    const PlaceAt own = window[lt.tile * 64 + q];
+    const Meets meet = meets<false>(map, lt.window, own, a.outside2, split.splits);
     const int *live = map.live + lt.window * map.tiles * 64;
     unsigned long long todo = meet.todo, later = todo & (todo - 1);
     Ahead<T, HD> ahead;
     auto rows = [&](int t) {
         ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
-        if (threadIdx.x < 64 && (!EVEN || (meet.mixed >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
+        if (threadIdx.x < 64 && (!EVEN || (meet.masks >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
     };
     if (todo) ahead.tokens(live, __builtin_ctzll(todo));
-    const PlaceAt own = window[lt.tile * 64 + q];
     // entry of the reversed row: middle - corner(q) + corner(k)
     Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
@@ -893,6 +908,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
     for (int c = 0; c < CB; ++c) o[c] = f32x4{};
     while (todo) {
         const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
+        const bool any = meet.any >> __builtin_ctzll(todo) & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();  // the tile before has been used
@@ -901,12 +917,13 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
         if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
         bias.store(bias_s);
         __syncthreads();
-        bias.take(bias_s, at_s);
         if (todo) {
             rows(__builtin_ctzll(todo));
             bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
             if (later) ahead.tokens(live, __builtin_ctzll(later));
         }
+        if (!any) continue;  // (the barriers are at the loop's head)
+        bias.take(bias_s, at_s);
         f32x4 s[4];
         float high = top;
 #pragma unroll
@@ -936,6 +953,11 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
         over_tokens<T, HD>(o, Vt, 0, p);
     }
     sum = fold_sum(sum);
+    if (own.label < 0) {  // padding: an empty row
+        top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) o[c] = f32x4{};
+    }
     const size_t padded = (((size_t)lt.window * a.heads + lt.head) * map.tiles + lt.tile) * 64 + q;
     if (split.splits > 1) {
         const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + padded;
@@ -1008,16 +1030,16 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
     const long long stride = 3LL * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
-    const Meets meet = meets(map, lt.window, lt.tile, a.outside2, split.splits);
+    const PlaceAt own = window[lt.tile * 64 + q];
+    const Meets meet = meets<false>(map, lt.window, own, a.outside2, split.splits);
     const int *live = map.live + lt.window * map.tiles * 64;
     unsigned long long todo = meet.todo, later = todo & (todo - 1);
     Ahead<T, HD> ahead;
     auto rows = [&](int t) {
         ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
-        if (threadIdx.x < 64 && (!EVEN || (meet.mixed >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
+        if (threadIdx.x < 64 && (!EVEN || (meet.masks >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
     };
     if (todo) ahead.tokens(live, __builtin_ctzll(todo));
-    const PlaceAt own = window[lt.tile * 64 + q];
     const int mine = own.label < 0 ? -1 : own.token;
     Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
@@ -1046,6 +1068,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
     for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
     while (todo) {
         const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
+        const bool any = meet.any >> __builtin_ctzll(todo) & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();
@@ -1055,12 +1078,13 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
         if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
         bias.store(bias_s);
         __syncthreads();
-        bias.take(bias_s, at_s);
         if (todo) {
             rows(__builtin_ctzll(todo));
             bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
             if (later) ahead.tokens(live, __builtin_ctzll(later));
         }
+        if (!any) continue;  // (the barriers are at the loop's head)
+        bias.take(bias_s, at_s);
         Frag ds[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1080,6 +1104,11 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
         over_tokens<T, HD>(dq, Kt, 0, ds);
     }
     rest = fold_sum(rest);
+    if (own.label < 0) {
+        near = rest = 0.f;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
+    }
     if (split.splits > 1) {
         const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + padded;
 #pragma unroll
@@ -1122,7 +1151,8 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     const T *base = qkv + (size_t)lt.head * a.hd, *gbase = dout + (size_t)lt.head * a.hd;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
     const size_t lines = ((size_t)lt.window * a.heads + lt.head) * map.tiles * 64;
-    const Meets meet = meets(map, lt.window, lt.tile, a.outside2, split.splits);
+    const PlaceAt own = window[lt.tile * 64 + k];
+    const Meets meet = meets<true>(map, lt.window, own, a.outside2, split.splits);
     const int *live = map.live + lt.window * map.tiles * 64;
     unsigned long long todo = meet.todo, later = todo & (todo - 1);
     Ahead<T, HD> ahead;
@@ -1130,14 +1160,13 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     auto rows = [&](int t) {
         ahead.rows(base, stride, gbase, C, a.hd);
         if (threadIdx.x < 64) {
-            if (!EVEN || (meet.mixed >> t & 1)) ahead.at = window[t * 64 + threadIdx.x];
+            if (!EVEN || (meet.masks >> t & 1)) ahead.at = window[t * 64 + threadIdx.x];
             const bool in = live[t * 64 + threadIdx.x] >= 0;
             shift = in ? lse[lines + t * 64 + threadIdx.x] : INFINITY;
             del = in ? delta[lines + t * 64 + threadIdx.x] : 0.f;
         }
     };
     if (todo) ahead.tokens(live, __builtin_ctzll(todo));
-    const PlaceAt own = window[lt.tile * 64 + k];
     const int mine = own.label < 0 ? -1 : own.token;
     // entry: corner(q) + middle - corner(k)
     Biases<EVEN> bias(map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr, a, own.corner,
@@ -1159,6 +1188,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
     while (todo) {
         const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
+        const bool any = meet.any >> __builtin_ctzll(todo) & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();
@@ -1173,12 +1203,13 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
         }
         bias.store(bias_s);
         __syncthreads();
-        bias.take(bias_s, at_s);
         if (todo) {
             rows(__builtin_ctzll(todo));
             bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
             if (later) ahead.tokens(live, __builtin_ctzll(later));
         }
+        if (!any) continue;  // (the barriers are at the loop's head)
+        bias.take(bias_s, at_s);
         Frag p[4], ds[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1197,6 +1228,10 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
         }
         over_tokens<T, HD>(dv, Gt, 0, p);
         over_tokens<T, HD>(dk, Qt, 0, ds);
+    }
+    if (own.label < 0) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
     }
     if (split.splits > 1) {
         const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + lines + lt.tile * 64 + k;
@@ -1337,7 +1372,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
         while (!todo) {
             if (++window >= w1) return Pair{0, 0, 0, false, false};
             bool any, mixed;
-            relation(tq, tk, a.outside2, any, mixed);
+            relation<false>(tq, tk, a.outside2, any, mixed);
             todo = __ballot(any && in);
             if (w.subs > 1) todo = __ballot(any && in && __popcll(todo & ((1ull << lane) - 1)) % w.subs == sub);
             mask = __ballot(mixed);
