@@ -95,29 +95,28 @@ __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const Pai
     // One axis: tokens i of a query's tile, `size` long, at distance d.  With m = d mod size the key is i - m in the tile
     // (d - m) / size away for i >= m, and i - m + size in the tile one further for i < m: two cases, each with what it adds
     // to the distance's number (distances are counted as 0, 1, -1, 2, -2, ...) and to the key's place.
+    // The sizes are powers of two.
     struct Axis {
-        int size, m, far[2], key[2];
-        __device__ Axis(int d, int tokens, int tiles, int distances, int pitch) : size(tokens / tiles)
+        int m, far[2], key[2];
+        __device__ Axis(int d, int log, int tiles, int distances, int pitch) : m(d & ((1 << log) - 1))
         {
-            m = d % size;
-            if (m < 0) m += size;
             for (int k = 0; k < 2; ++k) {
-                const int D = (d - m) / size + k;
+                const int D = ((d - m) >> log) + k;
                 far[k] = abs(D) >= tiles ? -(1 << 24) : (D > 0 ? 2 * D - 1 : -2 * D) * distances;  // beyond the window
-                key[k] = (k * size - m) * pitch;
+                key[k] = ((k << log) - m) * pitch;
             }
         }
     };
-    const int ew = a.ww / w.gw, eh = a.wh / w.gh;
-    const Axis x(dw, a.ww, w.gw, 1, 1), y(dh, a.wh, w.gh, 2 * w.gw - 1, ew);
-    const Axis z(dd, a.wd, w.gd, (2 * w.gh - 1) * (2 * w.gw - 1), ew * eh);
+    const int lw = __builtin_ctz(a.ww / w.gw), lh = __builtin_ctz(a.wh / w.gh), ld = __builtin_ctz(a.wd / w.gd);
+    const Axis x(dw, lw, w.gw, 1, 1), y(dh, lh, w.gh, 2 * w.gw - 1, 1 << lw);
+    const Axis z(dd, ld, w.gd, (2 * w.gh - 1) * (2 * w.gw - 1), 1 << (lw + lh));
     const unsigned stride = (unsigned)a.heads * 4096;
     float s = 0.f;
-    for (int share = 0; share < w.chunks * w.subs; ++share) {
+    for (int share = 0; share < w.chunks; ++share) {
         const float *from = dense + ((size_t)share * distances * a.heads + head) * 4096;
 #pragma unroll 8
         for (int q = wave * 16; q < wave * 16 + 16; ++q) {  // (the same q in every lane: its coordinates are scalars)
-            const int ix = q % ew, iy = q / ew % eh, iz = q / ew / eh;
+            const int ix = q & ((1 << lw) - 1), iy = q >> lw & ((1 << lh) - 1), iz = q >> (lw + lh);
             const int bx = ix < x.m, by = iy < y.m, bz = iz < z.m;
             const int far = (bx ? x.far[1] : x.far[0]) + (by ? y.far[1] : y.far[0]) + (bz ? z.far[1] : z.far[0]);
             const int key = (bx ? x.key[1] : x.key[0]) + (by ? y.key[1] : y.key[0]) + (bz ? z.key[1] : z.key[0]);
@@ -222,27 +221,21 @@ int make_args(const char *what, const artemis_ops_window *w, WindowArgs &a)
 }
 
 // How the table's gradient goes through a long window's pairs (long_bwd_pairs): 64 tokens in a row of the raster that fill
-// whole rows, or whole planes, evenly; and shares of the windows, then of a window's pairs (at most 64), until there is work
-// for about 2048 workgroups or four pairs are left for each on average.
-#ifndef OPS_PAIR_TARGET
-#define OPS_PAIR_TARGET 2048
-#endif
+// whole rows, or whole planes, evenly; and shares of the windows until there is work for about 1024 workgroups.
 PairWork pair_work(const WindowArgs &a)
 {
-    PairWork w{0, 0, 0, 1, 1};
+    PairWork w{0, 0, 0, 1};
     const int plane = a.wh * a.ww;
     if (a.ww % 64 == 0)
-        w = {a.wd, a.wh, a.ww / 64, 1, 1};
+        w = {a.wd, a.wh, a.ww / 64, 1};
     else if (64 % a.ww == 0 && a.wh % (64 / a.ww) == 0)
-        w = {a.wd, a.wh / (64 / a.ww), 1, 1, 1};
+        w = {a.wd, a.wh / (64 / a.ww), 1, 1};
     else if (64 % plane == 0 && a.wd % (64 / plane) == 0)
-        w = {a.wd / (64 / plane), 1, 1, 1, 1};
+        w = {a.wd / (64 / plane), 1, 1, 1};
     if (w.gd) {
-        const long long distances = (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1), groups = distances * a.heads;
-        const long long tiles = w.gd * w.gh * w.gw, want = OPS_PAIR_TARGET / groups;
+        const long long groups = (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads;
+        const long long want = 1024 / groups;
         w.chunks = (int)(want < 1 ? 1 : want < a.windows ? want : a.windows);
-        const long long more = OPS_PAIR_TARGET / (groups * w.chunks), most = tiles * tiles / distances / 4;
-        w.subs = (int)(more < 1 || most < 1 ? 1 : more < most ? more : most);
     }
     return w;
 }
@@ -292,7 +285,7 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
         if (backward && need_dtable) {
             l.work = pair_work(a);
             const PairWork &w = l.work;
-            l.dense = take(w.gd ? (size_t)w.chunks * w.subs * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
+            l.dense = take(w.gd ? (size_t)w.chunks * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
                                 : (size_t)a.heads * a.n * a.n * 4);
         }
     } else if (backward && need_dtable) {

@@ -13,6 +13,10 @@
 namespace aops {
 
 constexpr int kAttnThreads = 256;
+// Waves of a SIMD that the register budget is for: at two (256 registers) the compiler keeps products in vector registers; at
+// one it puts them into accumulation registers, and every value costs a move.  128 fp32 channels need more than 256.
+template <class T, int HD>
+constexpr int kWaves = HD * sizeof(T) <= 256 ? 2 : 1;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Division of numbers below 2^31 by a constant d: q = (mulhi(x, m) + x) >> s with m = floor(2^32 (2^s - d) / d) + 1,
@@ -150,13 +154,24 @@ __device__ __forceinline__ float fold_sum(float x)
     return x + __shfl_xor(x, 32);
 }
 
-// Loads four channels of a token's row, zeros where there is no token or no channel
+// Four channels of a token's row.  Loaded whether or not there is such a token and channel (from the tensor's first token
+// or the head's first channels then), and cleared where it is used: a load under a condition shares its registers with the
+// zeros, and the compiler waits for all loads in flight before it writes those.  (So guarded, a tile's eight
+// loads went one after the other: 118 us for what takes XX in the kernel of the table's gradient.)
+template <class T>
+__device__ __forceinline__ typename Mma<T>::Frag raw4(const T *__restrict__ base, long long stride, int token, int c, int hd)
+{
+    return *(const typename Mma<T>::Frag *)(base + (long long)(token < 0 ? 0 : token) * stride + (c < hd ? c : 0));
+}
+template <class T>
+__device__ __forceinline__ typename Mma<T>::Frag cleared(typename Mma<T>::Frag f, bool keep)
+{
+    return keep ? f : typename Mma<T>::Frag{};
+}
 template <class T>
 __device__ __forceinline__ typename Mma<T>::Frag load4(const T *__restrict__ base, long long stride, int token, int c, int hd)
 {
-    typename Mma<T>::Frag f{};
-    if (token >= 0 && c < hd) f = *(const typename Mma<T>::Frag *)(base + (long long)token * stride + c);
-    return f;
+    return cleared<T>(raw4<T>(base, stride, token, c, hd), token >= 0 && c < hd);
 }
 
 // 64 rows on their way to LDS: HD / 16 pieces of four channels in each thread
@@ -170,7 +185,21 @@ struct Rows {
     __device__ __forceinline__ void load(const T *__restrict__ base, long long stride, const int (&token)[kPieces], int hd)
     {
 #pragma unroll
-        for (int m = 0; m < kPieces; ++m) f[m] = load4<T>(base, stride, token[m], channel(), hd);
+        for (int m = 0; m < kPieces; ++m) f[m] = raw4<T>(base, stride, token[m], channel(), hd);
+    }
+    // `none`: bit m: there is no such piece.  For whole tiles it is 0 in every thread: one branch.
+    __device__ __forceinline__ void clear(unsigned none)
+    {
+        if (!__any(none != 0)) return;
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) f[m] = cleared<T>(f[m], !(none >> m & 1));
+    }
+    static __device__ __forceinline__ unsigned none_of(const int (&token)[kPieces], int hd)
+    {
+        unsigned none = channel() < hd ? 0u : ~0u;
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) none |= (unsigned)(token[m] < 0) << m;
+        return none;
     }
     __device__ __forceinline__ void store_rows(T *tile) const  // [64][HD + 4]
     {
@@ -379,7 +408,7 @@ __device__ __forceinline__ bool not_finite(const Rows<T, HD> &r)
 }
 
 template <class T, int HD, int NB>
-__global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, const T *__restrict__ qkv,
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(const WindowArgs a, const T *__restrict__ qkv,
                                                            const float *__restrict__ table,
                                                            const int *__restrict__ labels, T *__restrict__ out)
 {
@@ -416,30 +445,34 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
     __syncthreads();
     R kr, vr;
     Frag qn[CB];
+    unsigned none = 0;
     auto fetch = [&](const Spots &at) {
         int token[R::kPieces];
         tokens_at<T, HD>(at, token);
         kr.load(base + C, stride, token, a.hd);
         vr.load(base + 2 * C, stride, token, a.hd);
+        none = R::none_of(token, a.hd);
         const int t = at.label[q] < 0 ? -1 : at.token[q];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) qn[c] = load4<T>(base, stride, t, c * 16 + 4 * g, a.hd);
+        for (int c = 0; c < CB; ++c) qn[c] = raw4<T>(base, stride, t, c * 16 + 4 * g, a.hd);
     };
     fetch(spots[0]);
     int now = 0;  // of three spots: this tile's, the next one's, and the one being looked up
     for (long long tile = walk.tile; tile < tiles; tile += walk.step) {
         const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
         __syncthreads();  // the tile before has been used
+        kr.clear(none);
+        vr.clear(none);
         kr.store_rows(Ks);
         vr.store_columns(Vt);
         if constexpr (NB == 1) {
             if (not_finite(vr)) odd_s[now] = 1;
         }
+        const Spots &at = spots[now];
         Frag qf[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) qf[c] = qn[c];
+        for (int c = 0; c < CB; ++c) qf[c] = cleared<T>(qn[c], at.label[q] >= 0 && c * 16 + 4 * g < a.hd);
         __syncthreads();
-        const Spots &at = spots[now];
         const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
         const bool mixed = at.mixed;
         if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
@@ -456,14 +489,19 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
                 s[j][r] = acc[r] * scale2 + bias[j][r];
                 if (NB == 1 && bias[j][r] == -INFINITY) s[j][r] = -INFINITY;  // (of another window: whatever it is)
             }
-            if (mixed) {
+        }
+        if (mixed) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
                 const int key = (kb0 + j) * 16 + 4 * g;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
             }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) top = fmaxf(top, s[j][r]);
-        }
         top = fold_max(top);
         if (top == -INFINITY) top = 0.f;
         float sum = 0.f;
@@ -497,7 +535,7 @@ __global__ __launch_bounds__(kAttnThreads) void window_fwd(const WindowArgs a, c
 // has the keys of block w: dV^T = dO^T P and dK^T = Q^T dS, contracted over the queries of its unit.  The sum
 // of dS over the workgroup's windows, from which the table's gradient follows, stays in registers.
 template <class T, int HD, int NB>
-__global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, const T *__restrict__ qkv,
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(const WindowArgs a, const T *__restrict__ qkv,
                                                            const float *__restrict__ table,
                                                            const int *__restrict__ labels,
                                                            const T *__restrict__ dout, T *__restrict__ dqkv,
@@ -546,6 +584,7 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
     if (threadIdx.x < 3) odd_s[threadIdx.x] = 0;
     __syncthreads();
     R qr_, kr, vr, gr;
+    unsigned none = 0;
     auto fetch = [&](const Spots &at) {
         int token[R::kPieces];
         tokens_at<T, HD>(at, token);
@@ -553,12 +592,17 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
         kr.load(base + C, stride, token, a.hd);
         vr.load(base + 2 * C, stride, token, a.hd);
         gr.load(gbase, C, token, a.hd);
+        none = R::none_of(token, a.hd);
     };
     if (walk.tile < tiles) fetch(spots[0]);
     int now = 0;
     for (long long tile = walk.tile; tile < tiles; tile += walk.step) {
         const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
         __syncthreads();
+        qr_.clear(none);
+        kr.clear(none);
+        vr.clear(none);
+        gr.clear(none);
         qr_.store_columns(Qt);
         kr.store_rows(Ks);
         if constexpr (!K_BY_ROWS) kr.store_columns(Kt);
@@ -594,14 +638,19 @@ __global__ __launch_bounds__(kAttnThreads) void window_bwd(const WindowArgs a, c
                 s[j][r] = acc[r] * scale2 + bias[j][r];
                 if (NB == 1 && bias[j][r] == -INFINITY) s[j][r] = -INFINITY, dp[j][r] = 0.f;
             }
-            if (mixed) {
+        }
+        if (mixed) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
                 const int key = (kb0 + j) * 16 + 4 * g;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
             }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) top = fmaxf(top, s[j][r]);
-        }
         top = fold_max(top);
         if (top == -INFINITY) top = 0.f;
         float sum = 0.f, delta = 0.f;
@@ -807,8 +856,8 @@ struct Biases {
         if (!EVEN || !row) return;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int e = start + tile_corner + k * kAttnThreads + threadIdx.x;
-            ahead[k] = e >= 0 && e < a.entries ? row[e] : 0.f;
+            // (what lies outside the row is never used)
+            ahead[k] = row[min(max(start + tile_corner + k * kAttnThreads + (int)threadIdx.x, 0), a.entries - 1)];
         }
     }
     __device__ __forceinline__ void store(float *run)
@@ -828,29 +877,43 @@ struct Biases {
     }
 };
 
-// the scores of four pairs in the exponent of 2
-__device__ __forceinline__ f32x4 scores(f32x4 acc, float scale2, f32x4 bias, bool mixed, const PlaceAt &own, const PlaceAt *at,
-                                        float outside2)
+// The scores of a tile in the exponent of 2: all products first (one after the other they would each be waited for), then
+// one branch for the mask.
+template <class T, int HD>
+__device__ __forceinline__ void scores(f32x4 (&x)[4], const T *rows, const typename Mma<T>::Frag *own_row, float scale2,
+                                       const f32x4 (&bias)[4], bool mixed, const PlaceAt &own, const PlaceAt *at, float outside2)
 {
-    f32x4 x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = acc[r] * scale2 + bias[r];
-    if (mixed) {
+    for (int j = 0; j < 4; ++j) {
+        x[j] = over_channels<T, HD>(rows, j * 16, own_row);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = masked(x[r], own.label, own.wrap, at[r].label, at[r].wrap, outside2);
+        for (int r = 0; r < 4; ++r) x[j][r] = x[j][r] * scale2 + bias[j][r];
     }
-    return x;
+    if (mixed) {
+        const int g = threadIdx.x % 64 / 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const PlaceAt &p = at[j * 16 + 4 * g + r];
+                x[j][r] = masked(x[j][r], own.label, own.wrap, p.label, p.wrap, outside2);
+            }
+    }
 }
 
-// What a thread has in flight of the tiles to come: the rows of the next one, the tokens of the one after it.
+// What a thread has in flight of the tiles to come: the rows of the next one, the tokens of the one after it.  Nothing here is
+// loaded under a condition (see raw4).
 template <class T, int HD>
 struct Ahead {
     using R = Rows<T, HD>;
-    R x, y;        // rows of two tensors
-    PlaceAt at;    // of the tile's token threadIdx.x % 64
+    R x, y;         // rows of two tensors
+    unsigned none;  // of their pieces
     int token[R::kPieces];
     __device__ __forceinline__ void tokens(const int *live, int t)
     {
+        // (the tokens before have been turned into addresses and `none`: their registers take the new ones without a copy,
+        // which would have to wait for them)
+        asm volatile("" : "+v"(none)::"memory");
 #pragma unroll
         for (int m = 0; m < R::kPieces; ++m) token[m] = live[t * 64 + R::row(m)];
     }
@@ -858,11 +921,35 @@ struct Ahead {
     {
         x.load(xb, xs, token, hd);
         y.load(yb, ys, token, hd);
+        none = R::none_of(token, hd);
+    }
+    __device__ __forceinline__ void clear()
+    {
+        x.clear(none);
+        y.clear(none);
+    }
+};
+
+// Where the tokens of a tile lie and what they are, into LDS.  EVEN: wanted where there is a mask only, and loaded then.
+template <bool EVEN>
+struct TilePlaces {
+    i32x4 ahead;
+    __device__ __forceinline__ void fetch(const PlaceAt *tile)
+    {
+        if constexpr (!EVEN) ahead = *(const i32x4 *)(tile + threadIdx.x % 64);
+    }
+    __device__ __forceinline__ void store(PlaceAt *to, const PlaceAt *tile, bool wanted)
+    {
+        if constexpr (EVEN) {
+            if (wanted && threadIdx.x < 64) to[threadIdx.x] = tile[threadIdx.x];
+        } else if (threadIdx.x < 64) {
+            *(i32x4 *)(to + threadIdx.x) = ahead;
+        }
     }
 };
 
 template <class T, int HD, bool EVEN>
-__global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, const LongMap map, const Split split,
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const WindowArgs a, const LongMap map, const Split split,
                                                          const T *__restrict__ qkv, T *__restrict__ out,
                                                          float *__restrict__ lse)
 {
@@ -885,18 +972,20 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
     const int *live = map.live + lt.window * map.tiles * 64;
     unsigned long long todo = meet.todo, later = todo & (todo - 1);
     Ahead<T, HD> ahead;
+    TilePlaces<EVEN> at;
     auto rows = [&](int t) {
         ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
-        if (threadIdx.x < 64 && (!EVEN || (meet.masks >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
+        at.fetch(window + t * 64);
     };
-    if (todo) ahead.tokens(live, __builtin_ctzll(todo));
+    ahead.none = 0;
+    ahead.tokens(live, todo ? __builtin_ctzll(todo) : 0);
     // entry of the reversed row: middle - corner(q) + corner(k)
     Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
     if (todo) {
         rows(__builtin_ctzll(todo));
         bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
-        if (later) ahead.tokens(live, __builtin_ctzll(later));
+        ahead.tokens(live, later ? __builtin_ctzll(later) : 0);
     }
     Frag qf[CB];
 #pragma unroll
@@ -907,31 +996,31 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd(const WindowArgs a, con
 #pragma unroll
     for (int c = 0; c < CB; ++c) o[c] = f32x4{};
     while (todo) {
-        const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
-        const bool any = meet.any >> __builtin_ctzll(todo) & 1;
+        const int now = __builtin_ctzll(todo);
+        const bool mixed = meet.mixed >> now & 1, any = meet.any >> now & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();  // the tile before has been used
+        ahead.clear();
         ahead.x.store_rows(Ks);
         ahead.y.store_columns(Vt);
-        if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
+        at.store(at_s, window + now * 64, meet.masks >> now & 1);
         bias.store(bias_s);
         __syncthreads();
         if (todo) {
             rows(__builtin_ctzll(todo));
             bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
-            if (later) ahead.tokens(live, __builtin_ctzll(later));
+            ahead.tokens(live, later ? __builtin_ctzll(later) : 0);
         }
         if (!any) continue;  // (the barriers are at the loop's head)
         bias.take(bias_s, at_s);
         f32x4 s[4];
         float high = top;
+        scores<T, HD>(s, Ks, qf, scale2, bias.now, mixed, own, at_s, a.outside2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s[j] = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias.now[j], mixed, own, &at_s[j * 16 + 4 * g], a.outside2);
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) high = fmaxf(high, s[j][r]);
-        }
         high = fold_max(high);
         const float base2 = high == -INFINITY ? 0.f : high;
         const float fade = __builtin_amdgcn_exp2f(top - base2);
@@ -1010,7 +1099,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd_join(const WindowArgs a
 // rounded, so that product c is only near: dS = P (dP - c) serves dQ, which is rounded as coarsely itself, and
 // c + sum P (dP - c), summed here in fp32, is the delta that the table's gradient and dK are computed with.
 template <class T, int HD, bool EVEN>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, const LongMap map, const Split split,
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(const WindowArgs a, const LongMap map, const Split split,
                                                            const T *__restrict__ qkv, const T *__restrict__ out,
                                                            const float *__restrict__ lse, const T *__restrict__ dout,
                                                            T *__restrict__ dqkv, float *__restrict__ delta)
@@ -1035,18 +1124,20 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
     const int *live = map.live + lt.window * map.tiles * 64;
     unsigned long long todo = meet.todo, later = todo & (todo - 1);
     Ahead<T, HD> ahead;
+    TilePlaces<EVEN> at;
     auto rows = [&](int t) {
         ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
-        if (threadIdx.x < 64 && (!EVEN || (meet.masks >> t & 1))) ahead.at = window[t * 64 + threadIdx.x];
+        at.fetch(window + t * 64);
     };
-    if (todo) ahead.tokens(live, __builtin_ctzll(todo));
+    ahead.none = 0;
+    ahead.tokens(live, todo ? __builtin_ctzll(todo) : 0);
     const int mine = own.label < 0 ? -1 : own.token;
     Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
     if (todo) {
         rows(__builtin_ctzll(todo));
         bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
-        if (later) ahead.tokens(live, __builtin_ctzll(later));
+        ahead.tokens(live, later ? __builtin_ctzll(later) : 0);
     }
     Frag qf[CB], gf[CB];
     float near = 0.f;
@@ -1067,36 +1158,38 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
 #pragma unroll
     for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
     while (todo) {
-        const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
-        const bool any = meet.any >> __builtin_ctzll(todo) & 1;
+        const int now = __builtin_ctzll(todo);
+        const bool mixed = meet.mixed >> now & 1, any = meet.any >> now & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();
+        ahead.clear();
         ahead.x.store_rows(Ks);
         ahead.x.store_columns(Kt);
         ahead.y.store_rows(Vs);
-        if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
+        at.store(at_s, window + now * 64, meet.masks >> now & 1);
         bias.store(bias_s);
         __syncthreads();
         if (todo) {
             rows(__builtin_ctzll(todo));
             bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
-            if (later) ahead.tokens(live, __builtin_ctzll(later));
+            ahead.tokens(live, later ? __builtin_ctzll(later) : 0);
         }
         if (!any) continue;  // (the barriers are at the loop's head)
         bias.take(bias_s, at_s);
         Frag ds[4];
+        f32x4 x[4], dp[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Vs, j * 16, gf);
+        scores<T, HD>(x, Ks, qf, scale2, bias.now, mixed, own, at_s, a.outside2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias.now[j], mixed, own, &at_s[j * 16 + 4 * g],
-                                   a.outside2);
-            const f32x4 dp = over_channels<T, HD>(Vs, j * 16, gf);
             f32x4 d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 // (an empty row: -inf against +inf)
-                const float p = __builtin_amdgcn_exp2f(x[r] - shift);
-                d[r] = p * (dp[r] - near);
+                const float p = __builtin_amdgcn_exp2f(x[j][r] - shift);
+                d[r] = p * (dp[j][r] - near);
                 rest += d[r];
             }
             ds[j] = M::frag(d);
@@ -1128,7 +1221,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_q(const WindowArgs a, c
 // dK and dV: wave w has 16 keys and goes through the queries, S = Q K^T (rows: queries, lane: key), so that P and dS have the
 // layout of the B operands of dV^T = dO^T P and dK^T = Q^T dS.
 template <class T, int HD, bool EVEN>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, const LongMap map, const Split split,
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(const WindowArgs a, const LongMap map, const Split split,
                                                             const T *__restrict__ qkv, const float *__restrict__ lse,
                                                             const T *__restrict__ dout, T *__restrict__ dqkv,
                                                             const float *__restrict__ delta)
@@ -1156,17 +1249,18 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     const int *live = map.live + lt.window * map.tiles * 64;
     unsigned long long todo = meet.todo, later = todo & (todo - 1);
     Ahead<T, HD> ahead;
+    TilePlaces<EVEN> at;
     float shift = 0.f, del = 0.f;
+    int some = -1;  // (lse and delta of no token were never written)
     auto rows = [&](int t) {
         ahead.rows(base, stride, gbase, C, a.hd);
-        if (threadIdx.x < 64) {
-            if (!EVEN || (meet.masks >> t & 1)) ahead.at = window[t * 64 + threadIdx.x];
-            const bool in = live[t * 64 + threadIdx.x] >= 0;
-            shift = in ? lse[lines + t * 64 + threadIdx.x] : INFINITY;
-            del = in ? delta[lines + t * 64 + threadIdx.x] : 0.f;
-        }
+        at.fetch(window + t * 64);
+        some = live[t * 64 + threadIdx.x % 64];
+        shift = lse[lines + t * 64 + threadIdx.x % 64];
+        del = delta[lines + t * 64 + threadIdx.x % 64];
     };
-    if (todo) ahead.tokens(live, __builtin_ctzll(todo));
+    ahead.none = 0;
+    ahead.tokens(live, todo ? __builtin_ctzll(todo) : 0);
     const int mine = own.label < 0 ? -1 : own.token;
     // entry: corner(q) + middle - corner(k)
     Biases<EVEN> bias(map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr, a, own.corner,
@@ -1174,7 +1268,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
     if (todo) {
         rows(__builtin_ctzll(todo));
         bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
-        if (later) ahead.tokens(live, __builtin_ctzll(later));
+        ahead.tokens(live, later ? __builtin_ctzll(later) : 0);
     }
     Frag kf[CB], vf[CB];
 #pragma unroll
@@ -1187,41 +1281,43 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_kv(const WindowArgs a, 
 #pragma unroll
     for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
     while (todo) {
-        const bool mixed = meet.mixed >> __builtin_ctzll(todo) & 1;
-        const bool any = meet.any >> __builtin_ctzll(todo) & 1;
+        const int now = __builtin_ctzll(todo);
+        const bool mixed = meet.mixed >> now & 1, any = meet.any >> now & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();
+        ahead.clear();
         ahead.x.store_rows(Qs);
         ahead.x.store_columns(Qt);
         ahead.y.store_rows(Gs);
         ahead.y.store_columns(Gt);
+        at.store(at_s, window + now * 64, meet.masks >> now & 1);
         if (threadIdx.x < 64) {
-            at_s[threadIdx.x] = ahead.at;
-            lse_s[threadIdx.x] = shift;
-            delta_s[threadIdx.x] = del;
+            lse_s[threadIdx.x] = some >= 0 ? shift : INFINITY;
+            delta_s[threadIdx.x] = some >= 0 ? del : 0.f;
         }
         bias.store(bias_s);
         __syncthreads();
         if (todo) {
             rows(__builtin_ctzll(todo));
             bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
-            if (later) ahead.tokens(live, __builtin_ctzll(later));
+            ahead.tokens(live, later ? __builtin_ctzll(later) : 0);
         }
         if (!any) continue;  // (the barriers are at the loop's head)
         bias.take(bias_s, at_s);
         Frag p[4], ds[4];
+        f32x4 x[4], dp[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Gs, j * 16, vf);
+        scores<T, HD>(x, Qs, kf, scale2, bias.now, mixed, own, at_s, a.outside2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const f32x4 x = scores(over_channels<T, HD>(Qs, j * 16, kf), scale2, bias.now[j], mixed, own, &at_s[j * 16 + 4 * g],
-                                   a.outside2);
-            const f32x4 dp = over_channels<T, HD>(Gs, j * 16, vf);
             const f32x4 l = *(const f32x4 *)&lse_s[j * 16 + 4 * g], del4 = *(const f32x4 *)&delta_s[j * 16 + 4 * g];
             f32x4 pv, d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                pv[r] = __builtin_amdgcn_exp2f(x[r] - l[r]);
-                d[r] = pv[r] * (dp[r] - del4[r]);
+                pv[r] = __builtin_amdgcn_exp2f(x[j][r] - l[r]);
+                d[r] = pv[r] * (dp[j][r] - del4[r]);
             }
             p[j] = M::frag(pv);
             ds[j] = M::frag(d);
@@ -1292,11 +1388,9 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_join(const WindowArgs a
 struct PairWork {
     int gd, gh, gw;    // tiles along the axes; 0: not tiled evenly
     int chunks;        // shares of the windows
-    int subs;          // and of a window's pairs: every subs-th is one workgroup's
 };
-
 template <class T, int HD>
-__global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs a, const LongMap map, const PairWork w,
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_pairs(const WindowArgs a, const LongMap map, const PairWork w,
                                                                const T *__restrict__ qkv, const float *__restrict__ lse,
                                                                const T *__restrict__ dout, const float *__restrict__ delta,
                                                                float *__restrict__ dense)
@@ -1312,8 +1406,8 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
     const bool even = w.gd > 0;
     // which tiles: query tile qt0 + step against key tile kt0 + step, for nz * ny * nx <= 64 steps
     unsigned id = blockIdx.x;
-    const int share = (int)(id % (unsigned)(w.chunks * w.subs)), chunk = share / w.subs, sub = share % w.subs;
-    id /= (unsigned)(w.chunks * w.subs);
+    const int chunk = (int)(id % (unsigned)w.chunks);
+    id /= (unsigned)w.chunks;
     const int head = (int)(id % (unsigned)a.heads);
     id /= (unsigned)a.heads;
     int qt0, kt0, nz = 1, ny = 1, nx = 1;
@@ -1374,7 +1468,6 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
             bool any, mixed;
             relation<false>(tq, tk, a.outside2, any, mixed);
             todo = __ballot(any && in);
-            if (w.subs > 1) todo = __ballot(any && in && __popcll(todo & ((1ull << lane) - 1)) % w.subs == sub);
             mask = __ballot(mixed);
             look(window + 1);
         }
@@ -1384,9 +1477,9 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
         return Pair{window, qt0 + by, kt0 + by, (bool)(mask >> u & 1), true};
     };
     Ahead<T, HD> ahead;
+    ahead.none = 0;
     Frag qn[CB], gn[CB];
-    PlaceAt own_next{};
-    int mine_later = -1;
+    int mine_next = -1, mine_later = -1;
     float shift_next = 0.f, del_next = 0.f;
     auto tokens = [&](const Pair &p) {
         const int *live = map.live + p.window * map.tiles * 64;
@@ -1395,57 +1488,62 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_pairs(const WindowArgs 
     };
     auto rows = [&](const Pair &p) {
         ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
+        mine_next = mine_later;
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
-            qn[c] = load4<T>(base, stride, mine_later, c * 16 + 4 * g, a.hd);
-            gn[c] = load4<T>(gbase, C, mine_later, c * 16 + 4 * g, a.hd);
-        }
-        if (p.mixed) {
-            const PlaceAt *window = map.places + p.window * map.tiles * 64;
-            own_next = window[p.qt * 64 + q];
-            if (threadIdx.x < 64) ahead.at = window[p.kt * 64 + threadIdx.x];
+            qn[c] = raw4<T>(base, stride, mine_next, c * 16 + 4 * g, a.hd);
+            gn[c] = raw4<T>(gbase, C, mine_next, c * 16 + 4 * g, a.hd);
         }
         const size_t line = (((size_t)p.window * a.heads + head) * map.tiles + p.qt) * 64 + q;
-        shift_next = mine_later >= 0 ? lse[line] : INFINITY;
-        del_next = mine_later >= 0 ? delta[line] : 0.f;
+        shift_next = lse[line];
+        del_next = delta[line];
     };
     Pair now = advance(), next{};
     if (now.some) {
         tokens(now);
         rows(now);
         next = advance();
-        if (next.some) tokens(next);
+        tokens(next);
     }
     while (now.some) {
-        const bool mixed = now.mixed;
+        const Pair hand = now;
         Frag qf[CB], gf[CB];
+        PlaceAt own{};
         __syncthreads();
+        ahead.clear();
         ahead.x.store_rows(Ks);
         ahead.y.store_rows(Vs);
-        if (threadIdx.x < 64) at_s[threadIdx.x] = ahead.at;
+        if (hand.mixed) {  // (loaded when wanted)
+            const PlaceAt *window = map.places + hand.window * map.tiles * 64;
+            own = window[hand.qt * 64 + q];
+            if (threadIdx.x < 64) at_s[threadIdx.x] = window[hand.kt * 64 + threadIdx.x];
+        }
 #pragma unroll
-        for (int c = 0; c < CB; ++c) qf[c] = qn[c], gf[c] = gn[c];
-        const PlaceAt own = own_next;
-        const float shift = shift_next, del = del_next;
+        for (int c = 0; c < CB; ++c) {
+            const bool in = mine_next >= 0 && c * 16 + 4 * g < a.hd;
+            qf[c] = cleared<T>(qn[c], in);
+            gf[c] = cleared<T>(gn[c], in);
+        }
+        const float shift = mine_next >= 0 ? shift_next : INFINITY, del = mine_next >= 0 ? del_next : 0.f;
         __syncthreads();
         now = next;
         if (now.some) {
             rows(now);
             next = advance();
-            if (next.some) tokens(next);
+            tokens(next);
         }
+        f32x4 x[4], dp[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const f32x4 x = scores(over_channels<T, HD>(Ks, j * 16, qf), scale2, bias[j], mixed, own, &at_s[j * 16 + 4 * g],
-                                   a.outside2);
-            const f32x4 dp = over_channels<T, HD>(Vs, j * 16, gf);
+        for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Vs, j * 16, gf);
+        scores<T, HD>(x, Ks, qf, scale2, bias, hand.mixed, own, at_s, a.outside2);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum[j][r] += __builtin_amdgcn_exp2f(x[r] - shift) * (dp[r] - del);
-        }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[j][r] += __builtin_amdgcn_exp2f(x[j][r] - shift) * (dp[j][r] - del);
     }
-    if (even) {  // [share][distance of tiles][head][64][64]
-        const unsigned each = (unsigned)(w.chunks * w.subs * a.heads);
-        float *to = dense + (((size_t)share * (gridDim.x / each) + blockIdx.x / each) * a.heads + head) * 4096 + q * 64;
+    if (even) {  // [chunk][distance of tiles][head][64][64]
+        const unsigned each = (unsigned)(w.chunks * a.heads);
+        float *to = dense + (((size_t)chunk * (gridDim.x / each) + blockIdx.x / each) * a.heads + head) * 4096 + q * 64;
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(f32x4 *)&to[j * 16 + 4 * g] = sum[j];
         return;

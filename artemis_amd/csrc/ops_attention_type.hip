@@ -98,7 +98,8 @@ void launch_attention_bwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
         if (b.dense) {
             const PairWork &w = b.work;
             const unsigned distances = w.gd ? (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) : b.map.tiles * b.map.tiles;
-            hipLaunchKernelGGL((long_bwd_pairs<T, HD>), dim3(distances * a.heads * w.chunks * w.subs), dim3(kAttnThreads), 0, st, a, b.map, w,
+            hipLaunchKernelGGL((long_bwd_pairs<T, HD>), dim3(distances * a.heads * w.chunks), dim3(kAttnThreads),
+                               0, st, a, b.map, w,
                                (const T *)b.qkv, b.lse, (const T *)b.dout, b.delta, b.dense);
         }
     });
