@@ -36,25 +36,26 @@ __global__ __launch_bounds__(256) void places_of(const WindowArgs a, const int *
     if (lane == 0) tiles_at[tile] = what;
 }
 
-// dense[head][e] = the sum of the shares of the workgroups that have that head, in a fixed order: 16 elements for a
-// workgroup, 16 threads on each
+// dense[head][e] = the sum of the shares of the workgroups that have that head, in a fixed order: 64 elements for a
+// workgroup, 16 threads on each four of them
 __global__ __launch_bounds__(256) void pairs_fold(const float *__restrict__ pairs, float *__restrict__ dense, int heads,
                                                   int groups, int elements)
 {
-    __shared__ float fold[16][17];
+    __shared__ f32x4 fold[16][16];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int head = blockIdx.y, e = blockIdx.x * 16 + tx;
+    const int head = blockIdx.y, e = blockIdx.x * 64 + tx * 4;
     // workgroup b has head b / 8 % heads (walk_of): the k-th of a head's is ((k / 8) * heads + head) * 8 + k % 8
     const int mine = groups / heads;
-    float s = 0.f;
+    f32x4 s{};
+#pragma unroll 8
     for (int k = ty; k < mine; k += 16)
-        s += pairs[(size_t)(((k / 8) * heads + head) * 8 + k % 8) * elements + e];
+        s += *(const f32x4 *)(pairs + (size_t)(((k / 8) * heads + head) * 8 + k % 8) * elements + e);
     fold[ty][tx] = s;
     __syncthreads();
     if (ty == 0) {
-        float t = 0.f;
+        f32x4 t{};
         for (int k = 0; k < 16; ++k) t += fold[k][tx];
-        dense[(size_t)head * elements + e] = t;
+        *(f32x4 *)(dense + (size_t)head * elements + e) = t;
     }
 }
 
@@ -175,8 +176,11 @@ int small_groups(const WindowArgs &a, int target)
     if (want < 1) want = 1;
     return (int)((want < most ? want : most) * 8 * a.heads);
 }
+// Measured with 8192 windows of 64 tokens in fp32 (2 heads of 32 channels), and 16384 of 4 (4 heads): forward 138 and 71 us for
+// 2048 workgroups, 143 and 68 for 1024, 147 and 66 for 4096; backward with the sum of the table's shares 333 and 103 us for
+// 768, 331 and 106 for 512, 335 and 104 for 1024.
 int fwd_groups(const WindowArgs &a) { return small_groups(a, 2048); }
-int bwd_groups(const WindowArgs &a) { return small_groups(a, 1024); }
+int bwd_groups(const WindowArgs &a) { return small_groups(a, 768); }
 
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
@@ -252,7 +256,7 @@ int split_count(const WindowArgs &a)
 }
 
 struct Layout {
-    size_t bias, rev, places, live, tiles, pairs, dense, delta, split_a, split_b, split_rows, total;
+    size_t bias, rev, places, live, tiles, pairs, dense, delta, split_a, split_b, split_rows, spare, total;
     PairWork work;
     int splits;
 };
@@ -288,10 +292,13 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
             l.dense = take(w.gd ? (size_t)w.chunks * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
                                 : (size_t)a.heads * a.n * a.n * 4);
         }
-    } else if (backward && need_dtable) {
-        const int nb = small_nb(a.n);
-        l.pairs = take((size_t)bwd_groups(a) * 64 * 16 * nb * 4);
-        l.dense = take((size_t)a.heads * 64 * 16 * nb * 4);
+    } else {
+        l.spare = take(kSpareBytes);
+        if (backward && need_dtable) {
+            const int nb = small_nb(a.n);
+            l.pairs = take((size_t)bwd_groups(a) * 64 * 16 * nb * 4);
+            l.dense = take((size_t)a.heads * 64 * 16 * nb * 4);
+        }
     }
     l.total = at;
     return l;
@@ -370,6 +377,7 @@ int artemis_ops_window_attention_forward(const artemis_ops_window *w, const void
     b.out = out;
     b.lse = lse;
     b.groups = a.n <= 64 ? fwd_groups(a) : 0;
+    b.spare = (char *)workspace + l.spare;
     if (a.n > 64) long_buffers(b, a, l, table, labels, (char *)workspace, st);
     if (w->dtype == ARTEMIS_OPS_F32)
         launch_attention_fwd<float>(a, b, st);
@@ -413,6 +421,7 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
     b.dout = dout;
     b.dqkv = dqkv;
     b.groups = is_long ? 0 : bwd_groups(a);
+    b.spare = ws + l.spare;
     if (is_long) b.delta = (float *)(ws + l.delta);
     if (dtable) {
         b.dense = (float *)(ws + l.dense);
@@ -435,7 +444,7 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
                            a, b.dense, dtable);
     } else if (dtable) {
         const int nb = small_nb(a.n), elements = 64 * 16 * nb;
-        hipLaunchKernelGGL(pairs_fold, dim3(elements / 16, a.heads), dim3(256), 0, st, b.pairs, b.dense, a.heads, b.groups,
+        hipLaunchKernelGGL(pairs_fold, dim3(elements / 64, a.heads), dim3(256), 0, st, b.pairs, b.dense, a.heads, b.groups,
                            elements);
         hipLaunchKernelGGL(table_small, dim3((a.entries + 3) / 4, a.heads), dim3(256), 0, st, a, b.dense, dtable, nb);
     }

@@ -157,11 +157,12 @@ __device__ __forceinline__ float fold_sum(float x)
 // Four channels of a token's row.  Loaded whether or not there is such a token and channel (from the tensor's first token
 // or the head's first channels then), and cleared where it is used: a load under a condition shares its registers with the
 // zeros, and the compiler waits for all loads in flight before it writes those.  (So guarded, a tile's eight
-// loads went one after the other: 118 us for what takes XX in the kernel of the table's gradient.)
+// loads went one after the other: 118 us for what takes 89 in the kernel of the table's gradient, at 4096 tokens and 8 heads.)
 template <class T>
-__device__ __forceinline__ typename Mma<T>::Frag raw4(const T *__restrict__ base, long long stride, int token, int c, int hd)
+__device__ __forceinline__ typename Mma<T>::Frag raw4(const T *__restrict__ base, unsigned stride, int token, int c, int hd)
 {
-    return *(const typename Mma<T>::Frag *)(base + (long long)(token < 0 ? 0 : token) * stride + (c < hd ? c : 0));
+    return *(const typename Mma<T>::Frag *)(base + (unsigned long long)(unsigned)(token < 0 ? 0 : token) * stride +
+                                               (c < hd ? c : 0));
 }
 template <class T>
 __device__ __forceinline__ typename Mma<T>::Frag cleared(typename Mma<T>::Frag f, bool keep)
@@ -169,9 +170,17 @@ __device__ __forceinline__ typename Mma<T>::Frag cleared(typename Mma<T>::Frag f
     return keep ? f : typename Mma<T>::Frag{};
 }
 template <class T>
-__device__ __forceinline__ typename Mma<T>::Frag load4(const T *__restrict__ base, long long stride, int token, int c, int hd)
+__device__ __forceinline__ typename Mma<T>::Frag load4(const T *__restrict__ base, unsigned stride, int token, int c, int hd)
 {
     return cleared<T>(raw4<T>(base, stride, token, c, hd), token >= 0 && c < hd);
+}
+
+// Nothing below is loaded before x is there.  Where a register's next value is loaded while this one is still wanted, the
+// compiler loads into another and copies that, which waits for the load: so what becomes of this one is had first.
+template <class X>
+__device__ __forceinline__ void settle(X &x)
+{
+    asm volatile("" : "+v"(x)::"memory");
 }
 
 // 64 rows on their way to LDS: HD / 16 pieces of four channels in each thread
@@ -182,10 +191,15 @@ struct Rows {
     Frag f[kPieces];
     static __device__ __forceinline__ int row(int m) { return threadIdx.x / (HD / 4) + m * kRowStep; }
     static __device__ __forceinline__ int channel() { return threadIdx.x % (HD / 4) * 4; }
-    __device__ __forceinline__ void load(const T *__restrict__ base, long long stride, const int (&token)[kPieces], int hd)
+    __device__ __forceinline__ void load(const T *__restrict__ base, unsigned stride, const int (&token)[kPieces], int hd)
     {
 #pragma unroll
         for (int m = 0; m < kPieces; ++m) f[m] = raw4<T>(base, stride, token[m], channel(), hd);
+    }
+    __device__ __forceinline__ void arrive()
+    {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) settle(f[m]);
     }
     // `none`: bit m: there is no such piece.  For whole tiles it is 0 in every thread: one branch.
     __device__ __forceinline__ void clear(unsigned none)
@@ -270,7 +284,11 @@ __device__ __forceinline__ void over_tokens(f32x4 (&acc)[HD / 16], const T *tile
 // as many as fit 16 slots (NB = 1).  Wave w has the queries of slots 16w .. 16w+15; their keys are the NB
 // blocks of the unit.  A workgroup keeps one head and goes through tiles, so that the bias of its pairs stays in registers
 // (-inf where a pair is of two windows or of empty slots).
-// Bound by memory for the model's sizes (64 tokens, 32 channels: 16 products for each value read).
+// Bound by memory where windows are small or 16 bit, by memory and products together in fp32 at 64 tokens: 8192 windows with 2
+// heads of 32 channels take 138 us forward (537 MB at 3.9 TB/s) and 320 backward (940 MB at 2.9 TB/s; its products alone 136 on
+// the matrix cores); 131072 tokens in windows of 4, 4 heads: 68 us (3.9 TB/s) and 97 (4.8 TB/s); bf16, 8160 shifted windows of 64,
+// 4 heads, forward: 134 us (4.0 TB/s).  Registers for 3 and 4 waves on a SIMD were slower (spills), as was reading the operands
+// of the next products ahead of those at hand (150 us forward).
 // ================================================================================================
 
 // the head and first tile of a workgroup, and its step.  Workgroups 8 apart run on one XCD; the heads of a tile,
@@ -299,24 +317,6 @@ struct Slots {
     static __host__ __device__ int per_tile(int n) { return 4 / NB * (NB == 1 ? 16 / n : 1); }
 };
 
-// bias of (query slot of this lane, four keys of block kb), times log2 e
-template <int NB>
-__device__ __forceinline__ f32x4 pair_bias(const WindowArgs &a, const float *__restrict__ table, int head, int q, int key)
-{
-    f32x4 b;
-    int qw, qt;
-    Slots<NB>::of(a, q, qw, qt);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        int kw, kt;
-        Slots<NB>::of(a, key + r, kw, kt);
-        b[r] = -INFINITY;
-        if (qt >= 0 && kt >= 0 && qw == kw)
-            b[r] = table ? table[(size_t)(corner(a, qt) - corner(a, kt) + middle(a)) * a.heads + head] * kLog2e : 0.f;
-    }
-    return b;
-}
-
 // x = scores in the exponent of 2, masked: -inf for what may not be seen
 __device__ __forceinline__ float masked(float x, int ql, int qr, int kl, int kr, float outside2)
 {
@@ -328,7 +328,9 @@ __device__ __forceinline__ float masked(float x, int ql, int qr, int kl, int kr,
 
 // What the 64 slots of a tile hold.  `mixed`: some are of different regions, or padding.
 struct Spots {
-    int token[64], label[64], wrap[64], mixed;
+    int token[64], label[64], wrap[64];
+    int source[64];  // the token, or -1 for padding too
+    int mixed;
 };
 
 // The slot of this thread (the first wave's), and the spots of one tile after the other
@@ -345,11 +347,18 @@ struct Spotter {
     {
         return t < 0 ? Place{-1, -1, 0} : place_of(a, labels, first + window, td, th, tw);
     }
+    // where the bias table is entered: the slot's corner, and its window or -1
+    __device__ __forceinline__ void write_corners(const WindowArgs &a, Spots &to) const
+    {
+        to.token[threadIdx.x] = td * a.rd + th * a.rh + tw;
+        to.label[threadIdx.x] = t < 0 ? -1 : window;
+    }
     // (only pairs within a window meet, but one comparison serves all windows of the tile)
     __device__ __forceinline__ void write(Spots &to, const Place &p) const
     {
         const int s = threadIdx.x;
         to.token[s] = p.token;
+        to.source[s] = p.label < 0 ? -1 : p.token;
         to.label[s] = p.label;
         to.wrap[s] = p.wrap;
         const int label = __shfl(p.label, 0), wrap = __shfl(p.wrap, 0);
@@ -358,14 +367,42 @@ struct Spotter {
     }
 };
 
+// biases of (query slot q, key slots of NB blocks), times log2 e; -inf where the two are not of one window
+template <int NB>
+__device__ __forceinline__ void pair_biases(f32x4 (&b)[NB], const WindowArgs &a, const Spots &corners,
+                                            const float *__restrict__ table, int head, int q, int key)
+{
+    const int from = corners.token[q] + middle(a), window = corners.label[q];
+    unsigned meet = 0;
+    int entry[NB][4];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool m = window == corners.label[key + j * 16 + r];
+            entry[j][r] = m ? (from - corners.token[key + j * 16 + r]) * a.heads + head : 0;
+            meet |= (unsigned)m << (j * 4 + r);
+        }
+    if (window < 0) meet = 0;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) b[j] = f32x4{};
+    if (table) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) b[j][r] = table[entry[j][r]];
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[j][r] = meet >> (j * 4 + r) & 1 ? b[j][r] * kLog2e : -INFINITY;
+}
+
 template <class T, int HD>
 __device__ __forceinline__ void tokens_at(const Spots &at, int (&token)[Rows<T, HD>::kPieces])
 {
 #pragma unroll
-    for (int m = 0; m < Rows<T, HD>::kPieces; ++m) {
-        const int s = Rows<T, HD>::row(m);
-        token[m] = at.label[s] < 0 ? -1 : at.token[s];
-    }
+    for (int m = 0; m < Rows<T, HD>::kPieces; ++m) token[m] = at.source[Rows<T, HD>::row(m)];
 }
 
 // Windows that share a block of 16 slots meet in its products, where an operand 0 does not undo an infinity or a NaN of
@@ -407,11 +444,21 @@ __device__ __forceinline__ bool not_finite(const Rows<T, HD> &r)
     return x != 0.f;  // 0, or NaN
 }
 
-template <class T, int HD, int NB>
-__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(const WindowArgs a, const T *__restrict__ qkv,
-                                                           const float *__restrict__ table,
-                                                           const int *__restrict__ labels, T *__restrict__ out)
+// Stores are not made under a condition either: a wait for the next tile's loads counts the stores behind them, and where
+// their number is not known it waits for all of them.  What belongs to no token goes to `spare`.
+template <class T>
+__device__ __forceinline__ T *store_at(T *real, T *spare, bool wanted)
 {
+    return wanted ? real : spare + threadIdx.x % 64 * 4;
+}
+constexpr size_t kSpareBytes = 64 * 4 * sizeof(float);
+
+template <class T, int HD, int NB, bool LABELS>
+__global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(const WindowArgs a, const T *__restrict__ qkv,
+                                                           const float *__restrict__ table, const int *__restrict__ label_map,
+                                                           T *__restrict__ out, T *__restrict__ spare)
+{
+    const int *const labels = LABELS ? label_map : nullptr;
     using M = Mma<T>;
     using Frag = typename M::Frag;
     using R = Rows<T, HD>;
@@ -424,7 +471,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
     const int i = lane % 16, g = lane / 16;
     const Walk walk = walk_of(a.heads);
     const int C = a.heads * a.hd;
-    const long long stride = 3LL * C;
+    const unsigned stride = 3u * C;
     const T *base = qkv + (size_t)walk.head * a.hd;
     const int per = Slots<NB>::per_tile(a.n);
     const long long tiles = (a.windows + per - 1) / per;
@@ -432,17 +479,17 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
     const int kb0 = wave / NB * NB;  // the first key block of this wave's unit
     const int q = wave * 16 + i;
     f32x4 bias[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) bias[j] = pair_bias<NB>(a, table, walk.head, q, (kb0 + j) * 16 + 4 * g);
     const float scale2 = a.scale * kLog2e;
     const Spotter<NB> spotter(a);
     const bool first_wave = threadIdx.x < 64;
     if (first_wave) {
         spotter.write(spots[0], spotter.look(a, labels, walk.tile * per));
         spotter.write(spots[1], spotter.look(a, labels, (walk.tile + walk.step) * per));
+        spotter.write_corners(a, spots[2]);  // (tokens are written there in the first tile, behind its barriers)
     }
     if (threadIdx.x < 3) odd_s[threadIdx.x] = 0;
     __syncthreads();
+    pair_biases<NB>(bias, a, spots[2], table, walk.head, q, kb0 * 16 + 4 * g);
     R kr, vr;
     Frag qn[CB];
     unsigned none = 0;
@@ -452,11 +499,14 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
         kr.load(base + C, stride, token, a.hd);
         vr.load(base + 2 * C, stride, token, a.hd);
         none = R::none_of(token, a.hd);
-        const int t = at.label[q] < 0 ? -1 : at.token[q];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) qn[c] = raw4<T>(base, stride, t, c * 16 + 4 * g, a.hd);
+        for (int c = 0; c < CB; ++c) qn[c] = raw4<T>(base, stride, at.source[q], c * 16 + 4 * g, a.hd);
     };
     fetch(spots[0]);
+    kr.arrive();  // (so that within the loop the number of loads and stores behind a load is known)
+    vr.arrive();
+#pragma unroll
+    for (int c = 0; c < CB; ++c) settle(qn[c]);
     int now = 0;  // of three spots: this tile's, the next one's, and the one being looked up
     for (long long tile = walk.tile; tile < tiles; tile += walk.step) {
         const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
@@ -471,14 +521,14 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
         const Spots &at = spots[now];
         Frag qf[CB];
 #pragma unroll
-        for (int c = 0; c < CB; ++c) qf[c] = cleared<T>(qn[c], at.label[q] >= 0 && c * 16 + 4 * g < a.hd);
+        for (int c = 0; c < CB; ++c) qf[c] = cleared<T>(qn[c], at.source[q] >= 0 && c * 16 + 4 * g < a.hd);
         __syncthreads();
         const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
         const bool mixed = at.mixed;
         if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
-        if (tile + walk.step < tiles) fetch(spots[next]);
         Place coming;
         if (first_wave) coming = spotter.look(a, labels, (tile + 2 * walk.step) * per);
+        fetch(spots[next]);  // (behind the last tile: the first token's)
         f32x4 s[NB];
         float top = -INFINITY;
 #pragma unroll
@@ -523,45 +573,53 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
         over_unit<T, HD, NB>(o, Vt, kb0 * 16, p, NB == 1 && odd_s[now], a.n);
 #pragma unroll
         for (int c = 0; c < CB; ++c)
-            if (mine >= 0 && c * 16 + 4 * g < a.hd)
-                *(Frag *)(out + (size_t)mine * C + walk.head * a.hd + c * 16 + 4 * g) = M::frag(o[c]);
+            *(Frag *)store_at(out + (unsigned long long)(unsigned)mine * (unsigned)C + walk.head * a.hd + c * 16 + 4 * g, spare,
+                              mine >= 0 && c * 16 + 4 * g < a.hd) = M::frag(o[c]);
         if (first_wave) spotter.write(spots[after], coming);
         now = next;
     }
+}
+
+// Where (key, query of its unit) lies in an LDS tile of 64 keys: rows of 4 NB quads of queries, without gaps, the quads
+// permuted within a row so that neither the writes (one query of four groups of keys) nor the reads (a quad of 16 keys) meet in
+// a bank.
+template <int NB>
+__device__ __forceinline__ int pair_at(int key, int query)
+{
+    return key * 16 * NB + ((query / 4) ^ (key / (4 / NB) % (4 * NB))) * 4 + query % 4;
 }
 
 // Backward pass of a tile.  Wave w first has the queries of block w: P^T and dP^T as in the forward pass, the row sums
 // delta = sum P dP, dS^T = P^T (dP^T - delta), dQ^T = K^T dS^T.  P and dS go through LDS once; then wave w
 // has the keys of block w: dV^T = dO^T P and dK^T = Q^T dS, contracted over the queries of its unit.  The sum
 // of dS over the workgroup's windows, from which the table's gradient follows, stays in registers.
-template <class T, int HD, int NB>
+template <class T, int HD, int NB, bool LABELS>
 __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(const WindowArgs a, const T *__restrict__ qkv,
-                                                           const float *__restrict__ table,
-                                                           const int *__restrict__ labels,
+                                                           const float *__restrict__ table, const int *__restrict__ label_map,
                                                            const T *__restrict__ dout, T *__restrict__ dqkv,
-                                                           float *__restrict__ pairs)
+                                                           float *__restrict__ pairs, T *__restrict__ spare)
 {
+    const int *const labels = LABELS ? label_map : nullptr;
     using M = Mma<T>;
     using Frag = typename M::Frag;
     using R = Rows<T, HD>;
-    constexpr int PS = 16 * NB + 4;
     constexpr int CB = HD / 16;
-    constexpr int ROWS = 64 * (HD + 4), COLUMNS = HD * 68, PAIRS = 2 * 64 * PS;
-    // K by rows and (128 fp32 channels: no room) by columns, Q and dO by columns; V by rows, then P and dS by keys
+    constexpr int ROWS = 64 * (HD + 4), COLUMNS = HD * 68, PAIRS = 64 * 16 * NB;
+    // K by rows and (128 fp32 channels: no room) by columns, V by rows; then, in their place, P and dS by keys.  Q and dO by
+    // columns.  (32 fp32 channels: 52 KB, three workgroups on a CU.)
     constexpr bool K_BY_ROWS = HD * sizeof(T) > 256;
-    __shared__ __align__(16) T Ks[ROWS];
-    __shared__ __align__(16) T Kt[K_BY_ROWS ? 1 : COLUMNS];
+    constexpr int KV = 2 * ROWS + (K_BY_ROWS ? 0 : COLUMNS);
+    __shared__ __align__(16) T Ks[KV > 2 * PAIRS ? KV : 2 * PAIRS];
     __shared__ __align__(16) T Qt[COLUMNS];
     __shared__ __align__(16) T Gt[COLUMNS];
-    __shared__ __align__(16) T Vs[ROWS > PAIRS ? ROWS : PAIRS];
-    T *const Ps = Vs, *const Ss = Vs + 64 * PS;
+    T *const Vs = Ks + ROWS, *const Kt = Vs + ROWS, *const Ps = Ks, *const Ss = Ks + PAIRS;
     __shared__ Spots spots[3];
     __shared__ int odd_s[3];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16;
     const Walk walk = walk_of(a.heads);
     const int C = a.heads * a.hd;
-    const long long stride = 3LL * C;
+    const unsigned stride = 3u * C;
     const T *base = qkv + (size_t)walk.head * a.hd, *gbase = dout + (size_t)walk.head * a.hd;
     T *dbase = dqkv + (size_t)walk.head * a.hd;
     const int per = Slots<NB>::per_tile(a.n);
@@ -569,20 +627,19 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
     const int kb0 = wave / NB * NB;
     const int q = wave * 16 + i;
     f32x4 bias[NB], dbias[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        bias[j] = pair_bias<NB>(a, table, walk.head, q, (kb0 + j) * 16 + 4 * g);
-        dbias[j] = f32x4{};
-    }
     const float scale2 = a.scale * kLog2e;
     const Spotter<NB> spotter(a);
     const bool first_wave = threadIdx.x < 64;
     if (first_wave) {
         spotter.write(spots[0], spotter.look(a, labels, walk.tile * per));
         spotter.write(spots[1], spotter.look(a, labels, (walk.tile + walk.step) * per));
+        spotter.write_corners(a, spots[2]);
     }
     if (threadIdx.x < 3) odd_s[threadIdx.x] = 0;
     __syncthreads();
+    pair_biases<NB>(bias, a, spots[2], table, walk.head, q, kb0 * 16 + 4 * g);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) dbias[j] = f32x4{};
     R qr_, kr, vr, gr;
     unsigned none = 0;
     auto fetch = [&](const Spots &at) {
@@ -594,7 +651,11 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         gr.load(gbase, C, token, a.hd);
         none = R::none_of(token, a.hd);
     };
-    if (walk.tile < tiles) fetch(spots[0]);
+    fetch(spots[0]);
+    qr_.arrive();
+    kr.arrive();
+    vr.arrive();
+    gr.arrive();
     int now = 0;
     for (long long tile = walk.tile; tile < tiles; tile += walk.step) {
         const int next = now == 2 ? 0 : now + 1, after = next == 2 ? 0 : next + 1;
@@ -616,9 +677,9 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
         const bool mixed = at.mixed, odd = NB == 1 && odd_s[now];
         if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
-        if (tile + walk.step < tiles) fetch(spots[next]);
         Place coming;
         if (first_wave) coming = spotter.look(a, labels, (tile + 2 * walk.step) * per);
+        fetch(spots[next]);  // (behind the last tile: the first token's)
         Frag qf[CB], gf[CB];
 #pragma unroll
         for (int c = 0; c < CB; ++c)
@@ -685,24 +746,25 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         over_unit<T, HD, NB, K_BY_ROWS>(acc, K_BY_ROWS ? Ks : Kt, kb0 * 16, ds, odd, a.n);
 #pragma unroll
         for (int c = 0; c < CB; ++c)
-            if (mine >= 0 && c * 16 + 4 * g < a.hd)
-                *(Frag *)(dbase + (size_t)mine * stride + c * 16 + 4 * g) = M::frag(acc[c] * a.scale);
-        __syncthreads();  // V has been used
+            *(Frag *)store_at(dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g, spare, mine >= 0 && c * 16 + 4 * g < a.hd) =
+                M::frag(acc[c] * a.scale);
+        __syncthreads();  // K and V have been used
         const int ql_ = wave % NB * 16 + i;  // this lane's query within its unit
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int key = (kb0 + j) * 16 + 4 * g + r;
-                Ps[key * PS + ql_] = p[j][r];
-                Ss[key * PS + ql_] = ds[j][r];
+                const int at = pair_at<NB>((kb0 + j) * 16 + 4 * g + r, ql_);
+                Ps[at] = p[j][r];
+                Ss[at] = ds[j][r];
             }
         __syncthreads();
         // now slot q is this lane's key
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            p[j] = row4<T>(&Ps[q * PS + j * 16 + 4 * g]);
-            ds[j] = row4<T>(&Ss[q * PS + j * 16 + 4 * g]);
+            const int at = pair_at<NB>(q, j * 16 + 4 * g);
+            p[j] = row4<T>(&Ps[at]);
+            ds[j] = row4<T>(&Ss[at]);
         }
         f32x4 dv[CB];
 #pragma unroll
@@ -710,12 +772,12 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         over_unit<T, HD, NB>(dv, Gt, kb0 * 16, p, odd, a.n);
         over_unit<T, HD, NB>(acc, Qt, kb0 * 16, ds, odd, a.n);
 #pragma unroll
-        for (int c = 0; c < CB; ++c)
-            if (mine >= 0 && c * 16 + 4 * g < a.hd) {
-                T *to = dbase + (size_t)mine * stride + c * 16 + 4 * g;
-                *(Frag *)(to + C) = M::frag(acc[c] * a.scale);
-                *(Frag *)(to + 2 * C) = M::frag(dv[c]);
-            }
+        for (int c = 0; c < CB; ++c) {
+            T *to = dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g;
+            const bool wanted = mine >= 0 && c * 16 + 4 * g < a.hd;
+            *(Frag *)store_at(to + C, spare, wanted) = M::frag(acc[c] * a.scale);
+            *(Frag *)store_at(to + 2 * C, spare, wanted) = M::frag(dv[c]);
+        }
         if (first_wave) spotter.write(spots[after], coming);
         now = next;
     }
@@ -911,9 +973,7 @@ struct Ahead {
     int token[R::kPieces];
     __device__ __forceinline__ void tokens(const int *live, int t)
     {
-        // (the tokens before have been turned into addresses and `none`: their registers take the new ones without a copy,
-        // which would have to wait for them)
-        asm volatile("" : "+v"(none)::"memory");
+        settle(none);  // (the tokens before have become addresses and `none`)
 #pragma unroll
         for (int m = 0; m < R::kPieces; ++m) token[m] = live[t * 64 + R::row(m)];
     }
@@ -964,7 +1024,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const 
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
-    const long long stride = 3LL * C;
+    const unsigned stride = 3u * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
     const PlaceAt own = window[lt.tile * 64 + q];
@@ -1116,7 +1176,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
-    const long long stride = 3LL * C;
+    const unsigned stride = 3u * C;
     const T *base = qkv + (size_t)lt.head * a.hd;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
     const PlaceAt own = window[lt.tile * 64 + q];
@@ -1240,7 +1300,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
     const int i = lane % 16, g = lane / 16, k = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
     const int C = a.heads * a.hd;
-    const long long stride = 3LL * C;
+    const unsigned stride = 3u * C;
     const T *base = qkv + (size_t)lt.head * a.hd, *gbase = dout + (size_t)lt.head * a.hd;
     const PlaceAt *window = map.places + lt.window * map.tiles * 64;
     const size_t lines = ((size_t)lt.window * a.heads + lt.head) * map.tiles * 64;
@@ -1427,7 +1487,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_pairs(
         qt0 = (int)(id / (unsigned)map.tiles);
     }
     const int C = a.heads * a.hd;
-    const long long stride = 3LL * C;
+    const unsigned stride = 3u * C;
     const T *base = qkv + (size_t)head * a.hd, *gbase = dout + (size_t)head * a.hd;
     const float scale2 = a.scale * kLog2e;
     f32x4 sum[4], bias[4];
@@ -1479,59 +1539,64 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_pairs(
     Ahead<T, HD> ahead;
     ahead.none = 0;
     Frag qn[CB], gn[CB];
-    int mine_next = -1, mine_later = -1;
+    int mine = -1;
+    unsigned no_row = 0;
     float shift_next = 0.f, del_next = 0.f;
     auto tokens = [&](const Pair &p) {
         const int *live = map.live + p.window * map.tiles * 64;
         ahead.tokens(live, p.kt);
-        mine_later = live[p.qt * 64 + q];
+        mine = live[p.qt * 64 + q];
     };
     auto rows = [&](const Pair &p) {
         ahead.rows(base + C, stride, base + 2 * C, stride, a.hd);
-        mine_next = mine_later;
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
-            qn[c] = raw4<T>(base, stride, mine_next, c * 16 + 4 * g, a.hd);
-            gn[c] = raw4<T>(gbase, C, mine_next, c * 16 + 4 * g, a.hd);
+            qn[c] = raw4<T>(base, stride, mine, c * 16 + 4 * g, a.hd);
+            gn[c] = raw4<T>(gbase, C, mine, c * 16 + 4 * g, a.hd);
         }
         const size_t line = (((size_t)p.window * a.heads + head) * map.tiles + p.qt) * 64 + q;
         shift_next = lse[line];
         del_next = delta[line];
+        no_row = mine < 0 ? 1u : 0u;
+        settle(no_row);
     };
+    // (where there are no more pairs, the first window's first tiles are loaded for nothing: see raw4)
     Pair now = advance(), next{};
-    if (now.some) {
-        tokens(now);
-        rows(now);
-        next = advance();
-        tokens(next);
-    }
+    tokens(now);
+    rows(now);
+    next = advance();
+    tokens(next);
     while (now.some) {
         const Pair hand = now;
         Frag qf[CB], gf[CB];
-        PlaceAt own{};
         __syncthreads();
         ahead.clear();
         ahead.x.store_rows(Ks);
         ahead.y.store_rows(Vs);
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+            const bool in = !no_row && c * 16 + 4 * g < a.hd;
+            qf[c] = cleared<T>(qn[c], in);
+            gf[c] = cleared<T>(gn[c], in);
+            settle(qf[c]);
+            settle(gf[c]);
+        }
+        float shift = no_row ? INFINITY : shift_next, del = no_row ? 0.f : del_next;
+        settle(shift);
+        settle(del);
+        PlaceAt own{};
         if (hand.mixed) {  // (loaded when wanted)
             const PlaceAt *window = map.places + hand.window * map.tiles * 64;
             own = window[hand.qt * 64 + q];
             if (threadIdx.x < 64) at_s[threadIdx.x] = window[hand.kt * 64 + threadIdx.x];
+            settle(own.label);
+            settle(own.wrap);
         }
-#pragma unroll
-        for (int c = 0; c < CB; ++c) {
-            const bool in = mine_next >= 0 && c * 16 + 4 * g < a.hd;
-            qf[c] = cleared<T>(qn[c], in);
-            gf[c] = cleared<T>(gn[c], in);
-        }
-        const float shift = mine_next >= 0 ? shift_next : INFINITY, del = mine_next >= 0 ? del_next : 0.f;
         __syncthreads();
         now = next;
-        if (now.some) {
-            rows(now);
-            next = advance();
-            tokens(next);
-        }
+        rows(now);
+        next = advance();
+        tokens(next);
         f32x4 x[4], dp[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Vs, j * 16, gf);
@@ -1572,6 +1637,7 @@ struct AttnBuffers {
     const void *dout;
     void *dqkv;
     float *pairs, *dense, *delta;
+    void *spare;                // kSpareBytes that are written and never read
     int groups;                 // workgroups of window_fwd / window_bwd
 };
 template <class T>

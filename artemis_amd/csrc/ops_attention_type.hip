@@ -41,9 +41,9 @@ unsigned join_grid(const WindowArgs &a, const AttnBuffers &b)
 }
 
 template <class F>
-void with_even(bool even, F f)
+void with_bool(bool is, F f)
 {
-    if (even)
+    if (is)
         f(std::true_type{});
     else
         f(std::false_type{});
@@ -58,11 +58,13 @@ void launch_attention_fwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
     with_hd(a.hd, [&](auto HD) {
         if (a.n <= 64)
             with_nb(a.n, [&](auto NB) {
-                hipLaunchKernelGGL((window_fwd<T, HD, NB>), dim3(b.groups), dim3(kAttnThreads), 0, st, a, (const T *)b.qkv,
-                                   b.table, b.labels, (T *)b.out);
+                with_bool(b.labels != nullptr, [&](auto LABELS) {
+                    hipLaunchKernelGGL((window_fwd<T, HD, NB, LABELS>), dim3(b.groups), dim3(kAttnThreads), 0, st, a,
+                                       (const T *)b.qkv, b.table, b.labels, (T *)b.out, (T *)b.spare);
+                });
             });
         else
-            with_even(b.even, [&](auto EVEN) {
+            with_bool(b.even, [&](auto EVEN) {
                 hipLaunchKernelGGL((long_fwd<T, HD, EVEN>), long_grid(a, b), dim3(kAttnThreads), 0, st, a, b.map, b.split,
                                    (const T *)b.qkv, (T *)b.out, b.lse);
             });
@@ -79,13 +81,16 @@ void launch_attention_bwd<OPS_TYPE>(const WindowArgs &a, const AttnBuffers &b, h
     with_hd(a.hd, [&](auto HD) {
         if (a.n <= 64) {
             with_nb(a.n, [&](auto NB) {
-                hipLaunchKernelGGL((window_bwd<T, HD, NB>), dim3(b.groups), dim3(kAttnThreads), 0, st, a, (const T *)b.qkv,
-                                   b.table, b.labels, (const T *)b.dout, (T *)b.dqkv, b.pairs);
+                with_bool(b.labels != nullptr, [&](auto LABELS) {
+                    hipLaunchKernelGGL((window_bwd<T, HD, NB, LABELS>), dim3(b.groups), dim3(kAttnThreads), 0, st, a,
+                                       (const T *)b.qkv, b.table, b.labels, (const T *)b.dout, (T *)b.dqkv, b.pairs,
+                                       (T *)b.spare);
+                });
             });
             return;
         }
         const dim3 grid = long_grid(a, b), join(join_grid(a, b)), block(kAttnThreads);
-        with_even(b.even, [&](auto EVEN) {
+        with_bool(b.even, [&](auto EVEN) {
             hipLaunchKernelGGL((long_bwd_q<T, HD, EVEN>), grid, block, 0, st, a, b.map, b.split, (const T *)b.qkv,
                                (const T *)b.out_in, b.lse, (const T *)b.dout, (T *)b.dqkv, b.delta);
             if (b.split.splits > 1)
