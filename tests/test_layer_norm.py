@@ -87,6 +87,22 @@ def test_unaligned_views_shapes_and_expanded_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cols", [(torch.float32, 1031), (torch.float16, 2051), (torch.bfloat16, 4099)])
+def test_rows_over_a_workgroup_at_every_alignment(dtype, cols):
+    """More rows than workgroups, each held by all four waves; an odd width in a view that starts off 16 bytes."""
+    rows = 1300
+    x, w, b, dy = data(rows, cols, dtype, 21)
+    flat = torch.empty(x.numel() + 3, dtype=dtype, device=DEV)
+    flat[3:] = x.reshape(-1).to(DEV)
+    view, wd, bd = flat[3:].view(rows, cols).requires_grad_(True), w.to(DEV).requires_grad_(True), b.to(DEV).requires_grad_(True)
+    y = artemis_amd.layer_norm(view, wd, bd)
+    grads = torch.autograd.grad(y, (view, wd, bd), dy.to(DEV))
+    want = ref.layer_norm(x, w, b, 1e-5, dy)
+    for got, name in zip((y, *grads), ("y", "dx", "dw", "db")):
+        ref.assert_within(got, *want[name], name)
+
+
+@pytest.mark.gpu
 def test_parameters_of_16_bits_get_gradients_of_their_type():
     x, w, b, dy = data(50, 64, torch.bfloat16, 11)
     w, b = w.bfloat16(), b.bfloat16()
