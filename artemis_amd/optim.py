@@ -1,5 +1,5 @@
-"""AdamW over many tensors at once, moments in 32 or 8 bits (``include/artemis_ops.h``: a launch takes up to 64
-tensors).  ``adamw_step`` and ``adamw_step_8bit`` are the steps as functions on lists of tensors; ``AdamW``
+"""AdamW over many tensors at once, moments in 32 or 8 bits (``include/artemis_ops.h``: a launch takes up to 90
+tensors, 59 with 8-bit moments).  ``adamw_step`` and ``adamw_step_8bit`` are the steps as functions on lists of tensors; ``AdamW``
 is the optimizer around them (``train.py --optimizer adamw | adamw8``).
 
 The 8-bit moments: 256 consecutive elements share an int32 base; a uint8 code counts from it in steps of
@@ -51,7 +51,7 @@ def moments_from_8bit(codes, bases, signed):
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW whose step is one kernel launch for each 64 tensors.  ``moment_bits`` 32 or 8.  Parameters on HIP
+    """AdamW whose step is one kernel launch for each 90 tensors (8 bit: 59).  ``moment_bits`` 32 or 8.  Parameters on HIP
     devices, contiguous, fp32, bf16 or fp16; dense gradients."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, moment_bits=32, seed=0):

@@ -69,7 +69,7 @@ OPTIMIZERS = ("adamax", "adamw", "adamw8")
 
 def make_optimizer(name, parameters, lr, betas, weight_decay, seed):
     """"adamax": the reference's (main.py:45).  "adamw" / "adamw8": this package's AdamW with moments in 32 / 8
-    bits (2 bytes of state for a parameter instead of 8), one launch for each 64 tensors."""
+    bits (2 bytes of state for a parameter instead of 8), one launch for each 59 tensors (of 32 bits: 90)."""
     if name == "adamax":
         return torch.optim.Adamax(parameters, lr=lr, betas=betas)
     if name not in OPTIMIZERS:
