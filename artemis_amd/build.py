@@ -31,11 +31,10 @@ HIPCC_FLAGS = [
     # bits do not depend on which row slot of a tile computed it
     "-ffp-contract=on",
     "-Wall",
+    # no packed fp32 instructions: some of their forms have given wrong results on these machines now and then
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-
-# The operators of libartemis_ops.so: no packed fp32 instructions (some of their forms have given wrong results
-# on these machines now and then)
-OPS_FLAGS = HIPCC_FLAGS + ["-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+OPS_FLAGS = HIPCC_FLAGS + ["-std=c++17"]
 
 
 def _stale(path, prefix, header) -> bool:
