@@ -1,7 +1,7 @@
 """artemis_amd: the ArTEMIS frame-synthesis hot path (cupy_module/synth.py upstream) as
 hand-written MI355X (gfx950) HIP kernels behind a C ABI, with the reference's
 ``FunctionSynth`` operator interface on top; beside it the encoder's operators (layer norm, windowed attention) and
-the AdamW step, from a second library of the same kind.  See DESIGN.md / INTEGRATION.md."""
+the AdamW step, from a second library of the same kind."""
 from .synth import (FunctionSynth, FunctionSynthFrame, synth, synth_unpadded, synth_strip,  # noqa: F401
                     synth_options, options, offset_radius, suggest_tile_radius, adaptive_state,
                     FunctionChronoHead,
