@@ -278,12 +278,12 @@ void check_list(const char *name, const Tensors &ts, const Tensors &params, at::
     }
 }
 
-// two workgroups would update it at once
-void check_distinct(const char *name, const Tensors &ts)
+// What is written, in one list or in two: two workgroups would update it at once
+void check_distinct(std::unordered_set<const void *> &seen, const char *name, const Tensors &ts)
 {
-    std::unordered_set<const void *> seen;
     for (const at::Tensor &t : ts)
-        TORCH_CHECK_VALUE(t.numel() == 0 || seen.insert(t.const_data_ptr()).second, name, " holds a tensor twice");
+        TORCH_CHECK_VALUE(t.numel() == 0 || seen.insert(t.const_data_ptr()).second, name,
+                          " holds a tensor that was given twice");
 }
 
 void adamw(const Tensors &params, const Tensors &grads, const Tensors &m, const Tensors &v, const Tensors &m_base,
@@ -302,9 +302,14 @@ void adamw(const Tensors &params, const Tensors &grads, const Tensors &m, const 
         check_list("exp_avg_bases", m_base, params, at::kInt, true);
         check_list("exp_avg_sq_bases", v_base, params, at::kInt, true);
     }
-    check_distinct("params", params);
-    check_distinct("exp_avgs", m);
-    check_distinct("exp_avg_sqs", v);
+    std::unordered_set<const void *> seen;
+    check_distinct(seen, "params", params);
+    check_distinct(seen, "exp_avgs", m);
+    check_distinct(seen, "exp_avg_sqs", v);
+    if (bits == 8) {
+        check_distinct(seen, "exp_avg_bases", m_base);
+        check_distinct(seen, "exp_avg_sq_bases", v_base);
+    }
     TORCH_CHECK_VALUE(step >= 1, "step must be a whole number >= 1, got ", step);
     on_gpu(params[0]);
     std::vector<artemis_ops_tensor> list(params.size());

@@ -55,14 +55,22 @@ class AdamW(torch.optim.Optimizer):
     devices, contiguous, fp32, bf16 or fp16; dense gradients."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, moment_bits=32, seed=0):
-        if moment_bits not in (32, 8):
-            raise ValueError(f"moment_bits must be 32 or 8, got {moment_bits}")
-        if not lr >= 0 or not eps >= 0 or not weight_decay >= 0:
-            raise ValueError(f"lr={lr}, eps={eps} and weight_decay={weight_decay} must be >= 0")
-        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
-            raise ValueError(f"betas must lie in [0, 1), got {betas}")
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
-                                      moment_bits=moment_bits, seed=seed))
+        defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, moment_bits=moment_bits, seed=seed)
+        self._check(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check(group):
+        if group["moment_bits"] not in (32, 8):
+            raise ValueError(f"moment_bits must be 32 or 8, got {group['moment_bits']}")
+        if not group["lr"] >= 0 or not group["eps"] >= 0 or not group["weight_decay"] >= 0:
+            raise ValueError(f"lr={group['lr']}, eps={group['eps']} and weight_decay={group['weight_decay']} must be >= 0")
+        if not (0 <= group["betas"][0] < 1 and 0 <= group["betas"][1] < 1):
+            raise ValueError(f"betas must lie in [0, 1), got {group['betas']}")
+
+    def add_param_group(self, param_group):
+        self._check({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _start(self, p, bits):
         state = self.state[p]
@@ -92,8 +100,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW does not take sparse gradients")
                 state = self.state[p] or self._start(p, bits)
-                state["step"] += 1
-                calls.setdefault((p.dtype, p.device, state["step"]), []).append((p, p.grad.contiguous(), state))
+                calls.setdefault((p.dtype, p.device, state["step"] + 1), []).append((p, p.grad.contiguous(), state))
             for (_, _, number), items in calls.items():
                 ps, gs = [i[0] for i in items], [i[1] for i in items]
                 args = dict(lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
@@ -104,6 +111,8 @@ class AdamW(torch.optim.Optimizer):
                     adamw_step_8bit(ps, gs, *[[i[2][n] for i in items] for n in (
                         "exp_avg_codes", "exp_avg_bases", "exp_avg_sq_codes", "exp_avg_sq_bases")], number,
                         seed=group["seed"], **args)
+                for i in items:  # (a refused step is not counted)
+                    i[2]["step"] = number
         return loss
 
     def load_state_dict(self, state_dict):

@@ -322,3 +322,27 @@ def test_refusals():
                dict(moment_bits=16), dict(lr=math.nan)):
         with pytest.raises(ValueError):
             AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
+
+
+def test_a_tensor_for_two_purposes_is_refused():
+    p, g, m, v = ([torch.zeros(300)] for _ in range(4))
+    for lists in ((p, g, p, v), (p, g, m, m), (p, g, m, p)):
+        with pytest.raises(ValueError, match="twice"):
+            artemis_amd.adamw_step(*lists, 1)
+    c, d = ([torch.zeros(300, dtype=torch.uint8)] for _ in range(2))
+    bases = [torch.zeros(2, dtype=torch.int32)]
+    with pytest.raises(ValueError, match="twice"):
+        artemis_amd.adamw_step_8bit(p, g, c, bases, d, bases, 1)
+
+
+def test_a_refused_step_is_not_counted_and_groups_are_checked():
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    optimizer = AdamW([p])
+    with pytest.raises(NotImplementedError):
+        optimizer.step()                                         # (a parameter on the CPU)
+    assert optimizer.state[p]["step"] == 0
+    for kw in (dict(moment_bits=16), dict(lr=-1.0), dict(betas=(1.0, 0.9))):
+        with pytest.raises(ValueError):
+            optimizer.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2))], **kw})
+    assert len(optimizer.param_groups) == 1
