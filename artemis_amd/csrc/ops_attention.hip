@@ -131,6 +131,17 @@ __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const Pai
         dtable[(size_t)e * a.heads + head] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
 }
 
+// The shares of `dense`, into the first, in order
+__global__ __launch_bounds__(256) void shares_fold(float *dense, int shares, long long count)
+{
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i >= count) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < shares; ++k) s += dense[k * count + i];
+    dense[i] = s;
+}
+
 // dtable[e][head] for other long windows, from dense [head][n][n]: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
 // lane has one dw, so that neighbouring lanes read neighbouring keys.  Four waves take every fourth row.
 __global__ __launch_bounds__(256) void table_long(const WindowArgs a, const float *__restrict__ dense,
@@ -236,11 +247,10 @@ PairWork pair_work(const WindowArgs &a)
         w = {a.wd, a.wh / (64 / a.ww), 1, 1};
     else if (64 % plane == 0 && a.wd % (64 / plane) == 0)
         w = {a.wd / (64 / plane), 1, 1, 1};
-    if (w.gd) {
-        const long long groups = (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads;
-        const long long want = 1024 / groups;
-        w.chunks = (int)(want < 1 ? 1 : want < a.windows ? want : a.windows);
-    }
+    const long long tiles = (a.n + 63) / 64;
+    const long long groups = (w.gd ? (2LL * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) : tiles * tiles) * a.heads;
+    const long long want = 1024 / groups;
+    w.chunks = (int)(want < 1 ? 1 : want < a.windows ? want : a.windows);
     return w;
 }
 
@@ -290,7 +300,7 @@ Layout layout_of(const WindowArgs &a, bool backward, bool need_dtable, bool tabl
             l.work = pair_work(a);
             const PairWork &w = l.work;
             l.dense = take(w.gd ? (size_t)w.chunks * (2 * w.gd - 1) * (2 * w.gh - 1) * (2 * w.gw - 1) * a.heads * 4096 * 4
-                                : (size_t)a.heads * a.n * a.n * 4);
+                                : (size_t)w.chunks * a.heads * a.n * a.n * 4);
         }
     } else {
         l.spare = take(kSpareBytes);
@@ -440,6 +450,9 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
         hipLaunchKernelGGL(table_tiled, dim3((a.entries + 63) / 64, a.heads), dim3(256), 0, st, a, b.work, b.dense, dtable,
                            distances);
     } else if (dtable && is_long) {
+        const long long count = (long long)a.heads * a.n * a.n;
+        if (b.work.chunks > 1)
+            hipLaunchKernelGGL(shares_fold, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, b.dense, b.work.chunks, count);
         hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st,
                            a, b.dense, dtable);
     } else if (dtable) {

@@ -1444,7 +1444,8 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_join(const WindowArgs a
 // all three dividing the window's), the distances of a pair of tiles depend on the tiles' own distance alone: a
 // workgroup takes one distance of tiles and one head, goes through all such pairs of tiles of its share of the windows, and
 // adds their dS up in registers, where the bias is kept too.  64 x 64 sums for each distance of tiles are left.
-// Windows that 64 tokens do not tile: a workgroup takes one pair of tiles, and the sums are of n x n pairs.
+// Windows that 64 tokens do not tile: a workgroup takes one pair of tiles in its share of the windows, and the sums are of n x n
+// pairs.
 struct PairWork {
     int gd, gh, gw;    // tiles along the axes; 0: not tiled evenly
     int chunks;        // shares of the windows
@@ -1624,7 +1625,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_pairs(
         return;
     }
     if (qt0 * 64 + q >= a.n) return;
-    float *to = dense + ((size_t)head * a.n + qt0 * 64 + q) * a.n + kt0 * 64;
+    float *to = dense + (((size_t)chunk * a.heads + head) * a.n + qt0 * 64 + q) * a.n + kt0 * 64;  // [chunk][head][n][n]
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll

@@ -164,6 +164,15 @@ def test_more_tiles_than_workgroups():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape,window,heads", [((2, 1, 55, 44), (1, 11, 11), 2), ((3, 6, 21, 10), (3, 7, 5), 1)])
+def test_many_windows_that_64_tokens_do_not_tile(shape, window, heads, dtype):
+    """The table's gradient is summed over shares of the windows."""
+    qkv, table, dout = data(shape, window, heads, 16, dtype, 71)
+    check(qkv, table, window, heads, dout, shift=(0, 3, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_the_longest_window(dtype):
     shape = window = (4, 32, 32)
     qkv, table, dout = data((1, *shape), window, 1, 8, dtype, 19)
