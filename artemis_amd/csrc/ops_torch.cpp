@@ -4,11 +4,11 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <cmath>
 #include <limits>
-#include <unordered_set>
 
 #include "artemis_ops.h"
 
@@ -261,54 +261,97 @@ at::Tensor window_attention(const at::Tensor &qkv, const MaybeTensor &bias_table
 
 // ------------------------------------------------------------------------------------------------- AdamW
 
-using Tensors = std::vector<at::Tensor>;
 constexpr int64_t kGroup = 256;  // elements that share a base
 
-void check_list(const char *name, const Tensors &ts, const Tensors &params, at::ScalarType type, bool groups)
+// A Python list or tuple of tensors, read where it lies: a step over 318 tensors spends 92 us in copies of four
+// such lists and their checks, 28 so.
+class Tensors {
+public:
+    Tensors(const char *name, const pybind11::object &list) : name_(name)
+    {
+        held_ = pybind11::reinterpret_steal<pybind11::object>(PySequence_Fast(list.ptr(), "a list of tensors is wanted"));
+        if (!held_) throw pybind11::error_already_set();
+        items_ = PySequence_Fast_ITEMS(held_.ptr());
+        size_ = (size_t)PySequence_Fast_GET_SIZE(held_.ptr());
+        for (size_t i = 0; i < size_; ++i) TORCH_CHECK_TYPE(THPVariable_Check(items_[i]), name, "[", i, "] is not a tensor");
+    }
+    size_t size() const { return size_; }
+    bool empty() const { return size_ == 0; }
+    const char *name() const { return name_; }
+    const at::Tensor &operator[](size_t i) const { return THPVariable_Unpack(items_[i]); }
+
+private:
+    const char *name_;
+    pybind11::object held_;
+    PyObject **items_;
+    size_t size_;
+};
+
+void check_list(const Tensors &ts, const Tensors &params, at::ScalarType type, bool groups)
 {
-    TORCH_CHECK_VALUE(ts.size() == params.size(), params.size(), " params but ", ts.size(), " ", name);
+    TORCH_CHECK_VALUE(ts.size() == params.size(), params.size(), " ", params.name(), " but ", ts.size(), " ", ts.name());
+    const at::Device device = params[0].device();
     for (size_t i = 0; i < ts.size(); ++i) {
         const at::Tensor &t = ts[i];
-        TORCH_CHECK_TYPE(t.scalar_type() == type, name, "[", i, "] must be ", type, ", got ", t.scalar_type());
-        const int64_t want = groups ? (params[i].numel() + kGroup - 1) / kGroup : params[i].numel();
-        TORCH_CHECK_VALUE(t.numel() == want, name, "[", i, "] has ", t.numel(), " elements, ", want, " are wanted");
-        TORCH_CHECK_VALUE(t.device() == params[0].device(), name, "[", i, "] is on ", t.device(), ", params[0] on ",
-                          params[0].device());
-        assert_contiguous(t, name);
+        TORCH_CHECK_TYPE(t.scalar_type() == type, ts.name(), "[", i, "] must be ", type, ", got ", t.scalar_type());
+        const int64_t count = params[i].numel(), want = groups ? (count + kGroup - 1) / kGroup : count;
+        TORCH_CHECK_VALUE(t.numel() == want, ts.name(), "[", i, "] has ", t.numel(), " elements, ", want, " are wanted");
+        TORCH_CHECK_VALUE(t.device() == device, ts.name(), "[", i, "] is on ", t.device(), ", ", params.name(), "[0] on ", device);
+        assert_contiguous(t, ts.name());
     }
 }
 
 // What is written, in one list or in two: two workgroups would update it at once
-void check_distinct(std::unordered_set<const void *> &seen, const char *name, const Tensors &ts)
-{
-    for (const at::Tensor &t : ts)
-        TORCH_CHECK_VALUE(t.numel() == 0 || seen.insert(t.const_data_ptr()).second, name,
-                          " holds a tensor that was given twice");
-}
+class Distinct {
+public:
+    explicit Distinct(size_t most)
+    {
+        size_t n = 16;
+        while (n < 2 * most) n *= 2;
+        seen_.resize(n);
+    }
+    void add(const Tensors &ts)
+    {
+        const size_t mask = seen_.size() - 1;
+        for (size_t i = 0; i < ts.size(); ++i) {
+            if (ts[i].numel() == 0) continue;
+            const void *p = ts[i].const_data_ptr();
+            size_t at = ((size_t)p * 0x9E3779B97F4A7C15ull >> 32) & mask;
+            for (; seen_[at]; at = (at + 1) & mask)
+                TORCH_CHECK_VALUE(seen_[at] != p, ts.name(), " holds a tensor that was given twice");
+            seen_[at] = p;
+        }
+    }
 
-void adamw(const Tensors &params, const Tensors &grads, const Tensors &m, const Tensors &v, const Tensors &m_base,
-           const Tensors &v_base, int bits, int64_t step, double lr, double beta1, double beta2, double eps,
-           double weight_decay, int64_t seed)
+private:
+    std::vector<const void *> seen_;  // at most half full
+};
+
+void adamw(const pybind11::object &param_list, const pybind11::object &grad_list, const pybind11::object &m_list,
+           const pybind11::object &v_list, const pybind11::object &m_base_list, const pybind11::object &v_base_list, int bits,
+           int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed)
 {
+    const Tensors params("params", param_list), grads("grads", grad_list), m("exp_avgs", m_list), v("exp_avg_sqs", v_list);
+    const Tensors m_base("exp_avg_bases", m_base_list), v_base("exp_avg_sq_bases", v_base_list);
     if (params.empty() && grads.empty()) return;
     TORCH_CHECK_VALUE(!params.empty(), "no params but ", grads.size(), " grads");
     const int type = type_code(params[0], "params");
     const at::ScalarType kind = bits == 32 ? at::kFloat : at::kByte;
-    check_list("params", params, params, params[0].scalar_type(), false);
-    check_list("grads", grads, params, params[0].scalar_type(), false);
-    check_list("exp_avgs", m, params, kind, false);
-    check_list("exp_avg_sqs", v, params, kind, false);
+    check_list(params, params, params[0].scalar_type(), false);
+    check_list(grads, params, params[0].scalar_type(), false);
+    check_list(m, params, kind, false);
+    check_list(v, params, kind, false);
     if (bits == 8) {
-        check_list("exp_avg_bases", m_base, params, at::kInt, true);
-        check_list("exp_avg_sq_bases", v_base, params, at::kInt, true);
+        check_list(m_base, params, at::kInt, true);
+        check_list(v_base, params, at::kInt, true);
     }
-    std::unordered_set<const void *> seen;
-    check_distinct(seen, "params", params);
-    check_distinct(seen, "exp_avgs", m);
-    check_distinct(seen, "exp_avg_sqs", v);
+    Distinct distinct(5 * params.size());
+    distinct.add(params);
+    distinct.add(m);
+    distinct.add(v);
     if (bits == 8) {
-        check_distinct(seen, "exp_avg_bases", m_base);
-        check_distinct(seen, "exp_avg_sq_bases", v_base);
+        distinct.add(m_base);
+        distinct.add(v_base);
     }
     TORCH_CHECK_VALUE(step >= 1, "step must be a whole number >= 1, got ", step);
     on_gpu(params[0]);
@@ -322,19 +365,20 @@ void adamw(const Tensors &params, const Tensors &grads, const Tensors &m, const 
                          stream_of(params[0])),
        "artemis_ops_adamw");
     // what autograd saved of them is out of date
-    for (const at::Tensor &p : params)
-        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    for (size_t i = 0; i < params.size(); ++i)
+        if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
 }
 
-Tensors moments_from_8bit(const Tensors &codes, const Tensors &bases, bool is_signed)
+std::vector<at::Tensor> moments_from_8bit(const pybind11::object &code_list, const pybind11::object &base_list, bool is_signed)
 {
+    const Tensors codes("codes", code_list), bases("bases", base_list);
     if (codes.empty() && bases.empty()) return {};
     TORCH_CHECK_VALUE(!codes.empty(), "no codes but ", bases.size(), " bases");
-    check_list("codes", codes, codes, at::kByte, false);
-    check_list("bases", bases, codes, at::kInt, true);
+    check_list(codes, codes, at::kByte, false);
+    check_list(bases, codes, at::kInt, true);
     on_gpu(codes[0]);
     const c10::DeviceGuard guard(codes[0].device());
-    Tensors values;
+    std::vector<at::Tensor> values;
     std::vector<artemis_ops_tensor> list;
     for (size_t i = 0; i < codes.size(); ++i) {
         values.push_back(at::empty(codes[i].sizes(), codes[i].options().dtype(at::kFloat)));
