@@ -892,17 +892,24 @@ __device__ __forceinline__ Meets meets(const LongMap &m, long long window, const
 // EVEN (64 tokens tile the window, its rows are multiples of 4, and two tiles' distances span at most kSpan entries): the
 // entries of a pair of tiles are one run of the row, which the workgroup copies to LDS, a tile ahead; a lane's four lie
 // behind each other there.  (Loading them from the row itself is 16 bytes a lane at any alignment, and was a third of all
-// the work of the address units.)  Else: each by itself.
+// the work of the address units.)
+// Else: each by itself, from a copy of the head's whole row in LDS where it has at most TABLE entries.  (From the row itself
+// a tile's sixteen loads wait for the next tile's rows, which were asked for before: 7872 tiles of windows of 72 tokens, 64 channels
+// in fp16, take 99 us forward, 89 with the copy.  With 128 channels the registers for both forms leave one wave less on a SIMD:
+// 189 us instead of 160.)
 constexpr int kSpan = 512;
-template <bool EVEN>
+template <int HD>
+constexpr int kTable = HD <= 64 ? 2048 : 0;
+template <bool EVEN, int TABLE>
 struct Biases {
     f32x4 now[4];
     float ahead[2];
     int at[4], start;
     const float *row;  // this head's entries
+    bool copied;       // into LDS, all of them
     // `sign`: an entry's place grows with +-corner(own); `own`, `partner`: corners of this lane's token and of the first tile's
     __device__ __forceinline__ Biases(const float *head_row, const WindowArgs &a, int own, int own_tile, const PlaceAt *first_tile)
-        : row(head_row)
+        : row(head_row), copied(!EVEN && TABLE > 0 && a.entries <= TABLE)
     {
         const int g = threadIdx.x % 64 / 16;
         const int reach = EVEN ? first_tile[63].corner : 0;  // between the first and the last token of a tile
@@ -912,6 +919,13 @@ struct Biases {
             now[j] = f32x4{};
             at[j] = EVEN ? reach - (own - own_tile) + first_tile[j * 16 + 4 * g].corner : middle(a) - own;
         }
+    }
+    // (there is a barrier between this and take())
+    __device__ __forceinline__ void copy(const WindowArgs &a, float *to) const
+    {
+        if (TABLE == 0 || !row || !copied) return;
+#pragma unroll 2
+        for (int e = threadIdx.x; e < a.entries; e += kAttnThreads) to[e] = row[e];
     }
     __device__ __forceinline__ void fetch(const WindowArgs &a, int tile_corner)
     {
@@ -932,10 +946,17 @@ struct Biases {
     {
         if (!row) return;
         const int g = threadIdx.x % 64 / 16;
+        if (EVEN || (TABLE > 0 && copied)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) now[j][r] = run[at[j] + (EVEN ? r : tile[j * 16 + 4 * g + r].corner)];
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) now[j][r] = EVEN ? run[at[j] + r] : row[at[j] + tile[j * 16 + 4 * g + r].corner];
+            for (int r = 0; r < 4; ++r) now[j][r] = row[at[j] + tile[j * 16 + 4 * g + r].corner];
     }
 };
 
@@ -1019,7 +1040,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const 
     __shared__ __align__(16) T Ks[64 * (HD + 4)];
     __shared__ __align__(16) T Vt[HD * 68];
     __shared__ __align__(16) PlaceAt at_s[64];
-    __shared__ float bias_s[EVEN ? kSpan : 1];
+    __shared__ float bias_s[EVEN ? kSpan : kTable<HD> + 1];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
@@ -1040,8 +1061,9 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const 
     ahead.none = 0;
     ahead.tokens(live, todo ? __builtin_ctzll(todo) : 0);
     // entry of the reversed row: middle - corner(q) + corner(k)
-    Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
+    Biases<EVEN, kTable<HD>> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
+    bias.copy(a, bias_s);
     if (todo) {
         rows(__builtin_ctzll(todo));
         bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
@@ -1171,7 +1193,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
     __shared__ __align__(16) T Kt[HD * 68];
     __shared__ __align__(16) T Vs[64 * (HD + 4)];
     __shared__ __align__(16) PlaceAt at_s[64];
-    __shared__ float bias_s[EVEN ? kSpan : 1];
+    __shared__ float bias_s[EVEN ? kSpan : kTable<HD> + 1];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, q = wave * 16 + i;
     const LongTile lt = long_tile(a, map.tiles);
@@ -1192,8 +1214,9 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
     ahead.none = 0;
     ahead.tokens(live, todo ? __builtin_ctzll(todo) : 0);
     const int mine = own.label < 0 ? -1 : own.token;
-    Biases<EVEN> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
+    Biases<EVEN, kTable<HD>> bias(map.rev ? map.rev + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
+    bias.copy(a, bias_s);
     if (todo) {
         rows(__builtin_ctzll(todo));
         bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
@@ -1294,7 +1317,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
     __shared__ __align__(16) T Gs[64 * (HD + 4)];
     __shared__ __align__(16) T Gt[HD * 68];
     __shared__ __align__(16) PlaceAt at_s[64];
-    __shared__ float bias_s[EVEN ? kSpan : 1];
+    __shared__ float bias_s[EVEN ? kSpan : kTable<HD> + 1];
     __shared__ __align__(16) float lse_s[64], delta_s[64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16, k = wave * 16 + i;
@@ -1323,8 +1346,9 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
     ahead.tokens(live, todo ? __builtin_ctzll(todo) : 0);
     const int mine = own.label < 0 ? -1 : own.token;
     // entry: corner(q) + middle - corner(k)
-    Biases<EVEN> bias(map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr, a, own.corner,
+    Biases<EVEN, kTable<HD>> bias(map.bias ? map.bias + (size_t)lt.head * a.entries : nullptr, a, own.corner,
                       window[lt.tile * 64].corner, window);
+    bias.copy(a, bias_s);
     if (todo) {
         rows(__builtin_ctzll(todo));
         bias.fetch(a, __builtin_amdgcn_readlane(meet.corner, __builtin_ctzll(todo)));
