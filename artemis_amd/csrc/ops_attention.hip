@@ -83,11 +83,23 @@ __global__ __launch_bounds__(256) void table_small(const WindowArgs a, const flo
     if (lane == 0) dtable[(size_t)e * a.heads + head] = s;
 }
 
-// dtable[e][head] for long windows that tiles of ed x eh x ew = 64 tokens divide: dense is [share][distance of tiles]
-// [head][64][64] (long_bwd_pairs).  For each query of a tile the key at this distance is one token of one tile: 64 terms for
-// each share, a quarter for each wave.  Neighbouring lanes have neighbouring distances: they read neighbouring keys.
+// The shares of `dense`, into the first, in order.  (Summed where they are read, by few workgroups, 113 shares of 3 distances and 3
+// heads took 790 us; here 11, and 8 there.)
+__global__ __launch_bounds__(256) void shares_fold(float *dense, int shares, long long count)
+{
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i >= count) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < shares; ++k) s += dense[k * count + i];
+    dense[i] = s;
+}
+
+// dtable[e][head] for long windows that tiles of ed x eh x ew = 64 tokens divide: dense is [distance of tiles][head][64][64]
+// (long_bwd_pairs).  For each query of a tile the key at this distance is one token of one tile: 64 terms, a quarter for
+// each wave.  Neighbouring lanes have neighbouring distances: they read neighbouring keys.
 __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const PairWork w, const float *__restrict__ dense,
-                                                   float *__restrict__ dtable, int distances)
+                                                   float *__restrict__ dtable)
 {
     __shared__ float fold[4][64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, head = blockIdx.y;
@@ -113,33 +125,20 @@ __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const Pai
     const Axis z(dd, ld, w.gd, (2 * w.gh - 1) * (2 * w.gw - 1), 1 << (lw + lh));
     const unsigned stride = (unsigned)a.heads * 4096;
     float s = 0.f;
-    for (int share = 0; share < w.chunks; ++share) {
-        const float *from = dense + ((size_t)share * distances * a.heads + head) * 4096;
+    const float *from = dense + (size_t)head * 4096;
 #pragma unroll 8
-        for (int q = wave * 16; q < wave * 16 + 16; ++q) {  // (the same q in every lane: its coordinates are scalars)
-            const int ix = q & ((1 << lw) - 1), iy = q >> lw & ((1 << lh) - 1), iz = q >> (lw + lh);
-            const int bx = ix < x.m, by = iy < y.m, bz = iz < z.m;
-            const int far = (bx ? x.far[1] : x.far[0]) + (by ? y.far[1] : y.far[0]) + (bz ? z.far[1] : z.far[0]);
-            const int key = (bx ? x.key[1] : x.key[0]) + (by ? y.key[1] : y.key[0]) + (bz ? z.key[1] : z.key[0]);
-            // (the key's coordinates are the query's plus these: the query's place in the tile is q itself)
-            if (far >= 0) s += from[(unsigned long long)(unsigned)far * stride + (unsigned)(q * 65 + key)];
-        }
+    for (int q = wave * 16; q < wave * 16 + 16; ++q) {  // (the same q in every lane: its coordinates are scalars)
+        const int ix = q & ((1 << lw) - 1), iy = q >> lw & ((1 << lh) - 1), iz = q >> (lw + lh);
+        const int bx = ix < x.m, by = iy < y.m, bz = iz < z.m;
+        const int far = (bx ? x.far[1] : x.far[0]) + (by ? y.far[1] : y.far[0]) + (bz ? z.far[1] : z.far[0]);
+        const int key = (bx ? x.key[1] : x.key[0]) + (by ? y.key[1] : y.key[0]) + (bz ? z.key[1] : z.key[0]);
+        // (the key's coordinates are the query's plus these: the query's place in the tile is q itself)
+        if (far >= 0) s += from[(unsigned long long)(unsigned)far * stride + (unsigned)(q * 65 + key)];
     }
     fold[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && (int)blockIdx.x * 64 + lane < a.entries)
         dtable[(size_t)e * a.heads + head] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
-}
-
-// The shares of `dense`, into the first, in order
-__global__ __launch_bounds__(256) void shares_fold(float *dense, int shares, long long count)
-{
-    const long long i = blockIdx.x * 256LL + threadIdx.x;
-    if (i >= count) return;
-    float s = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < shares; ++k) s += dense[k * count + i];
-    dense[i] = s;
 }
 
 // dtable[e][head] for other long windows, from dense [head][n][n]: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
@@ -445,16 +444,17 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
         launch_attention_bwd<__bf16>(a, b, st);
     else
         launch_attention_bwd<_Float16>(a, b, st);
-    if (dtable && is_long && b.work.gd) {
-        const int distances = (2 * b.work.gd - 1) * (2 * b.work.gh - 1) * (2 * b.work.gw - 1);
-        hipLaunchKernelGGL(table_tiled, dim3((a.entries + 63) / 64, a.heads), dim3(256), 0, st, a, b.work, b.dense, dtable,
-                           distances);
-    } else if (dtable && is_long) {
-        const long long count = (long long)a.heads * a.n * a.n;
-        if (b.work.chunks > 1)
-            hipLaunchKernelGGL(shares_fold, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, b.dense, b.work.chunks, count);
-        hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st,
-                           a, b.dense, dtable);
+    if (dtable && is_long) {
+        const PairWork &p = b.work;
+        const long long count = p.gd ? (2LL * p.gd - 1) * (2 * p.gh - 1) * (2 * p.gw - 1) * a.heads * 4096
+                                     : (long long)a.heads * a.n * a.n;
+        if (p.chunks > 1)
+            hipLaunchKernelGGL(shares_fold, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, b.dense, p.chunks, count);
+        if (p.gd)
+            hipLaunchKernelGGL(table_tiled, dim3((a.entries + 63) / 64, a.heads), dim3(256), 0, st, a, p, b.dense, dtable);
+        else
+            hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st, a,
+                               b.dense, dtable);
     } else if (dtable) {
         const int nb = small_nb(a.n), elements = 64 * 16 * nb;
         hipLaunchKernelGGL(pairs_fold, dim3(elements / 64, a.heads), dim3(256), 0, st, b.pairs, b.dense, a.heads, b.groups,

@@ -173,6 +173,15 @@ def test_many_windows_that_64_tokens_do_not_tile(shape, window, heads, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape,window,heads", [((2, 2, 32, 32), (1, 8, 16), 2), ((3, 8, 8, 16), (4, 8, 8), 1)])
+def test_many_windows_that_64_tokens_tile(shape, window, heads, dtype):
+    """Likewise, by distances of tiles."""
+    qkv, table, dout = data(shape, window, heads, 16, dtype, 73)
+    check(qkv, table, window, heads, dout, shift=(0, 3, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_the_longest_window(dtype):
     shape = window = (4, 32, 32)
     qkv, table, dout = data((1, *shape), window, 1, 8, dtype, 19)
