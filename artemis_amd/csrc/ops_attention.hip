@@ -141,30 +141,42 @@ __global__ __launch_bounds__(256) void table_tiled(const WindowArgs a, const Pai
         dtable[(size_t)e * a.heads + head] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
 }
 
-// dtable[e][head] for other long windows, from dense [head][n][n]: the workgroup has the entries of one (dd, dh) and goes through the queries' rows; a
-// lane has one dw, so that neighbouring lanes read neighbouring keys.  Four waves take every fourth row.
-__global__ __launch_bounds__(256) void table_long(const WindowArgs a, const float *__restrict__ dense,
+// dtable[e][head] for other long windows, from dense [head][n][n]: the workgroup has the entries of one (dd, dh) and goes
+// through the queries' rows; a lane has one dw, so that neighbouring lanes read neighbouring keys.  Sixteen waves take every sixteenth
+// row.  Eight queries' loads are in flight, also of queries that have no such key (not added): 1386 tokens, 8 heads, 50 us; one
+// after the other, by four waves, 97.
+__global__ __launch_bounds__(1024) void table_long(const WindowArgs a, const float *__restrict__ dense,
                                                   float *__restrict__ dtable)
 {
-    __shared__ float fold[4][64];
+    __shared__ float fold[16][64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int head = blockIdx.z;
     const int dh = (int)blockIdx.y % (2 * a.wh - 1) - (a.wh - 1), dd = (int)blockIdx.y / (2 * a.wh - 1) - (a.wd - 1);
-    const int e = blockIdx.x * 64 + lane, dw = e - (a.ww - 1);
+    const int e = blockIdx.x * 64 + lane, dw = min(e, a.rh - 1) - (a.ww - 1);
+    const int lo = max(dw, 0), hi = min(a.ww, a.ww + dw);  // queries whose key is in the row: one at least
     float s = 0.f;
     const int rows = a.wd * a.wh;
-    for (int row = wave; row < rows; row += 4) {
+    for (int row = wave; row < rows; row += 16) {
         const int qd = row / a.wh, qh = row % a.wh, kd = qd - dd, kh = qh - dh;
         if (kd < 0 || kd >= a.wd || kh < 0 || kh >= a.wh) continue;
         const float *line = dense + ((size_t)head * a.n + (size_t)row * a.ww) * a.n + (kd * a.wh + kh) * a.ww - dw;
-        const int lo = dw > 0 ? dw : 0, hi = dw < 0 ? a.ww + dw : a.ww;  // queries whose key is in the row
-        if (e < a.rh)
-            for (int qw = lo; qw < hi; ++qw) s += line[(size_t)qw * a.n + qw];
+        for (int first = 0; first < a.ww; first += 8) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int qw = min(max(first + k, lo), hi - 1);
+                x[k] = line[(size_t)qw * a.n + qw];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += first + k >= lo && first + k < hi ? x[k] : 0.f;
+        }
     }
     fold[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && e < a.rh)
-        dtable[((size_t)blockIdx.y * a.rh + e) * a.heads + head] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
+    if (wave != 0 || e >= a.rh) return;
+    float t = 0.f;
+    for (int w = 0; w < 16; ++w) t += fold[w][lane];
+    dtable[((size_t)blockIdx.y * a.rh + e) * a.heads + head] = t;
 }
 
 __global__ void fill_zero(float *p, long long n)
@@ -453,7 +465,7 @@ int artemis_ops_window_attention_backward(const artemis_ops_window *w, const voi
         if (p.gd)
             hipLaunchKernelGGL(table_tiled, dim3((a.entries + 63) / 64, a.heads), dim3(256), 0, st, a, p, b.dense, dtable);
         else
-            hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(256), 0, st, a,
+            hipLaunchKernelGGL(table_long, dim3((a.rh + 63) / 64, (2 * a.wd - 1) * (2 * a.wh - 1), a.heads), dim3(1024), 0, st, a,
                                b.dense, dtable);
     } else if (dtable) {
         const int nb = small_nb(a.n), elements = 64 * 16 * nb;
