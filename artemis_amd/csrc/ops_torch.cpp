@@ -3,6 +3,8 @@
 // than the kernels on all but large inputs, and a step over 320 tensors 0.7 ms.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
@@ -89,6 +91,23 @@ variable_list once(variable_list grads)
     return grads;
 }
 
+// A leaf's gradient node is made with the first graph that has the leaf and lives with it.  Where that was on the default
+// stream and is alive, a backward pass under capture makes torch wait for the capture on the default stream, which ends the
+// capture, and may end the process: refused here, in front of that.
+void no_outside_graph()
+{
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (const auto &edge : node->next_edges()) {
+        auto *leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get());
+        if (!leaf) continue;
+        const auto stream = leaf->stream();
+        TORCH_CHECK(!stream || stream->id() != 0, "this backward pass is being captured while a graph of the same tensors that "
+                    "was made on the default stream is alive: delete its outputs before the capture");
+    }
+}
+
 // -------------------------------------------------------------------------------------------- layer norm
 
 class LayerNorm : public torch::autograd::Function<LayerNorm> {
@@ -120,6 +139,7 @@ public:
         const int64_t cols = x.size(-1), rows = cols ? x.numel() / cols : 0;
         const int type = type_code(x, "x");
         const c10::DeviceGuard guard(x.device());
+        no_outside_graph();
         const at::Tensor dy = dys[0].contiguous();
         const auto f32 = x.options().dtype(at::kFloat);
         at::Tensor dx, dw, db, workspace;
@@ -197,6 +217,7 @@ public:
         const std::string packed = ctx->saved_data["w"].toStringRef();
         memcpy(&w, packed.data(), sizeof(w));
         const c10::DeviceGuard guard(qkv.device());
+        no_outside_graph();
         const at::Tensor dout = aligned(douts[0].contiguous());
         const at::Tensor dqkv = at::empty_like(qkv);
         at::Tensor dtable;

@@ -8,7 +8,8 @@ learned relative-position bias and region masks.
 As for the synthesis op: tensors on a HIP device, contiguous (asserted), on torch's current stream; CPU
 tensors raise ``NotImplementedError``; no fallback.  fp32, bf16 and fp16; sums, softmax statistics and
 parameter gradients are fp32 whatever the type.  No atomics: results are the same bits in every run.  Every
-call only enqueues kernels, so it can be captured into a HIP graph.  First derivatives only.  The host side of a
+call only enqueues kernels, so it can be captured into a HIP graph -- a backward pass while no graph of the same
+leaves that was made on the default stream is alive (refused).  First derivatives only.  The host side of a
 call (checks, memory, autograd) is csrc/ops_torch.cpp.
 """
 from __future__ import annotations

@@ -125,3 +125,43 @@ def test_defaults_and_refusals():
     enc.blocks[0].norm1.ops = "hip"
     with pytest.raises(NotImplementedError):
         enc(torch.randn(1, 32, 4, 8, 8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["norm", "attention"])
+def test_a_capture_beside_an_eager_graph_is_refused(op):
+    """With an eager graph of the same leaves alive, torch would tie the capture to the default stream."""
+    g = torch.Generator().manual_seed(31)
+    if op == "norm":
+        x, w = torch.randn(8, 64, generator=g).cuda(), torch.randn(64, generator=g).cuda()
+        call = artemis_amd.layer_norm
+    else:
+        x, w = torch.randn(1, 1, 8, 8, 96, generator=g).cuda(), torch.randn(225, 1, generator=g).cuda()
+
+        def call(a, b):
+            return artemis_amd.window_attention(a, b, (1, 8, 8), 1)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+
+    def step():
+        out = call(x, w)
+        return (out, *torch.autograd.grad(out, (x, w), torch.ones_like(out)))
+
+    want = [t.detach().clone() for t in step()]
+    alive = call(x, w)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="being captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, want):
+            assert torch.equal(a, b)
+        again = step()
+        torch.cuda.synchronize()
+        assert torch.equal(again[1], want[1])
+        del again
