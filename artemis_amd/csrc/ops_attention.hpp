@@ -523,7 +523,6 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
 #pragma unroll
         for (int c = 0; c < CB; ++c) qf[c] = cleared<T>(qn[c], at.source[q] >= 0 && c * 16 + 4 * g < a.hd);
         __syncthreads();
-        const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
         const bool mixed = at.mixed;
         if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
         Place coming;
@@ -541,8 +540,10 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
             }
         }
         if (mixed) {
+            const int ql = at.label[q], qr = at.wrap[q];
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
+                __builtin_amdgcn_sched_barrier(0);  // (few labels at a time: their registers cost all tiles a wave)
                 const int key = (kb0 + j) * 16 + 4 * g;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
@@ -571,6 +572,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
 #pragma unroll
         for (int c = 0; c < CB; ++c) o[c] = f32x4{};
         over_unit<T, HD, NB>(o, Vt, kb0 * 16, p, NB == 1 && odd_s[now], a.n);
+        const int mine = at.token[q];
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             *(Frag *)store_at(out + (unsigned long long)(unsigned)mine * (unsigned)C + walk.head * a.hd + c * 16 + 4 * g, spare,
@@ -674,7 +676,6 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         }
         __syncthreads();
         const Spots &at = spots[now];
-        const int mine = at.token[q], ql = at.label[q], qr = at.wrap[q];
         const bool mixed = at.mixed, odd = NB == 1 && odd_s[now];
         if (NB == 1 && threadIdx.x == 0) odd_s[next] = 0;  // (its last readers were two tiles ago)
         Place coming;
@@ -701,8 +702,10 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
             }
         }
         if (mixed) {
+            const int ql = at.label[q], qr = at.wrap[q];
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
+                __builtin_amdgcn_sched_barrier(0);  // (few labels at a time: their registers cost all tiles a wave)
                 const int key = (kb0 + j) * 16 + 4 * g;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
@@ -744,6 +747,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
 #pragma unroll
         for (int c = 0; c < CB; ++c) acc[c] = f32x4{};
         over_unit<T, HD, NB, K_BY_ROWS>(acc, K_BY_ROWS ? Ks : Kt, kb0 * 16, ds, odd, a.n);
+        const int mine = at.token[q];
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             *(Frag *)store_at(dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g, spare, mine >= 0 && c * 16 + 4 * g < a.hd) =
@@ -751,13 +755,16 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         __syncthreads();  // K and V have been used
         const int ql_ = wave % NB * 16 + i;  // this lane's query within its unit
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < NB; ++j) {
+            settle(p[j]);  // (the rounded values, not their rounding once more)
+            settle(ds[j]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int at = pair_at<NB>((kb0 + j) * 16 + 4 * g + r, ql_);
                 Ps[at] = p[j][r];
                 Ss[at] = ds[j][r];
             }
+        }
         __syncthreads();
         // now slot q is this lane's key
 #pragma unroll
