@@ -279,6 +279,22 @@ __device__ __forceinline__ void over_tokens(f32x4 (&acc)[HD / 16], const T *tile
     }
 }
 
+// the same of a whole tile with two operands, each piece of the tile read once
+template <class T, int HD>
+__device__ __forceinline__ void over_tokens_both(f32x4 (&x)[HD / 16], f32x4 (&y)[HD / 16], const T *tile,
+                                                 const typename Mma<T>::Frag (&bx)[4], const typename Mma<T>::Frag (&by)[4])
+{
+    using M = Mma<T>;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            const typename M::Frag f0 = column<T, HD, false>(tile, c, j * 16), f1 = column<T, HD, false>(tile, c, j * 16 + 16);
+            x[c] = M::run2(f0, f1, bx[j], bx[j + 1], x[c]);
+            y[c] = M::run2(f0, f1, by[j], by[j + 1], y[c]);
+        }
+}
+
 // ================================================================================================
 // Windows of at most 64 tokens.  A tile is 64 slots: units of 16 * NB slots, each holding one window (NB > 1) or
 // as many as fit 16 slots (NB = 1).  Wave w has the queries of slots 16w .. 16w+15; their keys are the NB
@@ -830,7 +846,7 @@ struct LongMap {
 struct Split {
     int splits;
     float *a, *b;  // [split][window, head, tile, 64][head_dim]: sums of the products over tokens
-    float *rows;   // [split][window, head, tile, 64][2]: forward: maximum and sum of the softmax; dQ: delta's share
+    float *rows;   // [split][window, head, tile, 64][2]: forward: maximum and sum of the softmax; dQ: near and rest
 };
 
 struct LongTile {
@@ -1185,8 +1201,12 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd_join(const WindowArgs a
 }
 
 // dQ, and delta = sum over keys of P dP for each query.  delta is also the product of out and dout; in 16 bits `out` is
-// rounded, so that product c is only near: dS = P (dP - c) serves dQ, which is rounded as coarsely itself, and
-// c + sum P (dP - c), summed here in fp32, is the delta that the table's gradient and dK are computed with.
+// rounded, so that product c is only near: off by about half a step of |out| |dout|.  Where keys and values have a mean, as
+// behind a projection with a bias, that times sum P K is as large as dQ itself (4 deviations, 4096 tokens, bf16: dQ off by as much
+// as its size).  So dS = P (dP - c) is what the product with K takes, rest = sum P (dP - c), summed in fp32, gives
+// delta = c + rest, which the table's gradient and dK are computed with, and
+//     dQ = sum dS K - rest sum P K,
+// in which the rounding of P counts only for what c was off by.  In fp32 c is as near as any sum here: no second product.
 template <class T, int HD, bool EVEN>
 __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(const WindowArgs a, const LongMap map, const Split split,
                                                            const T *__restrict__ qkv, const T *__restrict__ out,
@@ -1244,9 +1264,9 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
     const float shift = own.token >= 0 ? lse[padded] : INFINITY;
     const float scale2 = a.scale * kLog2e;
     float rest = 0.f;
-    f32x4 dq[CB];
+    f32x4 dq[CB], pk[CB];  // pk: sum P K
 #pragma unroll
-    for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
+    for (int c = 0; c < CB; ++c) dq[c] = pk[c] = f32x4{};
     while (todo) {
         const int now = __builtin_ctzll(todo);
         const bool mixed = meet.mixed >> now & 1, any = meet.any >> now & 1;
@@ -1267,45 +1287,54 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
         }
         if (!any) continue;  // (the barriers are at the loop's head)
         bias.take(bias_s, at_s);
-        Frag ds[4];
+        Frag ds[4], pf[4];
         f32x4 x[4], dp[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Vs, j * 16, gf);
         scores<T, HD>(x, Ks, qf, scale2, bias.now, mixed, own, at_s, a.outside2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 d;
+            f32x4 p, d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 // (an empty row: -inf against +inf)
-                const float p = __builtin_amdgcn_exp2f(x[j][r] - shift);
-                d[r] = p * (dp[j][r] - near);
+                p[r] = __builtin_amdgcn_exp2f(x[j][r] - shift);
+                d[r] = p[r] * (dp[j][r] - near);
                 rest += d[r];
             }
             ds[j] = M::frag(d);
+            if constexpr (sizeof(T) == 2) pf[j] = M::frag(p);
         }
-        over_tokens<T, HD>(dq, Kt, 0, ds);
+        if constexpr (sizeof(T) == 2)
+            over_tokens_both<T, HD>(dq, pk, Kt, ds, pf);
+        else
+            over_tokens<T, HD>(dq, Kt, 0, ds);
     }
     rest = fold_sum(rest);
     if (own.label < 0) {
         near = rest = 0.f;
 #pragma unroll
-        for (int c = 0; c < CB; ++c) dq[c] = f32x4{};
+        for (int c = 0; c < CB; ++c) dq[c] = pk[c] = f32x4{};
     }
     if (split.splits > 1) {
         const size_t line = (size_t)blockIdx.y * gridDim.x * 64 + padded;
 #pragma unroll
         for (int c = 0; c < CB; ++c)
-            if (c * 16 + 4 * g < a.hd) *(f32x4 *)(split.a + line * a.hd + c * 16 + 4 * g) = dq[c];
-        if (g == 0) split.rows[line * 2] = blockIdx.y == 0 ? near + rest : rest;
+            if (c * 16 + 4 * g < a.hd) {
+                *(f32x4 *)(split.a + line * a.hd + c * 16 + 4 * g) = dq[c];
+                if constexpr (sizeof(T) == 2) *(f32x4 *)(split.b + line * a.hd + c * 16 + 4 * g) = pk[c];
+            }
+        if (g == 0) split.rows[line * 2] = near, split.rows[line * 2 + 1] = rest;
         return;
     }
     if (own.token < 0) return;
     if (g == 0) delta[padded] = near + rest;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
-        if (c * 16 + 4 * g < a.hd)
+        if (c * 16 + 4 * g < a.hd) {
+            if constexpr (sizeof(T) == 2) dq[c] -= pk[c] * rest;
             *(Frag *)(dqkv + (size_t)own.token * stride + lt.head * a.hd + c * 16 + 4 * g) = M::frag(dq[c] * a.scale);
+        }
 }
 
 // dK and dV: wave w has 16 keys and goes through the queries, S = Q K^T (rows: queries, lane: key), so that P and dS have the
@@ -1454,21 +1483,21 @@ __global__ __launch_bounds__(kAttnThreads) void long_bwd_join(const WindowArgs a
     const int head = (int)(r % (size_t)a.heads), C = a.heads * a.hd;
     const PlaceAt own = map.places[r / (size_t)a.heads * (size_t)map.tiles * 64 + line % ((size_t)map.tiles * 64)];
     if (own.token < 0) return;
+    constexpr bool TAKE_BACK = !KV && sizeof(T) == 2;  // what delta was off by, times sum P K: see long_bwd_q
     f32x4 x{}, y{};
-    float del = 0.f;
+    float rest = 0.f;
     for (int k = 0; k < split.splits; ++k) {
         x += *(const f32x4 *)(split.a + (k * lines + line) * a.hd + c);
-        if constexpr (KV)
-            y += *(const f32x4 *)(split.b + (k * lines + line) * a.hd + c);
-        else
-            del += split.rows[(k * lines + line) * 2];
+        if constexpr (KV || TAKE_BACK) y += *(const f32x4 *)(split.b + (k * lines + line) * a.hd + c);
+        if constexpr (!KV) rest += split.rows[(k * lines + line) * 2 + 1];
     }
+    if constexpr (TAKE_BACK) x -= y * rest;
     T *to = dqkv + (size_t)own.token * 3 * C + head * a.hd + c;
     *(typename Mma<T>::Frag *)(to + (KV ? C : 0)) = Mma<T>::frag(x * a.scale);
     if constexpr (KV)
         *(typename Mma<T>::Frag *)(to + 2 * C) = Mma<T>::frag(y);
     else if (c == 0)
-        delta[line] = del;
+        delta[line] = split.rows[line * 2] + rest;  // (`near` is the same in every share)
 }
 
 // The table's gradient sums dS over all pairs of one distance.  Where 64 tokens tile the window evenly (ed x eh x ew tokens,
