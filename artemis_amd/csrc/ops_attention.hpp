@@ -101,6 +101,26 @@ struct Mma<_Float16> {
     }
 };
 
+// fp16 operands.  Below 2^-14 the type's steps stay 2^-24 wide, and beyond 65504 there is nothing.  P of thousands of keys, and
+// dS = P (dP - delta) the more so where dout is small, lie below, though their sums do not (dS unscaled: at 4096 tokens and dout of
+// 1e-3, dQ and dK off by 7e-3 of their size); dS with a scaled loss may lie above.  So P enters the products times 2^15 (nothing is
+// above 1), and dS times a power of two of its column: a query in dQ, a key in dK, both of which a lane's column of the result
+// belongs to, and so does the way back.  bf16 has fp32's exponents and takes both as they are.
+template <class T>
+constexpr int kLift = 0;
+template <>
+inline constexpr int kLift<_Float16> = 15;
+template <class T>
+constexpr float kDown = kLift<T> ? 0x1p-15f : 1.f;
+
+// the exponent of a magnitude, -98 at least: its power of two and that one's reciprocal, times up to 2^29, are normal numbers
+__device__ __forceinline__ int exponent_of(float m)
+{
+    const int e = (int)(__builtin_bit_cast(unsigned, m) >> 23) - 127;
+    return e < -98 ? -98 : e;
+}
+__device__ __forceinline__ float two_to(int e) { return __builtin_bit_cast(float, (unsigned)(127 + e) << 23); }
+
 // four neighbours of an LDS tile as an operand
 template <class T>
 __device__ __forceinline__ typename Mma<T>::Frag row4(const T *p)
@@ -153,6 +173,49 @@ __device__ __forceinline__ float fold_sum(float x)
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
+
+// the largest finite magnitude of a lane's values (NaN: left out; an infinity: none is to be had)
+template <int N>
+__device__ __forceinline__ float largest(const f32x4 (&x)[N])
+{
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) m = fmaxf(m, fmaxf(fabsf(x[j][r]), fabsf(x[j][r + 1])));
+    return m;
+}
+
+// The power of two that brings a column's largest magnitude to 2^14 ..: all of the column is here.  1 where it is not finite.
+__device__ __forceinline__ float column_scale(float m)
+{
+    m = fold_max(m);
+    return m < INFINITY ? two_to(14 - exponent_of(m)) : 1.f;
+}
+
+// The same where a column comes tile by tile: the scale follows the largest magnitude met so far, and what has been summed
+// follows the scale.  A new one leaves room for 16 times as much, so that changes are few.
+struct RunningScale {
+    float s = 1.f, limit = 0.f;
+    template <int N, int C>
+    __device__ __forceinline__ void apply(f32x4 (&x)[N], f32x4 (&sum)[C])
+    {
+        float m = largest(x);
+        if (__any(m > limit)) {
+            m = fold_max(m);
+            if (m > limit && m < INFINITY) {  // (the same in the column's four lanes)
+                const int e = exponent_of(m);
+                const float to = two_to(10 - e), by = to / s;
+                s = to;
+                limit = two_to(e) * 32.f;  // 2^15 when scaled
+#pragma unroll
+                for (int c = 0; c < C; ++c) sum[c] *= by;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] *= s;
+    }
+};
 
 // Four channels of a token's row.  Loaded whether or not there is such a token and channel (from the tensor's first token
 // or the head's first channels then), and cleared where it is used: a load under a condition shares its registers with the
@@ -580,7 +643,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
                 sum += s[j][r];
             }
         sum = fold_sum(sum);
-        const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+        const float inv = sum > 0.f || sum != sum ? 1.0f / kDown<T> / sum : 0.f;
         Frag p[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) p[j] = M::frag(s[j] * inv);  // 16 bit: rounded once, as the product takes it
@@ -592,7 +655,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             *(Frag *)store_at(out + (unsigned long long)(unsigned)mine * (unsigned)C + walk.head * a.hd + c * 16 + 4 * g, spare,
-                              mine >= 0 && c * 16 + 4 * g < a.hd) = M::frag(o[c]);
+                              mine >= 0 && c * 16 + 4 * g < a.hd) = M::frag(o[c] * kDown<T>);
         if (first_wave) spotter.write(spots[after], coming);
         now = next;
     }
@@ -633,6 +696,8 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
     T *const Vs = Ks + ROWS, *const Kt = Vs + ROWS, *const Ps = Ks, *const Ss = Ks + PAIRS;
     __shared__ Spots spots[3];
     __shared__ int odd_s[3];
+    constexpr bool SCALED = kLift<T> != 0;
+    __shared__ __align__(16) float back_s[SCALED ? 64 : 4];  // by query: what undoes the scale of its dS
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16;
     const Walk walk = walk_of(a.heads);
@@ -746,19 +811,30 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
         delta = fold_sum(delta) * inv;
         Frag ds[NB], p[NB];
+        f32x4 d[NB];  // (times 2^kLift)
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            f32x4 pv = s[j] * inv;
-            f32x4 d = pv * (dp[j] - delta);
+            f32x4 pv = s[j] * (inv * (1.0f / kDown<T>));
+            d[j] = pv * (dp[j] - delta);
             if constexpr (NB == 1) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (bias[j][r] == -INFINITY) pv[r] = d[r] = 0.f;
+                    if (bias[j][r] == -INFINITY) pv[r] = d[j][r] = 0.f;
             }
-            dbias[j] += d;
+            dbias[j] += d[j];
             p[j] = M::frag(pv);
-            ds[j] = M::frag(d);  // 16 bit: rounded once, as the products take it; the table's gradient sums it unrounded
         }
+        float to_dq = a.scale * kDown<T>;
+        if constexpr (SCALED) {
+            const float up = column_scale(largest(d));
+#pragma unroll
+            for (int j = 0; j < NB; ++j) d[j] *= up;
+            if (g == 0) back_s[q] = 1.0f / up;
+            to_dq /= up;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) ds[j] = M::frag(d[j]);  // 16 bit: rounded once, as the products take it; the table's
+                                                             // gradient sums it unrounded
         f32x4 acc[CB];
 #pragma unroll
         for (int c = 0; c < CB; ++c) acc[c] = f32x4{};
@@ -767,7 +843,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             *(Frag *)store_at(dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g, spare, mine >= 0 && c * 16 + 4 * g < a.hd) =
-                M::frag(acc[c] * a.scale);
+                M::frag(acc[c] * to_dq);
         __syncthreads();  // K and V have been used
         const int ql_ = wave % NB * 16 + i;  // this lane's query within its unit
 #pragma unroll
@@ -789,6 +865,20 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
             p[j] = row4<T>(&Ps[at]);
             ds[j] = row4<T>(&Ss[at]);
         }
+        float to_dk = a.scale * kDown<T>;
+        if constexpr (SCALED) {  // from the queries' scales to this key's: exact but for what is 2^-29 of its largest
+            f32x4 v[NB];
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const f32x4 back = *(const f32x4 *)&back_s[kb0 * 16 + j * 16 + 4 * g];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[j][r] = (float)ds[j][r] * back[r];
+            }
+            const float up = column_scale(largest(v));
+            to_dk /= up;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) ds[j] = M::frag(v[j] * up);
+        }
         f32x4 dv[CB];
 #pragma unroll
         for (int c = 0; c < CB; ++c) acc[c] = dv[c] = f32x4{};
@@ -798,8 +888,8 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         for (int c = 0; c < CB; ++c) {
             T *to = dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g;
             const bool wanted = mine >= 0 && c * 16 + 4 * g < a.hd;
-            *(Frag *)store_at(to + C, spare, wanted) = M::frag(acc[c] * a.scale);
-            *(Frag *)store_at(to + 2 * C, spare, wanted) = M::frag(dv[c]);
+            *(Frag *)store_at(to + C, spare, wanted) = M::frag(acc[c] * to_dk);
+            *(Frag *)store_at(to + 2 * C, spare, wanted) = M::frag(dv[c] * kDown<T>);
         }
         if (first_wave) spotter.write(spots[after], coming);
         now = next;
@@ -807,7 +897,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
     if (!pairs) return;
     float *to = pairs + (size_t)blockIdx.x * 64 * 16 * NB;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) *(f32x4 *)&to[q * 16 * NB + j * 16 + 4 * g] = dbias[j];
+    for (int j = 0; j < NB; ++j) *(f32x4 *)&to[q * 16 * NB + j * 16 + 4 * g] = dbias[j] * kDown<T>;
 }
 
 // ================================================================================================
@@ -1136,7 +1226,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const 
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - base2);
+                s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - (base2 - kLift<T>));
                 part += s[j][r];
             }
             p[j] = M::frag(s[j]);  // 16 bit: rounded as the product takes it, the sum is of the unrounded ones
@@ -1168,7 +1258,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const 
         if (c * 16 + 4 * g < a.hd)
             *(Frag *)(out + (size_t)own.token * C + lt.head * a.hd + c * 16 + 4 * g) = M::frag(o[c] * inv);
     // log2 of the row's sum of 2^x; +inf for an empty row, so that its P is 0 in the backward pass
-    if (lse && g == 0) lse[padded] = top == -INFINITY ? INFINITY : top + log2f(sum);
+    if (lse && g == 0) lse[padded] = top == -INFINITY ? INFINITY : top + (log2f(sum) - kLift<T>);
 }
 
 // Joins the shares of a forward pass: hd / 4 threads for a query, each with four channels
@@ -1197,7 +1287,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd_join(const WindowArgs a
     }
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
     *(typename Mma<T>::Frag *)(out + (size_t)own.token * a.heads * a.hd + head * a.hd + c) = Mma<T>::frag(o * inv);
-    if (lse && c == 0) lse[line] = top == -INFINITY ? INFINITY : top + log2f(sum);
+    if (lse && c == 0) lse[line] = top == -INFINITY ? INFINITY : top + (log2f(sum) - kLift<T>);
 }
 
 // dQ, and delta = sum over keys of P dP for each query.  delta is also the product of out and dout; in 16 bits `out` is
@@ -1264,6 +1354,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
     const float shift = own.token >= 0 ? lse[padded] : INFINITY;
     const float scale2 = a.scale * kLog2e;
     float rest = 0.f;
+    RunningScale fit;
     f32x4 dq[CB], pk[CB];  // pk: sum P K
 #pragma unroll
     for (int c = 0; c < CB; ++c) dq[c] = pk[c] = f32x4{};
@@ -1288,29 +1379,35 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_q(cons
         if (!any) continue;  // (the barriers are at the loop's head)
         bias.take(bias_s, at_s);
         Frag ds[4], pf[4];
-        f32x4 x[4], dp[4];
+        f32x4 x[4], dp[4], d[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Vs, j * 16, gf);
         scores<T, HD>(x, Ks, qf, scale2, bias.now, mixed, own, at_s, a.outside2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 p, d;
+            f32x4 p;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 // (an empty row: -inf against +inf)
                 p[r] = __builtin_amdgcn_exp2f(x[j][r] - shift);
-                d[r] = p[r] * (dp[j][r] - near);
-                rest += d[r];
+                d[j][r] = p[r] * (dp[j][r] - near);
+                rest += d[j][r];
             }
-            ds[j] = M::frag(d);
             if constexpr (sizeof(T) == 2) pf[j] = M::frag(p);
         }
+        if constexpr (kLift<T> != 0) fit.apply(d, dq);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ds[j] = M::frag(d[j]);
         if constexpr (sizeof(T) == 2)
             over_tokens_both<T, HD>(dq, pk, Kt, ds, pf);
         else
             over_tokens<T, HD>(dq, Kt, 0, ds);
     }
     rest = fold_sum(rest);
+    if constexpr (kLift<T> != 0) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c) dq[c] *= 1.0f / fit.s;
+    }
     if (own.label < 0) {
         near = rest = 0.f;
 #pragma unroll
@@ -1397,6 +1494,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
         vf[c] = load4<T>(base + 2 * C, stride, mine, c * 16 + 4 * g, a.hd);
     }
     const float scale2 = a.scale * kLog2e;
+    RunningScale fit;
     f32x4 dk[CB], dv[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
@@ -1413,7 +1511,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
         ahead.y.store_columns(Gt);
         at.store(at_s, window + now * 64, meet.masks >> now & 1);
         if (threadIdx.x < 64) {
-            lse_s[threadIdx.x] = some >= 0 ? shift : INFINITY;
+            lse_s[threadIdx.x] = some >= 0 ? shift - kLift<T> : INFINITY;
             delta_s[threadIdx.x] = some >= 0 ? del : 0.f;
         }
         bias.store(bias_s);
@@ -1426,24 +1524,30 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
         if (!any) continue;  // (the barriers are at the loop's head)
         bias.take(bias_s, at_s);
         Frag p[4], ds[4];
-        f32x4 x[4], dp[4];
+        f32x4 x[4], dp[4], d[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Gs, j * 16, vf);
         scores<T, HD>(x, Qs, kf, scale2, bias.now, mixed, own, at_s, a.outside2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const f32x4 l = *(const f32x4 *)&lse_s[j * 16 + 4 * g], del4 = *(const f32x4 *)&delta_s[j * 16 + 4 * g];
-            f32x4 pv, d;
+            f32x4 pv;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 pv[r] = __builtin_amdgcn_exp2f(x[j][r] - l[r]);
-                d[r] = pv[r] * (dp[j][r] - del4[r]);
+                d[j][r] = pv[r] * (dp[j][r] - del4[r]);
             }
             p[j] = M::frag(pv);
-            ds[j] = M::frag(d);
         }
+        if constexpr (kLift<T> != 0) fit.apply(d, dk);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ds[j] = M::frag(d[j]);
         over_tokens<T, HD>(dv, Gt, 0, p);
         over_tokens<T, HD>(dk, Qt, 0, ds);
+    }
+    if constexpr (kLift<T> != 0) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c) dk[c] *= kDown<T> / fit.s, dv[c] *= kDown<T>;
     }
     if (own.label < 0) {
 #pragma unroll
