@@ -145,11 +145,13 @@ __device__ __forceinline__ Place place_of(const WindowArgs &a, const int *__rest
     const unsigned w1 = a.by_nw.of(w), kw = w - w1 * a.nw;
     const unsigned w2 = a.by_nh.of(w1), kh = w1 - w2 * a.nh;
     const unsigned b = a.by_nd.of(w2), kd = w2 - b * a.nd;
-    int d = (int)(kd * a.wd + td) + a.sd, h = (int)(kh * a.wh + th) + a.sh, x = (int)(kw * a.ww + tw) + a.sw;
-    if (d >= a.D) d -= a.D, r.wrap |= 1;
-    if (h >= a.H) h -= a.H, r.wrap |= 2;
-    if (x >= a.W) x -= a.W, r.wrap |= 4;
-    const int at = (d * a.H + h) * a.W + x;
+    // (unsigned: in front of the wrap a coordinate may pass 2^31)
+    const unsigned D = (unsigned)a.D, H = (unsigned)a.H, W = (unsigned)a.W;
+    unsigned d = kd * a.wd + td + a.sd, h = kh * a.wh + th + a.sh, x = kw * a.ww + tw + a.sw;
+    if (d >= D) d -= D, r.wrap |= 1;
+    if (h >= H) h -= H, r.wrap |= 2;
+    if (x >= W) x -= W, r.wrap |= 4;
+    const int at = (int)((d * H + h) * W + x);
     r.token = (int)b * a.D * a.H * a.W + at;
     r.label = labels ? labels[(size_t)(a.label_maps > 1 ? b : 0) * a.D * a.H * a.W + at] : 0;
     return r;
