@@ -479,6 +479,20 @@ __device__ __forceinline__ void pair_biases(f32x4 (&b)[NB], const WindowArgs &a,
         for (int r = 0; r < 4; ++r) b[j][r] = meet >> (j * 4 + r) & 1 ? b[j][r] * kLog2e : -INFINITY;
 }
 
+// the mask of (query slot q, key slots of NB blocks)
+template <int NB>
+__device__ __forceinline__ void mask_slots(f32x4 (&s)[NB], const Spots &at, int q, int key, float outside2)
+{
+    const int ql = at.label[q], qr = at.wrap[q];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        __builtin_amdgcn_sched_barrier(0);  // (few labels at a time: their registers cost all tiles a wave)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            s[j][r] = masked(s[j][r], ql, qr, at.label[key + j * 16 + r], at.wrap[key + j * 16 + r], outside2);
+    }
+}
+
 template <class T, int HD>
 __device__ __forceinline__ void tokens_at(const Spots &at, int (&token)[Rows<T, HD>::kPieces])
 {
@@ -559,6 +573,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
     if (walk.tile >= tiles) return;
     const int kb0 = wave / NB * NB;  // the first key block of this wave's unit
     const int q = wave * 16 + i;
+    const bool gaps = NB > 1 && a.n < 16 * NB;  // slots without a token beside a window's
     f32x4 bias[NB];
     const float scale2 = a.scale * kLog2e;
     const Spotter<NB> spotter(a);
@@ -620,15 +635,14 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
                 if (NB == 1 && bias[j][r] == -INFINITY) s[j][r] = -INFINITY;  // (of another window: whatever it is)
             }
         }
-        if (mixed) {
-            const int ql = at.label[q], qr = at.wrap[q];
+        if (gaps || mixed) {
+            if (gaps) {  // empty slots: 0 times an infinity is NaN
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                __builtin_amdgcn_sched_barrier(0);  // (few labels at a time: their registers cost all tiles a wave)
-                const int key = (kb0 + j) * 16 + 4 * g;
+                for (int j = 0; j < NB; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
+                    for (int r = 0; r < 4; ++r) s[j][r] = bias[j][r] == -INFINITY ? -INFINITY : s[j][r];
             }
+            if (mixed) mask_slots<NB>(s, at, q, kb0 * 16 + 4 * g, a.outside2);
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -711,6 +725,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
     const long long tiles = (a.windows + per - 1) / per;
     const int kb0 = wave / NB * NB;
     const int q = wave * 16 + i;
+    const bool gaps = NB > 1 && a.n < 16 * NB;  // slots without a token beside a window's
     f32x4 bias[NB], dbias[NB];
     const float scale2 = a.scale * kLog2e;
     const Spotter<NB> spotter(a);
@@ -784,15 +799,14 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
                 if (NB == 1 && bias[j][r] == -INFINITY) s[j][r] = -INFINITY, dp[j][r] = 0.f;
             }
         }
-        if (mixed) {
-            const int ql = at.label[q], qr = at.wrap[q];
+        if (gaps || mixed) {
+            if (gaps) {  // empty slots: 0 times an infinity is NaN
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                __builtin_amdgcn_sched_barrier(0);  // (few labels at a time: their registers cost all tiles a wave)
-                const int key = (kb0 + j) * 16 + 4 * g;
+                for (int j = 0; j < NB; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[j][r] = masked(s[j][r], ql, qr, at.label[key + r], at.wrap[key + r], a.outside2);
+                    for (int r = 0; r < 4; ++r) s[j][r] = bias[j][r] == -INFINITY ? -INFINITY : s[j][r];
             }
+            if (mixed) mask_slots<NB>(s, at, q, kb0 * 16 + 4 * g, a.outside2);
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -981,6 +995,7 @@ __device__ __forceinline__ TileAt tile_of(const PlaceAt &p, int corner)
 // of its waves meets, or every splits-th of them.
 struct Meets {
     unsigned long long todo, any, mixed, masks;  // masks: `mixed` of any wave
+    unsigned long long gaps;                     // tiles that may hold padding, or a window's end
     int corner;  // this lane's tile's first token's
 };
 template <bool PADDING_OK>
@@ -1000,7 +1015,7 @@ __device__ __forceinline__ Meets meets(const LongMap &m, long long window, const
 #pragma unroll
     for (int k = 0; k < W; ++k) all |= bits[k], masks |= bits[W + k];
     if (splits > 1) all = __ballot((all >> lane & 1) && __popcll(all & ((1ull << lane) - 1)) % splits == (int)blockIdx.y);
-    return {all, mine, masked, masks, other.corner};
+    return {all, mine, masked, masks, __ballot(other.state != kEven), other.corner};
 }
 
 // The bias of a tile's pairs.
@@ -1144,6 +1159,13 @@ struct TilePlaces {
     }
 };
 
+// log2 of a row's sum of 2^x; +inf for an empty row, so that its P is 0 in the backward pass (a sum of NaN alone stays NaN)
+template <class T>
+__device__ __forceinline__ float lse_of(float top, float sum)
+{
+    return top == -INFINITY && sum == 0.f ? INFINITY : top + (log2f(sum) - kLift<T>);
+}
+
 template <class T, int HD, bool EVEN>
 __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const WindowArgs a, const LongMap map, const Split split,
                                                          const T *__restrict__ qkv, T *__restrict__ out,
@@ -1259,8 +1281,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_fwd(const 
     for (int c = 0; c < CB; ++c)
         if (c * 16 + 4 * g < a.hd)
             *(Frag *)(out + (size_t)own.token * C + lt.head * a.hd + c * 16 + 4 * g) = M::frag(o[c] * inv);
-    // log2 of the row's sum of 2^x; +inf for an empty row, so that its P is 0 in the backward pass
-    if (lse && g == 0) lse[padded] = top == -INFINITY ? INFINITY : top + (log2f(sum) - kLift<T>);
+    if (lse && g == 0) lse[padded] = lse_of<T>(top, sum);
 }
 
 // Joins the shares of a forward pass: hd / 4 threads for a query, each with four channels
@@ -1289,7 +1310,7 @@ __global__ __launch_bounds__(kAttnThreads) void long_fwd_join(const WindowArgs a
     }
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
     *(typename Mma<T>::Frag *)(out + (size_t)own.token * a.heads * a.hd + head * a.hd + c) = Mma<T>::frag(o * inv);
-    if (lse && c == 0) lse[line] = top == -INFINITY ? INFINITY : top + (log2f(sum) - kLift<T>);
+    if (lse && c == 0) lse[line] = lse_of<T>(top, sum);
 }
 
 // dQ, and delta = sum over keys of P dP for each query.  delta is also the product of out and dout; in 16 bits `out` is
@@ -1495,6 +1516,14 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
         kf[c] = load4<T>(base + C, stride, mine, c * 16 + 4 * g, a.hd);
         vf[c] = load4<T>(base + 2 * C, stride, mine, c * 16 + 4 * g, a.hd);
     }
+    // Where there is no query its row is zeros, and 0 times an infinity of a key is NaN: where there are such keys, tiles with such
+    // rows are masked too.  (An infinity of V needs nothing: all that it meets in dK is NaN by itself.)
+    float zero = 0.f;
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) zero += (float)kf[c][r] * 0.f;
+    const unsigned long long gaps = __syncthreads_or(zero != 0.f) ? meet.gaps : 0;
     const float scale2 = a.scale * kLog2e;
     RunningScale fit;
     f32x4 dk[CB], dv[CB];
@@ -1502,7 +1531,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
     for (int c = 0; c < CB; ++c) dk[c] = dv[c] = f32x4{};
     while (todo) {
         const int now = __builtin_ctzll(todo);
-        const bool mixed = meet.mixed >> now & 1, any = meet.any >> now & 1;
+        const bool mixed = (meet.mixed | gaps) >> now & 1, any = meet.any >> now & 1;
         todo = later;
         later &= later - 1;
         __syncthreads();
@@ -1511,7 +1540,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_kv(con
         ahead.x.store_columns(Qt);
         ahead.y.store_rows(Gs);
         ahead.y.store_columns(Gt);
-        at.store(at_s, window + now * 64, meet.masks >> now & 1);
+        at.store(at_s, window + now * 64, (meet.masks | gaps) >> now & 1);
         if (threadIdx.x < 64) {
             lse_s[threadIdx.x] = some >= 0 ? shift - kLift<T> : INFINITY;
             delta_s[threadIdx.x] = some >= 0 ? del : 0.f;
@@ -1759,8 +1788,10 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_pairs(
             settle(gf[c]);
         }
         float shift = no_row ? INFINITY : shift_next, del = no_row ? 0.f : del_next;
+        unsigned empty = no_row;
         settle(shift);
         settle(del);
+        settle(empty);
         PlaceAt own{};
         if (hand.mixed) {  // (loaded when wanted)
             const PlaceAt *window = map.places + hand.window * map.tiles * 64;
@@ -1778,6 +1809,12 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void long_bwd_pairs(
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[j] = over_channels<T, HD>(Vs, j * 16, gf);
         scores<T, HD>(x, Ks, qf, scale2, bias, hand.mixed, own, at_s, a.outside2);
+        if (__any(empty != 0)) {  // the rows of no query are zeros, and 0 times an infinity of K or V is NaN
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[j][r] = empty ? 0.f : x[j][r], dp[j][r] = empty ? 0.f : dp[j][r];
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
