@@ -668,10 +668,11 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_fwd(cons
         for (int c = 0; c < CB; ++c) o[c] = f32x4{};
         over_unit<T, HD, NB>(o, Vt, kb0 * 16, p, NB == 1 && odd_s[now], a.n);
         const int mine = at.token[q];
+        const bool padding = LABELS && at.source[q] < 0;  // (0 whatever its window holds: 0 times an infinity is NaN)
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             *(Frag *)store_at(out + (unsigned long long)(unsigned)mine * (unsigned)C + walk.head * a.hd + c * 16 + 4 * g, spare,
-                              mine >= 0 && c * 16 + 4 * g < a.hd) = M::frag(o[c] * kDown<T>);
+                              mine >= 0 && c * 16 + 4 * g < a.hd) = cleared<T>(M::frag(o[c] * kDown<T>), !padding);
         if (first_wave) spotter.write(spots[after], coming);
         now = next;
     }
@@ -806,7 +807,13 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[j][r] = bias[j][r] == -INFINITY ? -INFINITY : s[j][r];
             }
-            if (mixed) mask_slots<NB>(s, at, q, kb0 * 16 + 4 * g, a.outside2);
+            if (mixed) {
+                mask_slots<NB>(s, at, q, kb0 * 16 + 4 * g, a.outside2);
+                if (LABELS && at.source[q] < 0) {  // (as a query: its P is 0, and 0 times an infinity is NaN)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) dp[j] = f32x4{};
+                }
+            }
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -856,10 +863,11 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         for (int c = 0; c < CB; ++c) acc[c] = f32x4{};
         over_unit<T, HD, NB, K_BY_ROWS>(acc, K_BY_ROWS ? Ks : Kt, kb0 * 16, ds, odd, a.n);
         const int mine = at.token[q];
+        const bool padding = LABELS && at.source[q] < 0;
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             *(Frag *)store_at(dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g, spare, mine >= 0 && c * 16 + 4 * g < a.hd) =
-                M::frag(acc[c] * to_dq);
+                cleared<T>(M::frag(acc[c] * to_dq), !padding);
         __syncthreads();  // K and V have been used
         const int ql_ = wave % NB * 16 + i;  // this lane's query within its unit
 #pragma unroll
@@ -904,8 +912,8 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
         for (int c = 0; c < CB; ++c) {
             T *to = dbase + (unsigned long long)(unsigned)mine * stride + c * 16 + 4 * g;
             const bool wanted = mine >= 0 && c * 16 + 4 * g < a.hd;
-            *(Frag *)store_at(to + C, spare, wanted) = M::frag(acc[c] * to_dk);
-            *(Frag *)store_at(to + 2 * C, spare, wanted) = M::frag(dv[c] * kDown<T>);
+            *(Frag *)store_at(to + C, spare, wanted) = cleared<T>(M::frag(acc[c] * to_dk), !padding);
+            *(Frag *)store_at(to + 2 * C, spare, wanted) = cleared<T>(M::frag(dv[c] * kDown<T>), !padding);
         }
         if (first_wave) spotter.write(spots[after], coming);
         now = next;

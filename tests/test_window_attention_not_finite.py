@@ -1,5 +1,5 @@
-"""artemis_amd.window_attention beside infinities: what the slots that a window leaves empty, and padding, must not turn
-them into.  (Windows of 17 to 63 tokens leave slots of their tile empty, longer ones of their last tile.)"""
+"""artemis_amd.window_attention beside infinities and NaN: what the slots that a window leaves empty, and padding, must not
+turn them into.  (Windows of 17 to 63 tokens leave slots of their tile empty, longer ones of their last tile.)"""
 import math
 
 import pytest
@@ -87,3 +87,22 @@ def test_a_query_that_sees_nothing(window, dtype, padded):
     want = ref.window_attention(qkv.flatten(4), table, window, 2, labels=labels)["out"][0]
     got[0].data[0, 0, 0, 0, 32:] = want[0, 0, 0, 0, 32:].to(got[0])
     check(got, qkv, table, window, dout, labels, but)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("window", [(3, 1, 1), (1, 5, 5), (1, 8, 8), (1, 9, 8)])
+@pytest.mark.parametrize("part", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("value", [INF, math.nan])
+def test_padding_beside_what_is_not_finite(window, dtype, part, value):
+    """Its output and gradients are 0 all the same."""
+    qkv, table, dout = data(window, dtype, 73)
+    if part == "dout":
+        dout[0, 0, 0, 0] = value
+    else:
+        qkv[0, 0, 0, 0, "qkv".index(part)] = value
+    labels = some_padding(window, True)
+    out, dqkv, _ = run(qkv, table, window, dout, labels)
+    pad = (labels < 0).to(DEV).expand(2, *labels.shape)
+    assert (out[pad] == 0).all() and (dqkv[pad] == 0).all()
+    assert not dqkv[0].isfinite().all()
