@@ -91,6 +91,18 @@ variable_list once(variable_list grads)
     return grads;
 }
 
+// The gradient node of the leaf that an edge leads to, itself or through copies: a parameter that was widened, an input that
+// was realigned (below), or what a caller cast.
+torch::autograd::AccumulateGrad *leaf_behind(const torch::autograd::Edge &edge)
+{
+    for (auto *node = edge.function.get(); node; node = node->next_edge(0).function.get()) {
+        if (auto *leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(node)) return leaf;
+        const std::string name = node->name();
+        if (node->num_outputs() != 1 || (name != "ToCopyBackward0" && name != "CloneBackward0")) return nullptr;
+    }
+    return nullptr;
+}
+
 // A leaf's gradient node is made with the first graph that has the leaf and lives with it.  Where that was on the default
 // stream and is alive, a backward pass under capture makes torch wait for the capture on the default stream, which ends the
 // capture, and may end the process: refused here, in front of that.
@@ -100,7 +112,7 @@ void no_outside_graph()
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
     for (const auto &edge : node->next_edges()) {
-        auto *leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get());
+        auto *leaf = leaf_behind(edge);
         if (!leaf) continue;
         const auto stream = leaf->stream();
         TORCH_CHECK(!stream || stream->id() != 0, "this backward pass is being captured while a graph of the same tensors that "
@@ -419,4 +431,6 @@ PYBIND11_MODULE(_artemis_ops, m)
     m.def("window_attention", &window_attention);
     m.def("adamw", &adamw);
     m.def("moments_from_8bit", &moments_from_8bit);
+    // whether the tensor is a leaf that wants a gradient, or a copy of one, as a captured backward pass looks for it
+    m.def("has_leaf", [](const at::Tensor &t) { return leaf_behind(torch::autograd::impl::gradient_edge(t)) != nullptr; });
 }
