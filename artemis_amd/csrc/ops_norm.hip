@@ -325,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_wide(const T *__restrict__ 
     }
 }
 
-// dw and db from the workgroups' shares: 16 columns for a workgroup, 64 threads on each, joined in order.  (16 threads
+// dw and db from the workgroups' shares: 16 columns at a time for a workgroup, 64 threads on each, joined in order.  (16 threads
 // on each: 17 us for 1024 shares of 2 x 64 columns, all of it waiting for 64 loads in a row.)
 constexpr int kFold = 1024;
 __global__ __launch_bounds__(kFold) void norm_fold(const float *__restrict__ partial, float *__restrict__ dw,
@@ -333,22 +333,25 @@ __global__ __launch_bounds__(kFold) void norm_fold(const float *__restrict__ par
 {
     __shared__ float fold[kFold / 16][17];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long long c = (long long)blockIdx.x * 16 + tx;  // of 2 * cols
-    float s = 0.f;
-    if (c < 2LL * cols) {
+    for (long long first = blockIdx.x * 16LL; first < 2LL * cols; first += gridDim.x * 16LL) {
+        const long long c = first + tx;  // of 2 * cols
+        float s = 0.f;
+        if (c < 2LL * cols) {
 #pragma unroll 8
-        for (int p = ty; p < parts; p += kFold / 16) s += partial[(size_t)p * 2 * cols + c];
-    }
-    fold[ty][tx] = s;
-    __syncthreads();
-    if (threadIdx.x < 16 && c < 2LL * cols) {
-        float t = 0.f;
-        for (int k = 0; k < kFold / 16; ++k) t += fold[k][tx];
-        if (c < cols) {
-            if (dw) dw[c] = t;
-        } else if (db) {
-            db[c - cols] = t;
+            for (int p = ty; p < parts; p += kFold / 16) s += partial[(size_t)p * 2 * cols + c];
         }
+        fold[ty][tx] = s;
+        __syncthreads();
+        if (threadIdx.x < 16 && c < 2LL * cols) {
+            float t = 0.f;
+            for (int k = 0; k < kFold / 16; ++k) t += fold[k][tx];
+            if (c < cols) {
+                if (dw) dw[c] = t;
+            } else if (db) {
+                db[c - cols] = t;
+            }
+        }
+        __syncthreads();  // the sums have been read
     }
 }
 
@@ -391,6 +394,13 @@ unsigned fwd_blocks(long long rows, int rows_at_once)
 {
     const long long need = (rows + rows_at_once - 1) / rows_at_once;
     return (unsigned)(need < (1 << 22) ? need : (1 << 22));
+}
+
+// 16 columns for each workgroup of norm_fold, up to 2^20 of them (a launch has at most 2^32 threads)
+unsigned fold_blocks(long long cols)
+{
+    const long long need = (2 * cols + 15) / 16;
+    return (unsigned)(need < (1 << 20) ? need : (1 << 20));
 }
 
 template <class T, class F>
@@ -445,8 +455,7 @@ int run_bwd(const void *x, const void *dy, const float *w, const float *mean, co
         hipLaunchKernelGGL((norm_bwd_wide<T>), dim3(parts), dim3(kThreads), 0, st, (const T *)x, (const T *)dy, w,
                            mean, rstd, (T *)dx, partial, rows, cols);
     if (partial)
-        hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2LL * cols + 15) / 16)), dim3(kFold), 0, st, partial,
-                           dw, db, parts, cols);
+        hipLaunchKernelGGL(norm_fold, dim3(fold_blocks(cols)), dim3(kFold), 0, st, partial, dw, db, parts, cols);
     return check_launch("artemis_ops_layer_norm_backward");
 }
 
@@ -505,8 +514,8 @@ int artemis_ops_layer_norm_backward(const void *x, const void *dy, const float *
     const bool sums = dweight || dbias;
     if (rows == 0) {  // sums over nothing
         if (sums)
-            hipLaunchKernelGGL(norm_fold, dim3((unsigned)((2 * cols + 15) / 16)), dim3(kFold), 0, st,
-                               (const float *)nullptr, dweight, dbias, 0, (int)cols);
+            hipLaunchKernelGGL(norm_fold, dim3(fold_blocks(cols)), dim3(kFold), 0, st, (const float *)nullptr, dweight, dbias, 0,
+                               (int)cols);
         return check_launch(what);
     }
     if (!x || !dy || !mean || !rstd) return fail(hipErrorInvalidValue, "%s: NULL tensor pointer", what);
