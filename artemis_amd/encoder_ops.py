@@ -41,5 +41,10 @@ def window_attention(qkv, bias_table, window, num_heads, *, shift=(0, 0, 0), lab
                 a cut video, say); tokens of a negative label are padding: not read, not attended to, output 0
     outside     added to the scores of tokens of different regions: the reference's -100, or -inf for never
     scale       of q k^T; head_dim ** -0.5 by default
+
+    Sizes: B * D * H * W below 2^31; windows * heads below 2^30, in windows of more than 64 tokens windows * heads *
+    ceil(tokens / 64) below 2^24.  The gradient of bias_table in windows of n > 64 tokens that runs of 64 do not tile
+    evenly takes heads * n * n * 4 bytes of memory during the backward pass, times the shares where windows are many and
+    short (16 heads of 62 x 62 tokens: 0.95 GB).
     """
     return _lib.load_ops_host().window_attention(qkv, bias_table, window, num_heads, shift, labels, outside, scale)

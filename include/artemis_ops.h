@@ -38,7 +38,7 @@ extern "C" {
  * var the mean of the squared deviations.  x and y are (rows, cols) contiguous of `dtype`, weight and
  * bias (either may be NULL: 1 and 0) fp32.  mean and rstd (rows each, fp32) are written for the backward
  * pass; both may be NULL.  Reference: nn.LayerNorm in model/sep_sts_layer.py:251,257.
- * cols >= 1 where rows > 0; rows and cols below 2^31. */
+ * cols >= 1 where rows > 0; rows below 2^31, cols below 2^30. */
 int artemis_ops_layer_norm_forward(const void *x, const float *weight, const float *bias, void *y,
                                    float *mean, float *rstd, long long rows, long long cols, float eps,
                                    int dtype, void *stream);
@@ -70,8 +70,15 @@ size_t artemis_ops_layer_norm_workspace_bytes(long long rows, long long cols, in
  *   out    (B, D, H, W, heads, head_dim) of `dtype`
  *   lse    fp32, artemis_ops_window_attention_lse_count elements: what the backward pass needs of the
  *          rows' softmax; may be NULL for a forward pass alone, and where the count is 0.
- * Limits: heads at most 1024; head_dim a multiple of 4, at most 128; wd*wh*ww at most 4096; D, H, W multiples of the window;
- * 0 <= shift < window; B*D*H*W and windows * heads below 2^31.
+ * Limits: heads at most 1024; head_dim a multiple of 4, at most 128; n = wd*wh*ww at most 4096; D, H, W multiples of the
+ * window; 0 <= shift < window; B*D*H*W below 2^31; windows * heads below 2^30 for n <= 64, windows * heads * ceil(n / 64)
+ * below 2^24 for longer windows.  The size functions return 0 for what is refused.
+ * Workspace: 1 KB for n <= 64, with dtable some 12 MB, or 144 KB for each head where that is more.  Longer windows: 20 bytes a
+ * token, two copies of the table, in a backward pass 4 bytes a token and head; where there are fewer than 1024 tiles of 64
+ * tokens and a head, up to 1024 * 64 * (head_dim + 2) * 4 bytes (backward: twice that) for their shares.  With dtable the
+ * sums of dS: heads * n * n * 4 bytes where runs of 64 tokens do not tile the window evenly (16 heads of 3844 tokens: 946 MB),
+ * 16 KB for each head and distance of two tiles where they do, both for as many shares of the windows as make about 1024
+ * workgroups.
  * Reference: model/sep_sts_layer.py:108-219 (attention), :262-337 (shift and mask). */
 typedef struct artemis_ops_window {
     int B, D, H, W;
