@@ -89,7 +89,9 @@ class HeadTrainer:
                  seed=103, fused=True, encoder_ops="torch", optimizer="adamax", weight_decay=1e-2):
         torch.manual_seed(seed)          # config.py:62; same init on every rank
         self.device = device
-        self.module = self.build(num_features, fused, encoder_ops).to(device)
+        # (a subclass's build may take two arguments, as it did before there was a choice)
+        kinds = {} if encoder_ops == "torch" else {"encoder_ops": encoder_ops}
+        self.module = self.build(num_features, fused, **kinds).to(device)
         self.world = torch.distributed.get_world_size() if torch.distributed.is_initialized() else 1
         self.rank = torch.distributed.get_rank() if self.world > 1 else 0
         self.model = self.module
