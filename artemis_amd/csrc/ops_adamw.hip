@@ -140,8 +140,8 @@ __global__ __launch_bounds__(kThreads) void adamw32(const Batch<Tensor32> b, con
     }
 }
 
-// 32 random bits from a counter: two rounds of multiplication by odd constants (32 bits of the fractions of
-// sqrt 2 and sqrt 3) between shifts, so that every bit of the counter reaches every bit of the result.
+// 32 random bits from a counter: two rounds of multiplication by odd constants (the first 32 bits of the fraction of
+// sqrt 2; those of sqrt 3 but for the first) between shifts, so that every bit of the counter reaches every bit of the result.
 __device__ __forceinline__ unsigned noise(unsigned counter)
 {
     unsigned z = counter;

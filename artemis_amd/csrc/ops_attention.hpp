@@ -366,10 +366,14 @@ __device__ __forceinline__ void over_tokens_both(f32x4 (&x)[HD / 16], f32x4 (&y)
 // blocks of the unit.  A workgroup keeps one head and goes through tiles, so that the bias of its pairs stays in registers
 // (-inf where a pair is of two windows or of empty slots).
 // Bound by memory where windows are small or 16 bit, by memory and products together in fp32 at 64 tokens: 8192 windows with 2
-// heads of 32 channels take 138 us forward (537 MB at 3.9 TB/s) and 320 backward (940 MB at 2.9 TB/s; its products alone 136 on
-// the matrix cores); 131072 tokens in windows of 4, 4 heads: 68 us (3.9 TB/s) and 97 (4.8 TB/s); bf16, 8160 shifted windows of 64,
-// 4 heads, forward: 134 us (4.0 TB/s).  Registers for 3 and 4 waves on a SIMD were slower (spills), as was reading the operands
-// of the next products ahead of those at hand (150 us forward).
+// heads of 32 channels take 124 us forward (537 MB at 4.3 TB/s) and 288 backward (940 MB at 3.3 TB/s; matrix units busy for half
+// of it, a quarter of the waves' time spent waiting), in bf16 71 (3.8 TB/s) and 151 (3.1); 131072 tokens in windows of 4, 4
+// heads: 70 us (3.8 TB/s) and 95 (4.9); bf16, 8160 shifted windows of 64, 4 heads, forward: 140 us (3.8 TB/s).  (Kernels alone, by
+// a trace of 200 passes.)  Registers for 3 and 4 waves on a SIMD were slower (spills), as was reading the operands of the
+// next products ahead of those at hand (by 8 %).
+// P (16 bit, and dS) is rounded to the type as the operand of a product that matrix instructions take, its sum is of the
+// unrounded ones.  Outputs then lie 0.0023 of their size (bf16) from the definition instead of the 0.0017 that their own rounding
+// makes; two operands, the rounded one and what is left of it, would double those products and their conversions.
 // ================================================================================================
 
 // the head and first tile of a workgroup, and its step.  Workgroups 8 apart run on one XCD; the heads of a tile,
@@ -926,14 +930,16 @@ __global__ __launch_bounds__(kAttnThreads, (kWaves<T, HD>)) void window_bwd(cons
 
 // ================================================================================================
 // Longer windows (65 .. 4096 tokens): tiles of 64 queries against tiles of 64 keys, with the running maximum and sum
-// of a softmax over the key tiles.  A head's scores take about nine vector instructions for each pair beside its
-// products (scale and bias, maximum, exponential, sum, rounding), against 4 hd / 1024 matrix instructions: for the
-// model's 32 channels the vector units bound it, so the pair loop holds nothing else --
+// of a softmax over the key tiles.  A head's scores take about eleven vector instructions for each pair beside its
+// products (scale and bias, maximum, exponential, sum, rounding), against 4 hd / 1024 matrix instructions: with the
+// model's 32 channels the vector units are busy for half of the forward pass (a third to two fifths of dQ, dK and dV, a quarter of
+// the table's gradient), the matrix units for a tenth, and waves wait a third of their time, at the two barriers of a
+// tile above all.  So the pair loop holds nothing else --
 //  * where tokens lie and what region they are of is written once for each call (`places`, `tiles`): a pair of
 //    tiles of one region needs no mask, one of two regions that never meet is skipped with its loads;
 //  * the bias comes from a copy of the table with one head's entries in a row, forwards and backwards, so that four
-//    neighbouring keys (or queries) have neighbouring entries: one load of 16 bytes where rows of the window are
-//    multiples of 4;
+//    neighbouring keys (or queries) have neighbouring entries: a pair of tiles needs one run of it, which goes through LDS,
+//    where rows of the window are multiples of 4;
 //  * the next tile's rows are in flight while this one is used, and what is contracted over tokens lies in LDS
 //    transposed, so that an operand is one read.
 // ================================================================================================

@@ -7,7 +7,10 @@ learned relative-position bias and region masks.
 
 As for the synthesis op: tensors on a HIP device, contiguous (asserted), on torch's current stream; CPU
 tensors raise ``NotImplementedError``; no fallback.  fp32, bf16 and fp16; sums, softmax statistics and
-parameter gradients are fp32 whatever the type.  No atomics: results are the same bits in every run.  Every
+parameter gradients are fp32 whatever the type.  In bf16 and fp16 the attention's probabilities, and in the backward pass
+dS = P (dP - delta), are rounded to the type as operands of the products with V, dout, Q and K, once each (in fp16 scaled, so
+that they lie in its normal range): outputs and gradients are off by about 1.4 times what rounding them alone would be.  No
+atomics: results are the same bits in every run.  Every
 call only enqueues kernels, so it can be captured into a HIP graph -- a backward pass while no graph of the same
 leaves that was made on the default stream is alive (refused).  First derivatives only.  The host side of a
 call (checks, memory, autograd) is csrc/ops_torch.cpp.
